@@ -69,7 +69,7 @@ extern "C" {
 
 /* ABI version of this header.  A TUNING build of the library (measurement arms compiled in: -DGS_TUNING_BUILD=1,
  * tools/build_variants.sh) reports GS_ABI_VERSION + GS_ABI_TUNING_OFFSET, which the product loader refuses. */
-#define GS_ABI_VERSION 36
+#define GS_ABI_VERSION 37
 #define GS_ABI_TUNING_OFFSET 1000
 
 const char *gs_last_error(void);
@@ -657,6 +657,59 @@ int gs_adam_step_features(float *features, const float *grad, float *exp_avg, fl
 int gs_adam_step_rows(float *param, const float *grad, float *exp_avg, float *exp_avg_sq, long long n_rows, int row_len,
                       double lr, double beta1, double beta2, double eps, int step, const int8_t *point_invalid_mask,
                       int32_t *last_step, double scale_regulariser_weight, int32_t *workspace, void *stream);
+
+/* ---------------------------------------------------------------- AdamW over many tensors
+ * The arrays named host_* hold one entry per tensor and are HOST memory (read before the call returns); the addresses in
+ * them are device addresses.  A tensor is numel consecutive elements of type dtype (GS_DTYPE_*).
+ *
+ * Moments in 32 bits: float[numel] each.  Moments in 8 bits (host_exponents given): uint8[numel] each plus two exponent
+ * bytes per block, uint8[blocks][2] = {X_m, X_v}.  A block is a row when host_row_len[i] = 1..64 (numel = rows * row_len),
+ * else (row_len 0) 64 consecutive elements, the last block shorter.  What the bytes stand for:
+ *   first moment:  c = 128 s + a:  (-1)^s * (a < 8 ? a 2^-9 : 2^((a >> 3) - 7) (1 + (a & 7) / 8)) * 2^(X_m - 135)
+ *   second moment: c = 0: 0, else 2^(c >> 3) (1 + (c & 7) / 8) * 2^(X_v - 158)
+ * X = 255: every element of the block is NaN.  X_m below 9 counts as 9, X_v below 32 as 32. */
+#define GS_DTYPE_F32 0
+#define GS_DTYPE_BF16 1
+#define GS_DTYPE_F16 2
+
+/* One AdamW step (decoupled weight decay), in place, of n_tensors tensors: with t the tensor's step count (1-based),
+ * c = *grad_scale (device float, null = 1) and g the gradient times c
+ *   m += (1 - beta1) (g - m);  v = beta2 v + (1 - beta2) g g
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * p is the parameter (rounded once to its type), or the float master copy where host_master has one (the parameter is then
+ * only written).  8-bit moments are rounded to the upper or the lower neighbour at random so that their mean is kept
+ * (bits: a hash of seed, host_tensor_id[i], t and the element's index); a second moment over zero stays over zero.
+ *   host_hyper[i]   : {lr, beta1, beta2, eps, weight_decay}
+ *   host_step[i]    : t;  host_step_device (nullable, entries too): device int64 that holds t instead
+ *   host_lr_device  : (nullable, entries too) device float that holds lr instead
+ *   host_row_mask   : (nullable, entries too; float tensors with row_len 1..64) int8[rows]: rows with a value other than 0
+ *                     are neither read nor written; host_last_step[i] int32[rows] = the last step that updated the row, a
+ *                     row that missed d steps starts from m beta1^d, v beta2^d
+ *   workspace       : gs_adamw_workspace_bytes(n_tensors), needed where host_step_device or host_lr_device is given
+ * No written range may overlap another range of the call. */
+long long gs_adamw_workspace_bytes(int n_tensors);
+int gs_adamw_step(int n_tensors, const uint64_t *host_param, const uint64_t *host_grad, const uint64_t *host_exp_avg,
+                  const uint64_t *host_exp_avg_sq, const uint64_t *host_exponents, const uint64_t *host_master,
+                  const uint64_t *host_row_mask, const uint64_t *host_last_step, const int64_t *host_numel,
+                  const int32_t *host_row_len, const int32_t *host_dtype, const int32_t *host_tensor_id,
+                  const double *host_hyper, const int64_t *host_step, const uint64_t *host_step_device,
+                  const uint64_t *host_lr_device, const float *grad_scale, uint32_t seed, void *workspace, void *stream);
+
+/* Values of 8-bit moments: host_m_out / host_v_out are buffers of numel elements of type out_dtype (GS_DTYPE_F32 or
+ * GS_DTYPE_BF16: both hold every value exactly). */
+int gs_read_moments(int n_tensors, const uint64_t *host_exp_avg, const uint64_t *host_exp_avg_sq,
+                    const uint64_t *host_exponents, const uint64_t *host_m_out, const uint64_t *host_v_out,
+                    const int64_t *host_numel, const int32_t *host_row_len, int out_dtype, void *stream);
+
+/* 2-norm of the gradients of many tensors, added up in double precision in a fixed order.  host_row_mask / host_row_len
+ * (nullable): rows with a mask other than 0 do not count.  Written: sq_sum double[1] (sum of squares), norm float[1],
+ * clip float[1] = min(1, max_norm / (norm + 1e-6)) (1 where max_norm <= 0), each float[n_tensors] (nullable) the tensors'
+ * own norms.  gs_clip_coefficient: norm and clip from a sum of squares (of several ranks, added up by the caller). */
+long long gs_grad_norm_workspace_bytes(int n_tensors);
+int gs_grad_norm(int n_tensors, const uint64_t *host_grad, const uint64_t *host_row_mask, const int64_t *host_numel,
+                 const int32_t *host_row_len, const int32_t *host_dtype, double max_norm, double *sq_sum, float *norm,
+                 float *clip, float *each, void *workspace, void *stream);
+int gs_clip_coefficient(const double *sq_sum, double max_norm, float *norm, float *clip, void *stream);
 
 #ifdef __cplusplus
 }

@@ -17,7 +17,7 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # GS_LIB_PATH: development knob (tuning sweeps load differently built variants of the library); default = in-tree build
 LIB_PATH = os.environ.get("GS_LIB_PATH") or os.path.join(_HERE, "libgsplat_hip.so")
-ABI_VERSION = 36
+ABI_VERSION = 37
 ABI_TUNING_OFFSET = 1000   # a tuning build of the library (measurement arms compiled in) reports ABI_VERSION + this
 
 _c = ctypes
@@ -88,6 +88,12 @@ _SIGNATURES = {
                                    _I, _P, _c.c_double, _P, _P]),
     "gs_adam_step_rows": (_I, [_P, _P, _P, _P, _c.c_longlong, _I, _c.c_double, _c.c_double, _c.c_double, _c.c_double, _I,
                            _P, _P, _c.c_double, _P, _P]),
+    "gs_adamw_workspace_bytes": (_c.c_longlong, [_I]),
+    "gs_adamw_step": (_I, [_I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _c.c_uint32, _P, _P]),
+    "gs_read_moments": (_I, [_I, _P, _P, _P, _P, _P, _P, _P, _I, _P]),
+    "gs_grad_norm_workspace_bytes": (_c.c_longlong, [_I]),
+    "gs_grad_norm": (_I, [_I, _P, _P, _P, _P, _P, _c.c_double, _P, _P, _P, _P, _P, _P]),
+    "gs_clip_coefficient": (_I, [_P, _c.c_double, _P, _P, _P]),
     "gs_controller_accumulate": (_I, [_P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _P, _P]),
     "gs_ellipsoid_offsets": (_I, [_P, _I, _P, _P]),
     "gs_sample_from_points": (_I, [_P, _P, _P, _I, _P, _P]),

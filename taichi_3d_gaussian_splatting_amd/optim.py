@@ -4,11 +4,20 @@ Same update rule, hyper-parameter names, ``param_groups`` and ``state_dict`` lay
 ``exp_avg_sq``) as ``torch.optim.Adam`` without weight decay / amsgrad -- what the reference instantiates at
 GaussianPointTrainer.py:126-129 -- so learning-rate schedulers and checkpoints work unchanged.  The step itself is one
 streaming HIP kernel per tensor (csrc/gs_optim.hip); there is no CPU path.
+
+``AdamW`` (decoupled weight decay) steps many tensors in one launch, with moments in 32 or in 8 bits, clips by the global
+norm of the gradients on the way and steps 16-bit parameters through a float32 master copy (csrc/gs_adamw.hip).  Its parts
+are functions on lists of tensors: ``adamw_step_``, ``grad_norm``, ``read_moments``, ``new_moments``.
 """
 from __future__ import annotations
 
+import contextlib
+from array import array
+from typing import List, Optional, Sequence, Tuple, Union
+
 import torch
 
+from . import _lib
 from ._lib import call, current_stream, ptr
 
 
@@ -100,3 +109,468 @@ class Adam(torch.optim.Optimizer):
                      float(group["lr"]), float(beta1), float(beta2), float(group["eps"]), state["step"],
                      current_stream(p.device))
         return loss
+
+
+# ---------------------------------------------------------------------------------------------- AdamW over many tensors
+MOMENT_BLOCK = 64        # elements that share the exponents of their 8-bit moments (a row of at most 64, where there are rows)
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}     # GS_DTYPE_*
+Scalar = Union[float, torch.Tensor]
+
+
+def _row_length(shape) -> int:
+    """Columns of a two-dimensional tensor whose rows are blocks (1..64 columns), else 0: blocks of 64 elements."""
+    return int(shape[1]) if len(shape) == 2 and 1 <= shape[1] <= MOMENT_BLOCK else 0
+
+
+def _num_blocks(shape) -> int:
+    row = _row_length(shape)
+    return int(shape[0]) if row else -(-int(torch.Size(shape).numel()) // MOMENT_BLOCK)
+
+
+def new_moments(param: torch.Tensor, bits: int = 32) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
+    """``(exp_avg, exp_avg_sq, exponents)`` of zeros for ``param``: float32 tensors and None with 32 bits; with 8 bits uint8
+    tensors of codes in the parameter's shape and uint8 ``[blocks, 2]`` exponents (of the first and the second moment).  A
+    block is a row of a two-dimensional parameter with at most 64 columns, else 64 consecutive elements."""
+    if bits == 32:
+        zeros = [torch.zeros(param.shape, dtype=torch.float32, device=param.device) for _ in range(2)]
+        return zeros[0], zeros[1], None
+    if bits != 8:
+        raise ValueError(f"moments in 8 or 32 bits, not {bits}")
+    codes = [torch.zeros(param.shape, dtype=torch.uint8, device=param.device) for _ in range(2)]
+    return codes[0], codes[1], torch.zeros(_num_blocks(param.shape), 2, dtype=torch.uint8, device=param.device)
+
+
+def _same_length(n: int, **lists) -> None:
+    for name, values in lists.items():
+        if values is not None and len(values) != n:
+            raise ValueError(f"{name}: {len(values)} entries for {n} tensors")
+
+
+def _check(name: str, tensors, dtype, shapes, device_index: int) -> None:
+    """Every tensor (None entries apart) is contiguous, of the type and shape asked for and on the device."""
+    for i, (t, shape) in enumerate(zip(tensors, shapes)):
+        if t is None:
+            continue
+        if t.get_device() != device_index:
+            raise RuntimeError(f"{name}[{i}] is on {t.device}: all tensors of a call belong on one HIP device")
+        if t.dtype is not (dtype if type(dtype) is torch.dtype else dtype[i]):
+            raise TypeError(f"{name}[{i}] is {t.dtype}, not {dtype if type(dtype) is torch.dtype else dtype[i]}")
+        if t.shape != shape:
+            raise ValueError(f"{name}[{i}] has shape {tuple(t.shape)}, not {tuple(shape)}")
+        if not t.is_contiguous():
+            raise ValueError(f"{name}[{i}] is not contiguous")
+
+
+def _one_device(tensors) -> torch.device:
+    device = tensors[0].device
+    if device.type != "cuda":
+        raise RuntimeError("this operator needs tensors on the HIP device: there is no CPU path")
+    return device
+
+
+def _pointers(tensors) -> array:
+    return array("Q", [0 if t is None else t.data_ptr() for t in tensors])
+
+
+def _address(values: Optional[array]):
+    return None if values is None else values.buffer_info()[0]
+
+
+def _on(device: torch.device):
+    """The device made current for a call's launches, if it is not."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _norm_of(grads, shapes, dtypes, row_masks, max_norm: float, each: bool, group=None):
+    """(norm, clip, each | None) of checked gradients, on their device's current stream."""
+    device, n = grads[0].device, len(grads)
+    out = torch.empty(2 + (n if each else 0), dtype=torch.float32, device=device)
+    floats = out.data_ptr()
+    bytes_needed = int(_lib.load().gs_grad_norm_workspace_bytes(n))
+    workspace = torch.empty(1 + (bytes_needed + 7) // 8, dtype=torch.float64, device=device)     # [0]: the sum of squares
+    pointers, numel = _pointers(grads), array("q", [g.numel() for g in grads])
+    rows, types = array("i", [_row_length(s) for s in shapes]), array("i", [_DTYPES[d] for d in dtypes])
+    masks = None if row_masks is None else _pointers(row_masks)
+    with _on(device):
+        stream = current_stream(device)
+        call("gs_grad_norm", n, _address(pointers), _address(masks), _address(numel), _address(rows), _address(types),
+             max_norm, workspace.data_ptr(), floats, floats + 4, floats + 8 if each else None, workspace.data_ptr() + 8, stream)
+        if group is not None:
+            _sum_over_ranks(workspace[:1], group)
+            call("gs_clip_coefficient", workspace.data_ptr(), max_norm, floats, floats + 4, stream)
+    return out[0], out[1], out[2:] if each else None
+
+
+def _sum_over_ranks(value: torch.Tensor, group) -> None:
+    import torch.distributed as dist
+    if dist.get_backend(group) == "nccl":
+        dist.all_reduce(value, group=group)
+        return
+    host = value.cpu()          # other back ends get host memory
+    dist.all_reduce(host, group=group)
+    value.copy_(host)
+
+
+def _check_masks(row_masks, params_or_grads, shapes, device: torch.device) -> None:
+    for i, mask in enumerate(row_masks):
+        if mask is None:
+            continue
+        if _row_length(shapes[i]) == 0:
+            raise ValueError(f"row_masks[{i}]: the tensor has no rows of 1 to {MOMENT_BLOCK} elements")
+    _check("row_masks", row_masks, torch.int8, [s[:1] for s in shapes], device.index)
+
+
+@torch.no_grad()
+def grad_norm(grads: Sequence[torch.Tensor], row_masks: Optional[Sequence[Optional[torch.Tensor]]] = None, *,
+              per_tensor: bool = False):
+    """2-norm of all ``grads`` together (float32 scalar on their device, no host wait); with ``per_tensor`` also the norms of
+    each (float32 ``[len(grads)]``).  float32, bfloat16 and float16 tensors may be mixed; squares are added up in double
+    precision in a fixed order, so equal inputs give equal bits.  ``row_masks``: int8 ``[N]`` (or None) for each tensor; rows
+    ``[N, 1..64]`` with a mask other than 0 do not count, whatever they hold.  An infinite or NaN gradient shows in the norm."""
+    grads = [g if g.is_contiguous() else g.contiguous() for g in grads]
+    if not grads:
+        raise ValueError("grad_norm: no gradients")
+    _same_length(len(grads), row_masks=row_masks)
+    device = _one_device(grads)
+    dtypes, shapes = [g.dtype for g in grads], [g.shape for g in grads]
+    for d in dtypes:
+        if d not in _DTYPES:
+            raise TypeError(f"grad_norm: {d} gradients (float32, bfloat16 or float16 are supported)")
+    _check("grads", grads, dtypes, shapes, device.index)
+    if row_masks is not None:
+        _check_masks(row_masks, grads, shapes, device)
+    norm, _, each = _norm_of(grads, shapes, dtypes, row_masks, 0.0, per_tensor)
+    return (norm, each) if per_tensor else norm
+
+
+@torch.no_grad()
+def adamw_step_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence[torch.Tensor],
+                exp_avg_sqs: Sequence[torch.Tensor], *, step: Union[int, torch.Tensor, Sequence[Union[int, torch.Tensor]]],
+                lr: Union[Scalar, Sequence[Scalar]] = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
+                weight_decay: Union[float, Sequence[float]] = 1e-2,
+                exponents: Optional[Sequence[torch.Tensor]] = None,
+                masters: Optional[Sequence[Optional[torch.Tensor]]] = None,
+                row_masks: Optional[Sequence[Optional[torch.Tensor]]] = None,
+                last_steps: Optional[Sequence[Optional[torch.Tensor]]] = None,
+                max_grad_norm: Optional[float] = None, norm_group=None, grad_scale: Optional[torch.Tensor] = None,
+                seed: int = 0, tensor_ids: Optional[Sequence[int]] = None) -> Optional[torch.Tensor]:
+    """One AdamW step of many tensors in place, as few launches as their types need.  With ``t`` a tensor's step::
+
+        g = grad * clip;  m += (1 - b1) (g - m);  v = b2 v + (1 - b2) g g
+        p = p (1 - lr weight_decay) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+
+    * ``params`` / ``grads``: contiguous tensors on one HIP device, each pair of one type: float32, bfloat16 or float16.
+    * ``exp_avgs`` / ``exp_avg_sqs`` / ``exponents``: as ``new_moments`` makes them -- float32 without exponents, or uint8 codes
+      with them.  8-bit moments are rounded at random so that their mean is kept (a code is 1/16 to 1/8 of its value, far more
+      than a step moves the second moment): the bits are a hash of ``seed``, the tensor's id (``tensor_ids``, else its place in
+      the list), its step and the element, so equal calls give equal results.  A block in which a moment is infinite or NaN
+      becomes NaN as a whole.
+    * ``masters``: float32 copies (or None) of 16-bit parameters; the step runs on the copy and the parameter receives its
+      rounded value.  Without a copy the parameter itself is rounded to nearest, and steps below half its spacing are lost.
+    * ``step``: this step's number (from 1), or a device tensor (int64, one element) that holds it when the kernels run;
+      ``lr``: a number or a device tensor (float32, one element); each for all tensors or one per tensor.  While a graph is
+      captured ``step`` has to be a tensor: a number would be the same at every replay.
+    * ``row_masks`` / ``last_steps``: for float32 tensors ``[N, 1..64]``, int8 ``[N]`` and int32 ``[N]``: rows with a mask
+      other than 0 are neither read nor written, and a row that missed ``d`` steps starts from ``m b1^d``, ``v b2^d``.
+    * ``max_grad_norm``: gradients are scaled by ``min(1, max_grad_norm / (norm + 1e-6))`` as they are read; the norm is that of
+      all gradients of the call (masked rows apart), over all ranks of ``norm_group`` where one is given, and is returned as a
+      float32 scalar on the device.  ``grads`` themselves stay as they are.
+    * ``grad_scale``: a float32 device scalar to multiply the gradients with instead.
+
+    Nothing waits for the device (but for a ``norm_group`` whose back end takes host memory).  Written buffers must not
+    overlap anything else in the call."""
+    n = len(params)
+    _same_length(n, grads=grads, exp_avgs=exp_avgs, exp_avg_sqs=exp_avg_sqs, exponents=exponents, masters=masters,
+                 row_masks=row_masks, last_steps=last_steps, tensor_ids=tensor_ids)
+    if (row_masks is None) != (last_steps is None):
+        raise ValueError("row_masks and last_steps come together")
+    if max_grad_norm is not None and not max_grad_norm > 0:
+        raise ValueError("max_grad_norm must be positive (None: no clipping)")
+    if max_grad_norm is not None and grad_scale is not None:
+        raise ValueError("max_grad_norm and grad_scale exclude each other")
+    beta1, beta2 = betas
+    if not (0 <= beta1 < 1 and 0 <= beta2 < 1 and eps >= 0):
+        raise ValueError("invalid AdamW hyper-parameters")
+    if n == 0:
+        if max_grad_norm is not None:
+            raise ValueError("the norm of no gradients")
+        return None
+    device = _one_device(params)
+    index = device.index
+    shapes, dtypes = [p.shape for p in params], [p.dtype for p in params]
+    for d in dtypes:
+        if d not in _DTYPES:
+            raise TypeError(f"AdamW steps float32, bfloat16 and float16 parameters, not {d}")
+    grads = [g if g.is_contiguous() else g.contiguous() for g in grads]
+    _check("params", params, dtypes, shapes, index)
+    _check("grads", grads, dtypes, shapes, index)
+    moment_type = torch.float32 if exponents is None else torch.uint8
+    _check("exp_avgs", exp_avgs, moment_type, shapes, index)
+    _check("exp_avg_sqs", exp_avg_sqs, moment_type, shapes, index)
+    if exponents is not None:
+        _check("exponents", exponents, torch.uint8, [(_num_blocks(s), 2) for s in shapes], index)
+    if masters is not None:
+        if any(c is not None and d is torch.float32 for c, d in zip(masters, dtypes)):
+            raise ValueError("a float32 parameter is its own master copy")
+        _check("masters", masters, torch.float32, shapes, index)
+    if row_masks is not None:
+        _check_masks(row_masks, params, shapes, device)
+        for i, (mask, stamp) in enumerate(zip(row_masks, last_steps)):
+            if (mask is None) != (stamp is None):
+                raise ValueError(f"row_masks[{i}] and last_steps[{i}] come together")
+            if mask is not None and dtypes[i] is not torch.float32:
+                raise TypeError(f"row_masks[{i}]: row masks are for float32 parameters")
+        _check("last_steps", last_steps, torch.int32, [s[:1] for s in shapes], index)
+    if grad_scale is not None and (grad_scale.get_device() != index or grad_scale.dtype is not torch.float32 or grad_scale.numel() != 1):
+        raise ValueError("grad_scale: one float32 on the parameters' device")
+
+    steps = list(step) if isinstance(step, (list, tuple)) else [step] * n
+    rates = list(lr) if isinstance(lr, (list, tuple)) else [lr] * n
+    decays = list(weight_decay) if isinstance(weight_decay, (list, tuple)) else [weight_decay] * n
+    _same_length(n, step=steps, lr=rates, weight_decay=decays)
+    step_tensors, step_numbers = _device_scalars("step", steps, torch.int64, index, 1)
+    rate_tensors, rate_numbers = _device_scalars("lr", rates, torch.float32, index, 0.0)
+    if step_tensors is None or 0 in step_tensors:
+        if min(s for s, t in zip(step_numbers, step_tensors or [0] * n) if t == 0) < 1:
+            raise ValueError("step counts from 1")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a captured step needs its step count in a device tensor: a number would be the same at every replay")
+    if min(rate_numbers) < 0 or min(decays) < 0:
+        raise ValueError("invalid AdamW hyper-parameters")
+
+    norm = clip = None
+    if max_grad_norm is not None:
+        norm, clip, _ = _norm_of(grads, shapes, dtypes, row_masks, float(max_grad_norm), False, norm_group)
+    elif grad_scale is not None:
+        clip = grad_scale
+    hyper = array("d")
+    for rate, decay in zip(rate_numbers, decays):
+        hyper.extend((rate, beta1, beta2, eps, decay))
+    columns = [_pointers(t) if t is not None else None
+               for t in (params, grads, exp_avgs, exp_avg_sqs, exponents, masters, row_masks, last_steps)]
+    numel = array("q", [s.numel() for s in shapes])
+    rows = array("i", [_row_length(s) for s in shapes])
+    types = array("i", [_DTYPES[d] for d in dtypes])
+    ids = array("i", range(n) if tensor_ids is None else tensor_ids)
+    counts = array("q", step_numbers)
+    workspace = None
+    if step_tensors is not None or rate_tensors is not None:
+        workspace = torch.empty(int(_lib.load().gs_adamw_workspace_bytes(n)), dtype=torch.uint8, device=device)
+    with _on(device):
+        call("gs_adamw_step", n, *[_address(c) for c in columns], _address(numel), _address(rows), _address(types), _address(ids),
+             _address(hyper), _address(counts), _address(step_tensors), _address(rate_tensors),
+             None if clip is None else clip.data_ptr(), seed & 0xFFFFFFFF,
+             None if workspace is None else workspace.data_ptr(), current_stream(device))
+    return norm
+
+
+def _device_scalars(name: str, values, dtype, device_index: int, stand_in):
+    """(addresses of the device tensors among ``values`` or None, the numbers with ``stand_in`` in the tensors' places)."""
+    if not any(isinstance(v, torch.Tensor) for v in values):
+        return None, values
+    for i, v in enumerate(values):
+        if isinstance(v, torch.Tensor) and (v.get_device() != device_index or v.dtype is not dtype or v.numel() != 1):
+            raise ValueError(f"{name}[{i}]: a number, or one {dtype} on the parameters' device")
+    return (array("Q", [v.data_ptr() if isinstance(v, torch.Tensor) else 0 for v in values]),
+            [stand_in if isinstance(v, torch.Tensor) else v for v in values])
+
+
+@torch.no_grad()
+def read_moments(exp_avgs: Sequence[torch.Tensor], exp_avg_sqs: Sequence[torch.Tensor], exponents: Sequence[torch.Tensor], *,
+                 dtype: torch.dtype = torch.float32, out: Optional[Tuple[Sequence[torch.Tensor], Sequence[torch.Tensor]]] = None
+                 ) -> Tuple[List[torch.Tensor], List[torch.Tensor]]:
+    """The values that 8-bit moments stand for, as two lists of ``dtype`` tensors (float32 or bfloat16: both hold every value
+    exactly) or written to ``out``."""
+    n = len(exp_avgs)
+    _same_length(n, exp_avg_sqs=exp_avg_sqs, exponents=exponents)
+    if n == 0:
+        return [], []
+    device = _one_device(exp_avgs)
+    shapes = [t.shape for t in exp_avgs]
+    if out is None:
+        if dtype not in (torch.float32, torch.bfloat16):
+            raise TypeError("read_moments: float32 or bfloat16 values")
+        out = tuple([torch.empty(s, dtype=dtype, device=device) for s in shapes] for _ in range(2))
+    else:
+        _same_length(n, out_exp_avgs=out[0], out_exp_avg_sqs=out[1])
+        dtype = out[0][0].dtype
+        if dtype not in (torch.float32, torch.bfloat16):
+            raise TypeError("read_moments: float32 or bfloat16 values")
+    _check("exp_avgs", exp_avgs, torch.uint8, shapes, device.index)
+    _check("exp_avg_sqs", exp_avg_sqs, torch.uint8, shapes, device.index)
+    _check("exponents", exponents, torch.uint8, [(_num_blocks(s), 2) for s in shapes], device.index)
+    for k in range(2):
+        _check("out", out[k], dtype, shapes, device.index)
+    columns = [_pointers(t) for t in (exp_avgs, exp_avg_sqs, exponents, out[0], out[1])]
+    numel, rows = array("q", [s.numel() for s in shapes]), array("i", [_row_length(s) for s in shapes])
+    with _on(device):
+        call("gs_read_moments", n, *[_address(c) for c in columns], _address(numel), _address(rows), _DTYPES[dtype],
+             current_stream(device))
+    return list(out[0]), list(out[1])
+
+
+class AdamW(torch.optim.Optimizer):
+    """``torch.optim.AdamW``'s rule (decoupled weight decay, no amsgrad) for float32, bfloat16 and float16 parameters on the
+    HIP device, all of them in one call of ``adamw_step_``.
+
+    * ``state_bits`` (also per group): 32 (float32 moments) or 8 (a code and a share of two exponents each: 2.03 bytes for an
+      element's two moments instead of 8), see ``new_moments``; ``moments(param)`` reads either.
+    * ``master_weights``: 16-bit parameters are stepped through a float32 copy (``state["master"]``).
+    * ``max_grad_norm``: the gradients of all groups are clipped by their global norm; ``last_grad_norm`` holds it (a device
+      scalar) after a step.  ``norm_group``: a process group whose ranks hold different parameters: the norm is that of all.
+    * ``capturable``: step counts live on the device, so a step can be captured into a graph and replayed; ``lr`` may then be a
+      float32 device tensor.  Run one step before the capture: the state is made there.
+    * ``seed``: of the rounding of 8-bit moments.
+
+    ``param_groups`` and the state's ``step`` / ``exp_avg`` / ``exp_avg_sq`` are named as in torch; a state_dict of
+    ``torch.optim.AdamW`` loads into 32-bit moments."""
+
+    def __init__(self, params, lr: Scalar = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *,
+                 state_bits: int = 32, master_weights: bool = True, max_grad_norm: Optional[float] = None, norm_group=None,
+                 capturable: bool = False, seed: int = 0):
+        if (not isinstance(lr, torch.Tensor) and lr < 0) or eps < 0 or weight_decay < 0 or not (0 <= betas[0] < 1 and 0 <= betas[1] < 1):
+            raise ValueError("invalid AdamW hyper-parameters")
+        if state_bits not in (8, 32):
+            raise ValueError(f"moments in 8 or 32 bits, not {state_bits}")
+        if max_grad_norm is not None and not max_grad_norm > 0:
+            raise ValueError("max_grad_norm must be positive (None: no clipping)")
+        if isinstance(lr, torch.Tensor) and not capturable:
+            raise ValueError("a learning rate in a tensor needs capturable=True")
+        self.master_weights, self.max_grad_norm, self.norm_group = bool(master_weights), max_grad_norm, norm_group
+        self.capturable, self.seed = bool(capturable), int(seed)
+        self.last_grad_norm: Optional[torch.Tensor] = None
+        self._row_mask = {}            # id(param) -> point_invalid_mask
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits))
+
+    def set_row_mask(self, param: torch.Tensor, point_invalid_mask: torch.Tensor) -> None:
+        """As ``Adam.set_row_mask``, for any float32 parameter ``[N, 1..64]``: rows marked in the int8 ``[N]`` mask (the live
+        tensor, read at every step) are not touched and do not count in the norm; their moments decay lazily."""
+        if _row_length(param.shape) == 0 or point_invalid_mask.shape != param.shape[:1]:
+            raise ValueError(f"set_row_mask: [N, 1..{MOMENT_BLOCK}] parameter and an [N] mask")
+        if point_invalid_mask.dtype != torch.int8 or param.dtype != torch.float32:
+            raise TypeError("set_row_mask: float32 parameter and int8 mask")
+        self._row_mask[id(param)] = point_invalid_mask
+
+    def _new_state(self, p: torch.Tensor, group: dict) -> dict:
+        m, v, exponents = new_moments(p, group["state_bits"])
+        state = dict(step=torch.zeros((), dtype=torch.int64, device=p.device) if self.capturable else 0, exp_avg=m, exp_avg_sq=v)
+        if exponents is not None:
+            state["exponents"] = exponents
+        if self.master_weights and p.dtype != torch.float32:
+            state["master"] = p.detach().to(torch.float32)
+        return state
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        work = {}           # (state_bits, betas, eps, device) -> columns of adamw_step_
+        place = -1
+        for group in self.param_groups:
+            for p in group["params"]:
+                place += 1
+                if p.grad is None:
+                    continue
+                if p.grad.is_sparse:
+                    raise RuntimeError("AdamW does not take sparse gradients")
+                if not p.is_cuda or not p.is_contiguous():
+                    raise RuntimeError("optim.AdamW needs contiguous parameters on the HIP device")
+                state = self.state[p]
+                mask = self._row_mask.get(id(p))
+                if not state or (mask is not None and "last_step" not in state):
+                    if torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError("run one step of AdamW before capturing one: its state is made there")
+                if not state:
+                    state.update(self._new_state(p, group))
+                if mask is not None and "last_step" not in state:
+                    # moments from a state_dict without row masks are current as of the previous step
+                    state["last_step"] = torch.full((p.shape[0],), int(state["step"]), dtype=torch.int32, device=p.device)
+                if not self.capturable:
+                    state["step"] += 1
+                bits = 8 if "exponents" in state else 32
+                columns = work.setdefault((bits, group["betas"], group["eps"], p.device), tuple([] for _ in range(12)))
+                for column, value in zip(columns, (p, p.grad, state["exp_avg"], state["exp_avg_sq"], state.get("exponents"),
+                                                   state.get("master"), mask, state.get("last_step"), state["step"], group["lr"],
+                                                   group["weight_decay"], place)):
+                    column.append(value)
+        if not work:
+            return loss
+        clip = None
+        if self.max_grad_norm is not None:
+            if len({key[3] for key in work}) > 1:
+                raise RuntimeError("max_grad_norm: all parameters belong on one device")
+            clip = self._clip([column for columns in work.values() for column in [columns]])
+        for (bits, betas, eps, _), columns in work.items():
+            params, grads, ms, vs, exponents, masters, masks, stamps, steps, rates, decays, places = columns
+            if self.capturable:
+                torch._foreach_add_(steps, 1)
+            masked = any(mask is not None for mask in masks)
+            adamw_step_(params, grads, ms, vs, step=steps, lr=rates, betas=betas, eps=eps, weight_decay=decays,
+                        exponents=exponents if bits == 8 else None,
+                        masters=masters if any(c is not None for c in masters) else None,
+                        row_masks=masks if masked else None,
+                        last_steps=[s if mask is not None else None for s, mask in zip(stamps, masks)] if masked else None,
+                        grad_scale=clip, seed=self.seed, tensor_ids=places)
+        return loss
+
+    def _clip(self, parts) -> torch.Tensor:
+        """The clipping coefficient of all gradients (and ``last_grad_norm``)."""
+        grads = [g if g.is_contiguous() else g.contiguous() for columns in parts for g in columns[1]]
+        masks = [mask for columns in parts for mask in columns[6]]
+        dtypes, shapes = [g.dtype for g in grads], [g.shape for g in grads]
+        if any(d not in _DTYPES for d in dtypes):
+            raise TypeError("AdamW steps float32, bfloat16 and float16 parameters")
+        if any(mask is not None for mask in masks):
+            _check_masks(masks, grads, shapes, grads[0].device)
+        else:
+            masks = None
+        self.last_grad_norm, clip, _ = _norm_of(grads, shapes, dtypes, masks, float(self.max_grad_norm), False, self.norm_group)
+        return clip
+
+    def moments(self, param: torch.Tensor, dtype: torch.dtype = torch.float32) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Values of a parameter's first and second moment, whatever they are held in."""
+        state = self.state.get(param)
+        if not state:
+            raise KeyError("the parameter has no state yet")
+        if "exponents" not in state:
+            return state["exp_avg"].to(dtype), state["exp_avg_sq"].to(dtype)
+        m, v = read_moments([state["exp_avg"]], [state["exp_avg_sq"]], [state["exponents"]], dtype=dtype)
+        return m[0], v[0]
+
+    def load_state_dict(self, state_dict) -> None:
+        """As in torch, but the state keeps its own types (torch would cast codes, counts and float32 moments of 16-bit
+        parameters to the parameter's type).  Whether moments have 8 or 32 bits is what was saved."""
+        super().load_state_dict(state_dict)
+        saved = [i for group in state_dict["param_groups"] for i in group["params"]]
+        params = [(p, group) for group in self.param_groups for p in group["params"]]
+        for group in self.param_groups:
+            group.setdefault("state_bits", self.defaults["state_bits"])
+            group["betas"] = tuple(group["betas"])
+        for i, (p, group) in zip(saved, params):
+            held = state_dict["state"].get(i)
+            if not held:
+                continue
+            shapes = {"exp_avg": p.shape, "exp_avg_sq": p.shape, "master": p.shape, "exponents": (_num_blocks(p.shape), 2),
+                      "last_step": p.shape[:1]}
+            eight = "exponents" in held
+            types = {"exp_avg": torch.uint8 if eight else torch.float32, "exponents": torch.uint8, "master": torch.float32,
+                     "last_step": torch.int32}
+            types["exp_avg_sq"] = types["exp_avg"]
+            state = {}
+            for name, value in held.items():
+                if name == "step":
+                    state[name] = torch.full((), int(value), dtype=torch.int64, device=p.device) if self.capturable else int(value)
+                elif name in shapes:
+                    if tuple(value.shape) != tuple(shapes[name]):
+                        raise ValueError(f"state_dict: {name} has shape {tuple(value.shape)}, not {tuple(shapes[name])}")
+                    if eight and name.startswith("exp_avg") and value.dtype != torch.uint8:
+                        raise TypeError(f"state_dict: {name} with exponents is uint8, not {value.dtype}")
+                    state[name] = value.detach().to(device=p.device, dtype=types[name], copy=True).contiguous()
+            if not {"step", "exp_avg", "exp_avg_sq"} <= set(state):
+                raise ValueError("state_dict: no AdamW state")
+            if self.master_weights and p.dtype != torch.float32 and "master" not in state:
+                state["master"] = p.detach().to(torch.float32)
+            group["state_bits"] = 8 if eight else 32
+            self.state[p] = state
