@@ -104,6 +104,7 @@ _SIGNATURES = {
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 
 _lib: Optional[ctypes.CDLL] = None
+_host = None
 HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "gsplat_hip.h")
 
 
@@ -186,6 +187,19 @@ def load() -> ctypes.CDLL:
                                "(include/gsplat_hip.h and the built library disagree)")
         _lib = lib
     return _lib
+
+
+def host():
+    """The CPython module ``_gs_host`` (csrc/gs_host.cpp), built next to the library by the same Makefile; no fallback."""
+    global _host
+    if _host is None:
+        try:
+            from . import _gs_host
+        except ImportError as e:
+            raise RuntimeError(f"_gs_host is missing or does not load ({e}): build it with `make -C {os.path.join(_HERE, 'csrc')}` "
+                               "(or __graft_entry__.build()).  There is no fallback path.") from e
+        _host = _gs_host
+    return _host
 
 
 def ptr(t: Optional[torch.Tensor]):

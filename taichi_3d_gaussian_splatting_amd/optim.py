@@ -13,7 +13,7 @@ from __future__ import annotations
 
 import contextlib
 from array import array
-from typing import List, Optional, Sequence, Tuple, Union
+from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -140,64 +140,27 @@ def new_moments(param: torch.Tensor, bits: int = 32) -> Tuple[torch.Tensor, torc
     return codes[0], codes[1], torch.zeros(_num_blocks(param.shape), 2, dtype=torch.uint8, device=param.device)
 
 
-def _same_length(n: int, **lists) -> None:
-    for name, values in lists.items():
-        if values is not None and len(values) != n:
-            raise ValueError(f"{name}: {len(values)} entries for {n} tensors")
-
-
-def _check(name: str, tensors, dtype, shapes, device_index: int) -> None:
-    """Every tensor (None entries apart) is contiguous, of the type and shape asked for and on the device."""
-    for i, (t, shape) in enumerate(zip(tensors, shapes)):
-        if t is None:
-            continue
-        if t.get_device() != device_index:
-            raise RuntimeError(f"{name}[{i}] is on {t.device}: all tensors of a call belong on one HIP device")
-        if t.dtype is not (dtype if type(dtype) is torch.dtype else dtype[i]):
-            raise TypeError(f"{name}[{i}] is {t.dtype}, not {dtype if type(dtype) is torch.dtype else dtype[i]}")
-        if t.shape != shape:
-            raise ValueError(f"{name}[{i}] has shape {tuple(t.shape)}, not {tuple(shape)}")
-        if not t.is_contiguous():
-            raise ValueError(f"{name}[{i}] is not contiguous")
-
-
-def _one_device(tensors) -> torch.device:
-    device = tensors[0].device
-    if device.type != "cuda":
-        raise RuntimeError("this operator needs tensors on the HIP device: there is no CPU path")
-    return device
-
-
-def _pointers(tensors) -> array:
-    return array("Q", [0 if t is None else t.data_ptr() for t in tensors])
-
-
-def _address(values: Optional[array]):
-    return None if values is None else values.buffer_info()[0]
-
-
-def _on(device: torch.device):
+def _on(device_index: int):
     """The device made current for a call's launches, if it is not."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return contextlib.nullcontext() if torch.cuda.current_device() == device_index else torch.cuda.device(device_index)
 
 
-def _norm_of(grads, shapes, dtypes, row_masks, max_norm: float, each: bool, group=None):
-    """(norm, clip, each | None) of checked gradients, on their device's current stream."""
-    device, n = grads[0].device, len(grads)
+def _norm_of(collected, masks, max_norm: float, each: bool, group=None):
+    """(norm, clip, each | None) of collected gradients, on their device's current stream."""
+    (grads, *_), numel, rows, types, index, _ = collected
+    device, n = torch.device("cuda", index), len(numel) // 8
     out = torch.empty(2 + (n if each else 0), dtype=torch.float32, device=device)
     floats = out.data_ptr()
     bytes_needed = int(_lib.load().gs_grad_norm_workspace_bytes(n))
     workspace = torch.empty(1 + (bytes_needed + 7) // 8, dtype=torch.float64, device=device)     # [0]: the sum of squares
-    pointers, numel = _pointers(grads), array("q", [g.numel() for g in grads])
-    rows, types = array("i", [_row_length(s) for s in shapes]), array("i", [_DTYPES[d] for d in dtypes])
-    masks = None if row_masks is None else _pointers(row_masks)
-    with _on(device):
+    sq_sum = workspace.data_ptr()
+    with _on(index):
         stream = current_stream(device)
-        call("gs_grad_norm", n, _address(pointers), _address(masks), _address(numel), _address(rows), _address(types),
-             max_norm, workspace.data_ptr(), floats, floats + 4, floats + 8 if each else None, workspace.data_ptr() + 8, stream)
+        call("gs_grad_norm", n, grads, masks, numel, rows, types, max_norm, sq_sum, floats, floats + 4,
+             floats + 8 if each else None, sq_sum + 8, stream)
         if group is not None:
             _sum_over_ranks(workspace[:1], group)
-            call("gs_clip_coefficient", workspace.data_ptr(), max_norm, floats, floats + 4, stream)
+            call("gs_clip_coefficient", sq_sum, max_norm, floats, floats + 4, stream)
     return out[0], out[1], out[2:] if each else None
 
 
@@ -211,15 +174,6 @@ def _sum_over_ranks(value: torch.Tensor, group) -> None:
     value.copy_(host)
 
 
-def _check_masks(row_masks, params_or_grads, shapes, device: torch.device) -> None:
-    for i, mask in enumerate(row_masks):
-        if mask is None:
-            continue
-        if _row_length(shapes[i]) == 0:
-            raise ValueError(f"row_masks[{i}]: the tensor has no rows of 1 to {MOMENT_BLOCK} elements")
-    _check("row_masks", row_masks, torch.int8, [s[:1] for s in shapes], device.index)
-
-
 @torch.no_grad()
 def grad_norm(grads: Sequence[torch.Tensor], row_masks: Optional[Sequence[Optional[torch.Tensor]]] = None, *,
               per_tensor: bool = False):
@@ -227,19 +181,11 @@ def grad_norm(grads: Sequence[torch.Tensor], row_masks: Optional[Sequence[Option
     each (float32 ``[len(grads)]``).  float32, bfloat16 and float16 tensors may be mixed; squares are added up in double
     precision in a fixed order, so equal inputs give equal bits.  ``row_masks``: int8 ``[N]`` (or None) for each tensor; rows
     ``[N, 1..64]`` with a mask other than 0 do not count, whatever they hold.  An infinite or NaN gradient shows in the norm."""
-    grads = [g if g.is_contiguous() else g.contiguous() for g in grads]
-    if not grads:
+    if len(grads) == 0:
         raise ValueError("grad_norm: no gradients")
-    _same_length(len(grads), row_masks=row_masks)
-    device = _one_device(grads)
-    dtypes, shapes = [g.dtype for g in grads], [g.shape for g in grads]
-    for d in dtypes:
-        if d not in _DTYPES:
-            raise TypeError(f"grad_norm: {d} gradients (float32, bfloat16 or float16 are supported)")
-    _check("grads", grads, dtypes, shapes, device.index)
-    if row_masks is not None:
-        _check_masks(row_masks, grads, shapes, device)
-    norm, _, each = _norm_of(grads, shapes, dtypes, row_masks, 0.0, per_tensor)
+    host = _lib.host()
+    collected = host.collect(("grads", grads, host.GRADS), ("row_masks", row_masks, host.MASK))
+    norm, _, each = _norm_of(collected, collected[0][1], 0.0, per_tensor)
     return (norm, each) if per_tensor else norm
 
 
@@ -280,8 +226,6 @@ def adamw_step_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], e
     Nothing waits for the device (but for a ``norm_group`` whose back end takes host memory).  Written buffers must not
     overlap anything else in the call."""
     n = len(params)
-    _same_length(n, grads=grads, exp_avgs=exp_avgs, exp_avg_sqs=exp_avg_sqs, exponents=exponents, masters=masters,
-                 row_masks=row_masks, last_steps=last_steps, tensor_ids=tensor_ids)
     if (row_masks is None) != (last_steps is None):
         raise ValueError("row_masks and last_steps come together")
     if max_grad_norm is not None and not max_grad_norm > 0:
@@ -291,122 +235,70 @@ def adamw_step_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], e
     beta1, beta2 = betas
     if not (0 <= beta1 < 1 and 0 <= beta2 < 1 and eps >= 0):
         raise ValueError("invalid AdamW hyper-parameters")
+    if tensor_ids is not None and len(tensor_ids) != n:
+        raise ValueError(f"tensor_ids: {len(tensor_ids)} entries for {n} tensors")
+    host = _lib.host()
+    moment = host.FLOAT if exponents is None else host.CODE
+    collected = host.collect(("params", params, host.PARAM), ("grads", grads, host.GRAD), ("exp_avgs", exp_avgs, moment),
+                             ("exp_avg_sqs", exp_avg_sqs, moment), ("exponents", exponents, host.EXPONENTS),
+                             ("masters", masters, host.MASTER), ("row_masks", row_masks, host.PARAM_MASK),
+                             ("last_steps", last_steps, host.STAMP))
     if n == 0:
         if max_grad_norm is not None:
             raise ValueError("the norm of no gradients")
         return None
-    device = _one_device(params)
-    index = device.index
-    shapes, dtypes = [p.shape for p in params], [p.dtype for p in params]
-    for d in dtypes:
-        if d not in _DTYPES:
-            raise TypeError(f"AdamW steps float32, bfloat16 and float16 parameters, not {d}")
-    grads = [g if g.is_contiguous() else g.contiguous() for g in grads]
-    _check("params", params, dtypes, shapes, index)
-    _check("grads", grads, dtypes, shapes, index)
-    moment_type = torch.float32 if exponents is None else torch.uint8
-    _check("exp_avgs", exp_avgs, moment_type, shapes, index)
-    _check("exp_avg_sqs", exp_avg_sqs, moment_type, shapes, index)
-    if exponents is not None:
-        _check("exponents", exponents, torch.uint8, [(_num_blocks(s), 2) for s in shapes], index)
-    if masters is not None:
-        if any(c is not None and d is torch.float32 for c, d in zip(masters, dtypes)):
-            raise ValueError("a float32 parameter is its own master copy")
-        _check("masters", masters, torch.float32, shapes, index)
-    if row_masks is not None:
-        _check_masks(row_masks, params, shapes, device)
-        for i, (mask, stamp) in enumerate(zip(row_masks, last_steps)):
-            if (mask is None) != (stamp is None):
-                raise ValueError(f"row_masks[{i}] and last_steps[{i}] come together")
-            if mask is not None and dtypes[i] is not torch.float32:
-                raise TypeError(f"row_masks[{i}]: row masks are for float32 parameters")
-        _check("last_steps", last_steps, torch.int32, [s[:1] for s in shapes], index)
+    columns, numel, rows, types, index, kept = collected
+    device = torch.device("cuda", index)
     if grad_scale is not None and (grad_scale.get_device() != index or grad_scale.dtype is not torch.float32 or grad_scale.numel() != 1):
         raise ValueError("grad_scale: one float32 on the parameters' device")
-
-    steps = list(step) if isinstance(step, (list, tuple)) else [step] * n
-    rates = list(lr) if isinstance(lr, (list, tuple)) else [lr] * n
-    decays = list(weight_decay) if isinstance(weight_decay, (list, tuple)) else [weight_decay] * n
-    _same_length(n, step=steps, lr=rates, weight_decay=decays)
-    step_tensors, step_numbers = _device_scalars("step", steps, torch.int64, index, 1)
-    rate_tensors, rate_numbers = _device_scalars("lr", rates, torch.float32, index, 0.0)
-    if step_tensors is None or 0 in step_tensors:
-        if min(s for s, t in zip(step_numbers, step_tensors or [0] * n) if t == 0) < 1:
-            raise ValueError("step counts from 1")
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("a captured step needs its step count in a device tensor: a number would be the same at every replay")
-    if min(rate_numbers) < 0 or min(decays) < 0:
-        raise ValueError("invalid AdamW hyper-parameters")
+    hyper, counts, step_tensors, rate_tensors, numbers = host.scalars(n, step, lr, weight_decay, beta1, beta2, eps, index)
+    if numbers and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("a captured step needs its step count in a device tensor: a number would be the same at every replay")
 
     norm = clip = None
     if max_grad_norm is not None:
-        norm, clip, _ = _norm_of(grads, shapes, dtypes, row_masks, float(max_grad_norm), False, norm_group)
+        norm, clip, _ = _norm_of((columns[1:2], numel, rows, types, index, kept), columns[6], float(max_grad_norm), False, norm_group)
     elif grad_scale is not None:
         clip = grad_scale
-    hyper = array("d")
-    for rate, decay in zip(rate_numbers, decays):
-        hyper.extend((rate, beta1, beta2, eps, decay))
-    columns = [_pointers(t) if t is not None else None
-               for t in (params, grads, exp_avgs, exp_avg_sqs, exponents, masters, row_masks, last_steps)]
-    numel = array("q", [s.numel() for s in shapes])
-    rows = array("i", [_row_length(s) for s in shapes])
-    types = array("i", [_DTYPES[d] for d in dtypes])
     ids = array("i", range(n) if tensor_ids is None else tensor_ids)
-    counts = array("q", step_numbers)
     workspace = None
     if step_tensors is not None or rate_tensors is not None:
         workspace = torch.empty(int(_lib.load().gs_adamw_workspace_bytes(n)), dtype=torch.uint8, device=device)
-    with _on(device):
-        call("gs_adamw_step", n, *[_address(c) for c in columns], _address(numel), _address(rows), _address(types), _address(ids),
-             _address(hyper), _address(counts), _address(step_tensors), _address(rate_tensors),
+    with _on(index):
+        call("gs_adamw_step", n, *columns, numel, rows, types, ids.buffer_info()[0], hyper, counts, step_tensors, rate_tensors,
              None if clip is None else clip.data_ptr(), seed & 0xFFFFFFFF,
              None if workspace is None else workspace.data_ptr(), current_stream(device))
     return norm
 
 
-def _device_scalars(name: str, values, dtype, device_index: int, stand_in):
-    """(addresses of the device tensors among ``values`` or None, the numbers with ``stand_in`` in the tensors' places)."""
-    if not any(isinstance(v, torch.Tensor) for v in values):
-        return None, values
-    for i, v in enumerate(values):
-        if isinstance(v, torch.Tensor) and (v.get_device() != device_index or v.dtype is not dtype or v.numel() != 1):
-            raise ValueError(f"{name}[{i}]: a number, or one {dtype} on the parameters' device")
-    return (array("Q", [v.data_ptr() if isinstance(v, torch.Tensor) else 0 for v in values]),
-            [stand_in if isinstance(v, torch.Tensor) else v for v in values])
-
-
 @torch.no_grad()
 def read_moments(exp_avgs: Sequence[torch.Tensor], exp_avg_sqs: Sequence[torch.Tensor], exponents: Sequence[torch.Tensor], *,
                  dtype: torch.dtype = torch.float32, out: Optional[Tuple[Sequence[torch.Tensor], Sequence[torch.Tensor]]] = None
-                 ) -> Tuple[List[torch.Tensor], List[torch.Tensor]]:
+                 ) -> Tuple[Sequence[torch.Tensor], Sequence[torch.Tensor]]:
     """The values that 8-bit moments stand for, as two lists of ``dtype`` tensors (float32 or bfloat16: both hold every value
     exactly) or written to ``out``."""
     n = len(exp_avgs)
-    _same_length(n, exp_avg_sqs=exp_avg_sqs, exponents=exponents)
-    if n == 0:
-        return [], []
-    device = _one_device(exp_avgs)
-    shapes = [t.shape for t in exp_avgs]
+    host = _lib.host()
+    inputs = ("exp_avgs", exp_avgs, host.CODE), ("exp_avg_sqs", exp_avg_sqs, host.CODE), ("exponents", exponents, host.EXPONENTS)
     if out is None:
         if dtype not in (torch.float32, torch.bfloat16):
             raise TypeError("read_moments: float32 or bfloat16 values")
-        out = tuple([torch.empty(s, dtype=dtype, device=device) for s in shapes] for _ in range(2))
+        collected = host.collect(*inputs)
+        out = tuple([torch.empty(t.shape, dtype=dtype, device=t.device) for t in exp_avgs] for _ in range(2))
+        if n == 0:
+            return out
+        (_, m_out, v_out), *_ = host.collect(inputs[0], ("out", out[0], host.VALUE), ("out", out[1], host.VALUE))
+        (m, v, x), numel, rows, _, index, _ = collected
     else:
-        _same_length(n, out_exp_avgs=out[0], out_exp_avg_sqs=out[1])
+        (m, v, x, m_out, v_out), numel, rows, _, index, _ = host.collect(*inputs, ("out", out[0], host.VALUE), ("out", out[1], host.VALUE))
+        if n == 0:
+            return out
         dtype = out[0][0].dtype
-        if dtype not in (torch.float32, torch.bfloat16):
-            raise TypeError("read_moments: float32 or bfloat16 values")
-    _check("exp_avgs", exp_avgs, torch.uint8, shapes, device.index)
-    _check("exp_avg_sqs", exp_avg_sqs, torch.uint8, shapes, device.index)
-    _check("exponents", exponents, torch.uint8, [(_num_blocks(s), 2) for s in shapes], device.index)
-    for k in range(2):
-        _check("out", out[k], dtype, shapes, device.index)
-    columns = [_pointers(t) for t in (exp_avgs, exp_avg_sqs, exponents, out[0], out[1])]
-    numel, rows = array("q", [s.numel() for s in shapes]), array("i", [_row_length(s) for s in shapes])
-    with _on(device):
-        call("gs_read_moments", n, *[_address(c) for c in columns], _address(numel), _address(rows), _DTYPES[dtype],
-             current_stream(device))
-    return list(out[0]), list(out[1])
+        if out[1][0].dtype is not dtype:
+            raise TypeError("out: both lists have one type")
+    with _on(index):
+        call("gs_read_moments", n, m, v, x, m_out, v_out, numel, rows, _DTYPES[dtype], current_stream(torch.device("cuda", index)))
+    return out
 
 
 class AdamW(torch.optim.Optimizer):
@@ -501,7 +393,7 @@ class AdamW(torch.optim.Optimizer):
         if self.max_grad_norm is not None:
             if len({key[3] for key in work}) > 1:
                 raise RuntimeError("max_grad_norm: all parameters belong on one device")
-            clip = self._clip([column for columns in work.values() for column in [columns]])
+            clip = self._clip(list(work.values()))
         for (bits, betas, eps, _), columns in work.items():
             params, grads, ms, vs, exponents, masters, masks, stamps, steps, rates, decays, places = columns
             if self.capturable:
@@ -517,16 +409,10 @@ class AdamW(torch.optim.Optimizer):
 
     def _clip(self, parts) -> torch.Tensor:
         """The clipping coefficient of all gradients (and ``last_grad_norm``)."""
-        grads = [g if g.is_contiguous() else g.contiguous() for columns in parts for g in columns[1]]
-        masks = [mask for columns in parts for mask in columns[6]]
-        dtypes, shapes = [g.dtype for g in grads], [g.shape for g in grads]
-        if any(d not in _DTYPES for d in dtypes):
-            raise TypeError("AdamW steps float32, bfloat16 and float16 parameters")
-        if any(mask is not None for mask in masks):
-            _check_masks(masks, grads, shapes, grads[0].device)
-        else:
-            masks = None
-        self.last_grad_norm, clip, _ = _norm_of(grads, shapes, dtypes, masks, float(self.max_grad_norm), False, self.norm_group)
+        host = _lib.host()
+        grads, masks = [g for columns in parts for g in columns[1]], [mask for columns in parts for mask in columns[6]]
+        collected = host.collect(("grads", grads, host.GRADS), ("row_masks", masks, host.MASK))
+        self.last_grad_norm, clip, _ = _norm_of(collected, collected[0][1], float(self.max_grad_norm), False, self.norm_group)
         return clip
 
     def moments(self, param: torch.Tensor, dtype: torch.dtype = torch.float32) -> Tuple[torch.Tensor, torch.Tensor]:
