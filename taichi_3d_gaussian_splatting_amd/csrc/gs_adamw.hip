@@ -31,11 +31,17 @@ struct AdamwScalars {
     uint32_t key;
 };
 
+// Quads of four consecutive elements a lane, so that an access is 16 bytes of each float buffer.  Two side by side (PAIR)
+// where the parameter has 16 bits, its moments 8 and there is no master copy: 16 bytes of the parameter again, and half the
+// instructions an element for a block's largest value, exponents and scales, which bound that case.
+constexpr bool pairs(int dtype, bool master, bool state8) { return state8 && dtype != GS_DTYPE_F32 && !master; }
+constexpr int MASKED_ROWS = 32;     // packed rows that a wave has in flight (8, 16, 32: 206, 202, 196 us for 1.2M rows, 30 % live)
+
 // How a tensor is cut among lanes
 enum Form : int {
-    FOURS,          // units of 64, or rows of 20, 24 .. 64 elements: 16 lanes a unit, four consecutive elements a lane
-    FOURS_MASKED,   // the same rows under a mask: a wave packs the live ones of 64 rows
-    NARROW,         // float rows of 1 to 4 elements: four rows a lane
+    QUADS,          // units of 64, or long rows: 16 lanes a unit, or 8 with pairs of quads
+    QUADS_MASKED,   // the same rows under a mask: a wave packs the live ones of 64 rows
+    NARROW,         // float rows of 1 to 4 elements: whole quads of rows a lane
     ELEMENTS        // anything else, unaligned tensors: element by element
 };
 
@@ -74,9 +80,10 @@ __host__ __device__ __forceinline__ uint32_t tensor_key(uint32_t seed, uint32_t 
     return mix32(mix32(seed + 0x9E3779B1u * tensor) + step);
 }
 
-// One hash serves four consecutive elements, each with another rotation of it; of an element's 32 bits the lower half
-// rounds the first moment, the upper half the second.
-__device__ __forceinline__ uint32_t element_bits(uint32_t hash, int j) { return __builtin_rotateleft32(hash, 8 * j); }
+// One hash serves four consecutive elements, element j with the hash rotated by 8 j; of an element's 32 bits the lower half
+// rounds the first moment, the upper half the second.  Here: a half in the middle of 20 bits, 16 h + 8.
+__device__ __forceinline__ uint32_t bits_for_m(uint32_t hash, int j) { return (__builtin_rotateleft32(hash, 8 * j + 4) & 0xFFFF0u) | 8u; }
+__device__ __forceinline__ uint32_t bits_for_v(uint32_t hash, int j) { return (__builtin_rotateleft32(hash, 8 * j + 20) & 0xFFFF0u) | 8u; }
 
 // ------------------------------------------------------------------ elements
 template <int DT>
@@ -120,69 +127,66 @@ __device__ __forceinline__ void store_four(void *p, long long i, f32x4 x) {
 __device__ __forceinline__ float from_bits(uint32_t u) { return __builtin_bit_cast(float, u); }
 __device__ __forceinline__ uint32_t to_bits(float x) { return __builtin_bit_cast(uint32_t, x); }
 
-// 2^(X - 127 + shift) for an exponent byte; NaN for 255
-__device__ __forceinline__ float exponent_scale(int x, int low, int shift) {
-    const int e = x < low ? low : x;
-    return x == 255 ? __builtin_nanf("") : from_bits((uint32_t)(e + shift) << 23);
+// A first moment's code is an 8-bit float of 4 exponent and 3 mantissa bits (with gradual underflow), which the hardware
+// converts; its block's factor is 2^(X - 135).  A second moment's code c is the upper bits of a float: its bits are
+// (c << 20) + v_base with v_base = (X - 31) << 23, no factor needed.
+__device__ __forceinline__ float m_scale(uint32_t x) {
+    const uint32_t xm = x & 255u;
+    return xm == 255u ? __builtin_nanf("") : from_bits(((xm < 9u ? 9u : xm) - 8u) << 23);
+}
+__device__ __forceinline__ uint32_t v_base(uint32_t x) {
+    const uint32_t xv = x >> 8 & 255u;
+    return ((xv < 32u ? 32u : xv) - 31u) << 23;
+}
+__device__ __forceinline__ bool v_is_nan(uint32_t x) { return (x >> 8 & 255u) == 255u; }
+__device__ __forceinline__ float v_of(uint32_t c, uint32_t base) { return c == 0u ? 0.f : from_bits((c << 20) + base); }
+__device__ __forceinline__ float unit_of(uint32_t c) { return __builtin_amdgcn_cvt_f32_fp8((int)c, 0); }
+
+template <int J>
+__device__ __forceinline__ float unit_byte(uint32_t codes) { return __builtin_amdgcn_cvt_f32_fp8((int)codes, J); }
+__device__ __forceinline__ float unit_at(uint32_t codes, int j) {
+    return j == 0 ? unit_byte<0>(codes) : j == 1 ? unit_byte<1>(codes) : j == 2 ? unit_byte<2>(codes) : unit_byte<3>(codes);
 }
 
-__device__ __forceinline__ float decode_m(uint32_t c, float scale) {
-    const uint32_t a = c & 127u;
-    const float size = a < 8u ? (float)a * 0x1p-9f : from_bits((a + 960u) << 20);
-    return (c & 128u ? -size : size) * scale;
-}
-__device__ __forceinline__ float decode_v(uint32_t c, float scale) {
-    return c == 0u ? 0.f * scale : from_bits((c << 20) + (127u << 23)) * scale;
-}
-
-// Four codes of each moment (the first in the lowest byte) under the exponent bytes X_m | X_v << 8
-__device__ __forceinline__ void decode_four(uint32_t mc, uint32_t vc, uint32_t x, f32x4 &m, f32x4 &v) {
-    const float scale_m = exponent_scale((int)(x & 255u), 9, -8), scale_v = exponent_scale((int)(x >> 8 & 255u), 32, -31);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        m[j] = decode_m((mc >> (8 * j)) & 255u, scale_m);
-        v[j] = decode_v((vc >> (8 * j)) & 255u, scale_v);
-    }
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ f32x4 units_of(uint32_t codes) {
+    const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, true);
+    return f32x4{a[0], a[1], b[0], b[1]};
 }
 
 // Exponent byte of a block from the bits of its largest magnitude (positive floats order like their bits, NaN above all):
-// `carry` moves values whose mantissa is over the largest code's to the next power, so that rounding up stays in range.
-__device__ __forceinline__ int block_exponent(uint32_t largest, uint32_t carry, int low) {
-    if (largest >= 0x7F800000u) return 255;
-    const int x = (int)((largest + carry) >> 23);
-    return x < low ? low : (x > 254 ? 254 : x);
+// `carry` moves values whose mantissa is over the largest code's to the next power, so that rounding up stays in range;
+// what has no finite value, or none below the largest power's end, makes 255.
+__device__ __forceinline__ uint32_t block_exponent(uint32_t largest, uint32_t carry, uint32_t low) {
+    return min(max((largest + carry) >> 23, low), 255u);
+}
+constexpr uint32_t CARRY_M = 0x1FFFFFu, CARRY_V = 0x0FFFFFu, LOW_M = 9u, LOW_V = 32u;
+
+// Code of a first moment, in the top byte of a word.  |m| 2^(15 - X) is a float whose bits, cut after the third mantissa
+// bit, are the code: float's own gradual underflow falls where the code's begins.  The 20 bits below meet 20 random ones:
+// the carry into the code has the chance that keeps the mean.
+__device__ __forceinline__ uint32_t m_word(float m, uint32_t xm, uint32_t bits) {
+    const uint32_t u = (to_bits(ldexpf(fabsf(m), 15 - (int)xm)) + bits) << 4;
+    return (u & 0x7FFFFFFFu) | (to_bits(m) & 0x80000000u);
+}
+// Code of a second moment: v's bits less the block's base, rounded the same way; a value over zero stays over zero (it is a
+// divisor's square).  The difference is negative below the smallest code, and does not pass 2^28 above.
+__device__ __forceinline__ uint32_t v_code(float v, uint32_t base, uint32_t bits) {
+    const int c = (int)(to_bits(v) - base + bits) >> 20;
+    return (uint32_t)max(c, (int)min(to_bits(v), 1u));
+}
+__device__ __forceinline__ uint32_t pack_top_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __builtin_amdgcn_perm(b, a, 0x0c0c0703u) | __builtin_amdgcn_perm(d, c, 0x07030c0cu);
 }
 
-// |m| 2^(135 - X) to sign, 4 exponent and 3 mantissa bits.  The 20 bits below the third mantissa bit meet 20 random ones
-// (16 of them, and a half): the carry into the code has the chance that keeps the mean.  Below 2^-6 the codes are evenly
-// spaced: there 2^-6 is added first, so that the same bits are the ones below the code.
-__device__ __forceinline__ uint32_t encode_m(float m, int x, uint32_t bits) {
-    if (x == 255) return 0u;
-    const float unscale = from_bits((uint32_t)(262 - x) << 23);
-    const float t = fabsf(m) * unscale;
-    const bool tiny = t < 0x1p-6f;
-    const uint32_t u = to_bits(tiny ? t + 0x1p-6f : t) + ((bits & 0xFFFFu) << 4) + 8u;
-    uint32_t a = (u >> 20) - (tiny ? 968u : 960u);
-    a = a > 126u ? 126u : a;
-    return a | (m < 0.f ? 128u : 0u);
-}
-// v 2^(158 - X) to 5 exponent and 3 mantissa bits; a value over zero stays over zero (it is a divisor's square).
-__device__ __forceinline__ uint32_t encode_v(float v, int x, uint32_t bits) {
-    if (x == 255) return 0u;
-    const float unscale = from_bits((uint32_t)(285 - x) << 23);
-    const int u = (int)(to_bits(v * unscale) - (127u << 23));
-    // (u is within +-2^30 except for zero and tiny values, which are the negative ones: the sum does not pass 2^31)
-    int c = (u + (int)((bits >> 16) << 4) + 8) >> 20;
-    c = c < 1 ? 1 : (c > 255 ? 255 : c);
-    return v > 0.f ? (uint32_t)c : 0u;
-}
-
-// Largest of GROUP consecutive lanes, in all of them (GROUP = 4: quad permutations, 16: rotations of a DPP row)
+// Largest of GROUP consecutive lanes, in all of them (GROUP = 4: quad permutations, 8: and a mirrored half row, 16: rotations
+// of a DPP row)
 template <int GROUP>
 __device__ __forceinline__ uint32_t group_max(uint32_t x) {
-    if (GROUP == 4) {
+    if (GROUP == 4 || GROUP == 8) {
         x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0xB1, 0xF, 0xF, true));
         x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x4E, 0xF, 0xF, true));
+        if (GROUP == 8) x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x141, 0xF, 0xF, true));
     } else if (GROUP == 16) {
         x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x128, 0xF, 0xF, true));
         x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x124, 0xF, 0xF, true));
@@ -212,19 +216,35 @@ __device__ __forceinline__ float scaled(float g, float scale) {
     return g * scale;
 }
 
-// The moments in 32 bits take the correctly rounded square root and division (they are hidden behind 28 bytes an element);
-// with 8 bits hardware's own, one unit in the last place each, are as good: the moments' codes do not depend on them.
-template <bool FAST, bool MASTER>
-__device__ __forceinline__ float update_one(float p, float g, float &m, float &v, const AdamwScalars &k) {
-    m = fmaf(k.one_minus_beta1, g - m, m);
-    v = fmaf(k.one_minus_beta2 * g, g, k.beta2 * v);
-    float change;
-    if (FAST) change = m * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v) * k.root + k.eps);
-    else change = m / (sqrtf(v) * k.root + k.eps);
+template <bool MASTER>
+__device__ __forceinline__ float moved(float p, float change, const AdamwScalars &k) {
     p = p * k.keep - k.rate * change;
     // (a 16-bit parameter is its master copy rounded: without the stop the conversion may join the last operation)
     if (MASTER) asm volatile("" : "+v"(p));
     return p;
+}
+
+// Moments in 32 bits: the correctly rounded square root and division, hidden behind 28 bytes an element
+template <bool MASTER>
+__device__ __forceinline__ float update_one(float p, float g, float &m, float &v, const AdamwScalars &k) {
+    m = fmaf(k.one_minus_beta1, g - m, m);
+    v = fmaf(k.one_minus_beta2 * g, g, k.beta2 * v);
+    return moved<MASTER>(p, m / (sqrtf(v) * k.root + k.eps), k);
+}
+
+// Moments in 8 bits are bound by their arithmetic: what is the same for a block goes into two factors, and the square root
+// and the reciprocal are the hardware's (one unit in the last place each; the codes do not depend on them).
+struct OldBlock {
+    float m_factor, v_factor;       // beta1 2^(X - 135) and beta2, times what late rows lost; NaN for 255
+    uint32_t base;
+    __device__ __forceinline__ OldBlock(uint32_t x, float decay_m, float decay_v, const AdamwScalars &k)
+        : m_factor(k.beta1 * decay_m * m_scale(x)), v_factor(v_is_nan(x) ? __builtin_nanf("") : k.beta2 * decay_v), base(v_base(x)) {}
+};
+template <bool MASTER>
+__device__ __forceinline__ float update_coded(float p, float g, float m_unit, uint32_t v_old, const OldBlock &o, float &m, float &v, const AdamwScalars &k) {
+    m = fmaf(k.one_minus_beta1, g, o.m_factor * m_unit);
+    v = fmaf(k.one_minus_beta2 * g, g, o.v_factor * v_of(v_old, o.base));
+    return moved<MASTER>(p, m * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v) * k.root + k.eps), k);
 }
 
 // What a row that was last stepped at `last` has to be multiplied with before this step
@@ -236,81 +256,167 @@ __device__ __forceinline__ void row_decay(const AdamwScalars &k, int last, float
     }
 }
 
-// Codes and exponents of a block from the lanes that share it: four elements a lane
-template <int GROUP>
-__device__ __forceinline__ uint32_t encode_four(const f32x4 &m, const f32x4 &v, uint32_t hash, uint32_t &mc, uint32_t &vc) {
+// Codes and exponent bytes of a block from the lanes that share it: Q quads of consecutive elements a lane
+template <int GROUP, int Q>
+__device__ __forceinline__ uint32_t encode(const f32x4 (&m)[Q], const f32x4 (&v)[Q], uint32_t quad, uint32_t key, uint32_t (&mc)[Q], uint32_t (&vc)[Q]) {
     uint32_t top_m = 0u, top_v = 0u;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        top_m = max(top_m, to_bits(m[j]) & 0x7FFFFFFFu);
-        top_v = max(top_v, to_bits(v[j]) & 0x7FFFFFFFu);
+    for (int e = 0; e < 4 * Q; ++e) {
+        top_m = max(top_m, to_bits(m[e / 4][e % 4]) & 0x7FFFFFFFu);
+        top_v = max(top_v, to_bits(v[e / 4][e % 4]));
     }
-    const int xm = block_exponent(group_max<GROUP>(top_m), 0x1FFFFFu, 9), xv = block_exponent(group_max<GROUP>(top_v), 0x0FFFFFu, 32);
-    mc = vc = 0u;
+    // (v is not negative; a NaN may carry a sign)
+    const uint32_t xm = block_exponent(group_max<GROUP>(top_m), CARRY_M, LOW_M), xv = block_exponent(group_max<GROUP>(top_v & 0x7FFFFFFFu), CARRY_V, LOW_V);
+    const uint32_t base = (xv - 31u) << 23;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const uint32_t bits = element_bits(hash, j);
-        mc |= encode_m(m[j], xm, bits) << (8 * j);
-        vc |= encode_v(v[j], xv, bits) << (8 * j);
+    for (int c = 0; c < Q; ++c) {
+        const uint32_t hash = mix32((quad + c) ^ key);
+        uint32_t w[4];
+        vc[c] = 0u;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            w[j] = m_word(m[c][j], xm, bits_for_m(hash, j));
+            vc[c] |= v_code(v[c][j], base, bits_for_v(hash, j)) << (8 * j);
+        }
+        mc[c] = xm == 255u ? 0u : pack_top_bytes(w[0], w[1], w[2], w[3]);
+        vc[c] = xv == 255u ? 0u : vc[c];
     }
-    return (uint32_t)(xm | xv << 8);
+    return xm | xv << 8;
 }
 
-template <bool FAST, bool MASTER>
-__device__ __forceinline__ void update_four(f32x4 &p, const f32x4 &g, f32x4 &m, f32x4 &v, float scale, const AdamwScalars &k) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        float mj = m[j], vj = v[j];
-        p[j] = update_one<FAST, MASTER>(p[j], scaled(g[j], scale), mj, vj, k);
-        m[j] = mj;
-        v[j] = vj;
-    }
-}
-
-// Four consecutive elements a lane: what a lane reads before the step and writes after it
+// A tensor's buffers from one place on (the same for a whole workgroup or wave: scalar registers), indexed by 32 bits
 template <int DT, bool MASTER, bool STATE8>
-struct Quad {
-    typename Four<MASTER ? GS_DTYPE_F32 : DT>::type p;
-    typename Four<DT>::type g;
-    f32x4 m, v;
-    uint32_t mc, vc;
-
-    __device__ __forceinline__ void clear() {
-        p = {};
-        g = {};
-        m = v = f32x4{0.f, 0.f, 0.f, 0.f};
-        mc = vc = 0u;
+struct Buffers {
+    const char *source;     // what the step starts from: the master copy or the parameter
+    char *param;
+    const char *grad;
+    char *m, *v;
+    uint8_t *exponents;
+    uint32_t quad;          // the first element's index / 4, for the rounding bits
+    __device__ __forceinline__ Buffers(const AdamwTensor &t, long long element, long long unit) {
+        constexpr int BYTES = DT == GS_DTYPE_F32 ? 4 : 2, STATE = STATE8 ? 1 : 4;
+        source = (const char *)(MASTER ? t.master_or_mask : t.param) + element * (MASTER ? 4 : BYTES);
+        param = (char *)t.param + element * BYTES;
+        grad = (const char *)t.grad + element * BYTES;
+        m = (char *)t.exp_avg + element * STATE;
+        v = (char *)t.exp_avg_sq + element * STATE;
+        exponents = t.exponents + 2 * unit;
+        quad = (uint32_t)(element >> 2);
     }
-    __device__ __forceinline__ void load(const AdamwTensor &t, long long i) {
-        p = *(const decltype(p) *)((const char *)(MASTER ? t.master_or_mask : t.param) + i * (long long)(sizeof(p) / 4));
-        g = *(const decltype(g) *)((const char *)t.grad + i * (long long)(sizeof(g) / 4));
-        if (STATE8) {
-            mc = *(const uint32_t *)((const uint8_t *)t.exp_avg + i);
-            vc = *(const uint32_t *)((const uint8_t *)t.exp_avg_sq + i);
+};
+
+// Parameter, gradient and moments are read once and written once a step, and the next reader of most of them is the next step:
+// they pass the caches by.
+template <typename T>
+__device__ __forceinline__ T stream_load(const char *p) { return __builtin_nontemporal_load((const T *)p); }
+template <typename T>
+__device__ __forceinline__ void stream_store(char *p, T x) { __builtin_nontemporal_store(x, (T *)p); }
+
+// One or two quads of consecutive elements a lane: what a lane reads before the step and writes after it.  (Two float quads
+// a lane are no gain: an access of the wave then covers half of each cache line, and every line is asked for twice.)
+template <int DT, bool MASTER, bool STATE8, bool STREAM = true>
+struct Share {
+    typedef Buffers<DT, MASTER, STATE8> B;
+    typedef typename Four<DT>::type Value;
+    typedef typename Four<MASTER ? GS_DTYPE_F32 : DT>::type Source;
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    static constexpr bool PAIR = pairs(DT, MASTER, STATE8);
+    static constexpr int Q = PAIR ? 2 : 1, GROUP = 16 / Q;
+    Source p[Q];
+    Value g[Q];
+    f32x4 m[Q], v[Q];
+    uint32_t mc[Q], vc[Q];
+    uint32_t e;             // the first element, counted from the buffers' beginning
+
+    // Lane `sub` of a block that begins at `first` and has `len` elements; a lane past its end takes the block's last ones.
+    __device__ __forceinline__ void place(uint32_t first, uint32_t len, uint32_t sub) { e = first + min(4u * Q * sub, len - 4u * Q); }
+    static __device__ __forceinline__ bool inside(uint32_t len, uint32_t sub) { return 4u * Q * sub < len; }
+
+    template <typename T>
+    static __device__ __forceinline__ T get(const char *p) { return STREAM ? stream_load<T>(p) : *(const T *)p; }
+    template <typename T>
+    static __device__ __forceinline__ void put(char *p, T x) {
+        if (STREAM) stream_store(p, x);
+        else *(T *)p = x;
+    }
+    __device__ __forceinline__ void load(const B &b) {
+        if constexpr (PAIR) {
+            const u32x4 x = get<u32x4>(b.source + e * 2u), y = get<u32x4>(b.grad + e * 2u);
+            const u32x2 a = get<u32x2>(b.m + e), d = get<u32x2>(b.v + e);
+#pragma unroll
+            for (int c = 0; c < Q; ++c) {
+                p[c] = __builtin_bit_cast(Source, (u32x2){x[2 * c], x[2 * c + 1]});
+                g[c] = __builtin_bit_cast(Value, (u32x2){y[2 * c], y[2 * c + 1]});
+                mc[c] = a[c];
+                vc[c] = d[c];
+            }
         } else {
-            m = *(const f32x4 *)((const float *)t.exp_avg + i);
-            v = *(const f32x4 *)((const float *)t.exp_avg_sq + i);
+            p[0] = get<Source>(b.source + e * (uint32_t)(sizeof(Source) / 4));
+            g[0] = get<Value>(b.grad + e * (uint32_t)(sizeof(Value) / 4));
+            if constexpr (STATE8) {
+                mc[0] = get<uint32_t>(b.m + e);
+                vc[0] = get<uint32_t>(b.v + e);
+            } else {
+                m[0] = get<f32x4>(b.m + e * 4u);
+                v[0] = get<f32x4>(b.v + e * 4u);
+            }
+        }
+    }
+    __device__ __forceinline__ void store(const B &b, const f32x4 (&out)[Q]) const {
+        if constexpr (PAIR) {
+            const u32x2 x = __builtin_bit_cast(u32x2, __builtin_convertvector(out[0], Value)), y = __builtin_bit_cast(u32x2, __builtin_convertvector(out[1], Value));
+            put(b.param + e * 2u, (u32x4){x[0], x[1], y[0], y[1]});
+            put(b.m + e, (u32x2){mc[0], mc[1]});
+            put(b.v + e, (u32x2){vc[0], vc[1]});
+        } else {
+            if (MASTER) put((char *)b.source + e * 4u, out[0]);
+            put(b.param + e * (uint32_t)(sizeof(Value) / 4), __builtin_convertvector(out[0], Value));
+            if constexpr (STATE8) {
+                put(b.m + e, mc[0]);
+                put(b.v + e, vc[0]);
+            } else {
+                put(b.m + e * 4u, m[0]);
+                put(b.v + e * 4u, v[0]);
+            }
         }
     }
     // The step; returns the exponent bytes of the block that GROUP lanes share
-    template <int GROUP>
-    __device__ __forceinline__ uint32_t step(f32x4 &out, uint32_t x, float decay_m, float decay_v, long long i, float scale, const AdamwScalars &k) {
-        out = __builtin_convertvector(p, f32x4);
-        if (STATE8) decode_four(mc, vc, x, m, v);
-        m *= decay_m;
-        v *= decay_v;
-        update_four<STATE8, MASTER>(out, __builtin_convertvector(g, f32x4), m, v, scale, k);
-        return STATE8 ? encode_four<GROUP>(m, v, mix32((uint32_t)(i >> 2) ^ k.key), mc, vc) : 0u;
-    }
-    __device__ __forceinline__ void store(const AdamwTensor &t, long long i, const f32x4 &out) const {
-        if (MASTER) *(f32x4 *)((float *)t.master_or_mask + i) = out;
-        *(decltype(g) *)((char *)t.param + i * (long long)(sizeof(g) / 4)) = __builtin_convertvector(out, decltype(g));
-        if (STATE8) {
-            *(uint32_t *)((uint8_t *)t.exp_avg + i) = mc;
-            *(uint32_t *)((uint8_t *)t.exp_avg_sq + i) = vc;
+    template <bool LATE>
+    __device__ __forceinline__ uint32_t step(f32x4 (&out)[Q], uint32_t x, float decay_m, float decay_v, uint32_t first_quad, float scale, const AdamwScalars &k) {
+#pragma unroll
+        for (int c = 0; c < Q; ++c) out[c] = __builtin_convertvector(p[c], f32x4);
+        if constexpr (STATE8) {
+            const OldBlock o(x, decay_m, decay_v, k);
+#pragma unroll
+            for (int c = 0; c < Q; ++c) {
+                const f32x4 units = units_of(mc[c]), grad = __builtin_convertvector(g[c], f32x4);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float mj, vj;
+                    out[c][j] = update_coded<MASTER>(out[c][j], scaled(grad[j], scale), units[j], (vc[c] >> (8 * j)) & 255u, o, mj, vj, k);
+                    m[c][j] = mj;
+                    v[c][j] = vj;
+                }
+            }
+            return encode<GROUP>(m, v, first_quad + (e >> 2), k.key, mc, vc);
         } else {
-            *(f32x4 *)((float *)t.exp_avg + i) = m;
-            *(f32x4 *)((float *)t.exp_avg_sq + i) = v;
+#pragma unroll
+            for (int c = 0; c < Q; ++c) {
+                const f32x4 grad = __builtin_convertvector(g[c], f32x4);
+                if (LATE) {
+                    m[c] *= decay_m;
+                    v[c] *= decay_v;
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float mj = m[c][j], vj = v[c][j];
+                    out[c][j] = update_one<MASTER>(out[c][j], scaled(grad[j], scale), mj, vj, k);
+                    m[c][j] = mj;
+                    v[c][j] = vj;
+                }
+            }
+            return 0u;
         }
     }
 };
@@ -331,41 +437,34 @@ __device__ __forceinline__ void step_unit(const AdamwTensor &t, const AdamwScala
     }
     const int count = live ? max(0, (len - sub + GROUP - 1) / GROUP) : 0;     // element j of this lane exists for j < count
     float p[4], m[4], v[4];
-    float scale_m = 1.f, scale_v = 1.f;
-    if (STATE8 && live) {
-        scale_m = exponent_scale(t.exponents[2 * unit], 9, -8);
-        scale_v = exponent_scale(t.exponents[2 * unit + 1], 32, -31);
-    }
+    const uint32_t x = STATE8 && live ? t.exponents[2 * unit] | (uint32_t)t.exponents[2 * unit + 1] << 8 : 0u;
+    const OldBlock o(x, decay_m, decay_v, k);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        float g = 0.f;
         p[j] = m[j] = v[j] = 0.f;
         if (j < count) {
             const long long i = base + sub + j * GROUP;
             p[j] = MASTER ? ((const float *)t.master_or_mask)[i] : load_one<DT>(t.param, i);
-            g = load_one<DT>(t.grad, i);
+            const float g = scaled(load_one<DT>(t.grad, i), scale);
             if (STATE8) {
-                m[j] = decode_m(((const uint8_t *)t.exp_avg)[i], scale_m);
-                v[j] = decode_v(((const uint8_t *)t.exp_avg_sq)[i], scale_v);
+                p[j] = update_coded<MASTER>(p[j], g, unit_of(((const uint8_t *)t.exp_avg)[i]), ((const uint8_t *)t.exp_avg_sq)[i], o, m[j], v[j], k);
             } else {
-                m[j] = ((const float *)t.exp_avg)[i];
-                v[j] = ((const float *)t.exp_avg_sq)[i];
+                m[j] = ((const float *)t.exp_avg)[i] * decay_m;
+                v[j] = ((const float *)t.exp_avg_sq)[i] * decay_v;
+                p[j] = update_one<MASTER>(p[j], g, m[j], v[j], k);
             }
         }
-        m[j] *= decay_m;
-        v[j] *= decay_v;
-        p[j] = update_one<STATE8, MASTER>(p[j], scaled(g, scale), m[j], v[j], k);
     }
-    int xm = 0, xv = 0;
+    uint32_t xm = 0, xv = 0;
     if (STATE8) {
         uint32_t top_m = 0u, top_v = 0u;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            top_m = j < count ? max(top_m, to_bits(m[j]) & 0x7FFFFFFFu) : top_m;
-            top_v = j < count ? max(top_v, to_bits(v[j]) & 0x7FFFFFFFu) : top_v;
+            top_m = max(top_m, to_bits(m[j]) & 0x7FFFFFFFu);
+            top_v = max(top_v, to_bits(v[j]) & 0x7FFFFFFFu);
         }
-        xm = block_exponent(group_max<GROUP>(top_m), 0x1FFFFFu, 9);
-        xv = block_exponent(group_max<GROUP>(top_v), 0x0FFFFFu, 32);
+        xm = block_exponent(group_max<GROUP>(top_m), CARRY_M, LOW_M);
+        xv = block_exponent(group_max<GROUP>(top_v), CARRY_V, LOW_V);
         if (live && sub == 0) {
             t.exponents[2 * unit] = (uint8_t)xm;
             t.exponents[2 * unit + 1] = (uint8_t)xv;
@@ -379,9 +478,10 @@ __device__ __forceinline__ void step_unit(const AdamwTensor &t, const AdamwScala
             if (MASTER) ((float *)t.master_or_mask)[i] = p[j];
             store_one<DT>(t.param, i, p[j]);
             if (STATE8) {
-                const uint32_t bits = element_bits(mix32((uint32_t)(i >> 2) ^ k.key), (int)(i & 3));
-                ((uint8_t *)t.exp_avg)[i] = (uint8_t)encode_m(m[j], xm, bits);
-                ((uint8_t *)t.exp_avg_sq)[i] = (uint8_t)encode_v(v[j], xv, bits);
+                const uint32_t hash = mix32((uint32_t)(i >> 2) ^ k.key);
+                const int place = (int)(i & 3);
+                ((uint8_t *)t.exp_avg)[i] = xm == 255u ? 0 : (uint8_t)(m_word(m[j], xm, bits_for_m(hash, place)) >> 24);
+                ((uint8_t *)t.exp_avg_sq)[i] = xv == 255u ? 0 : (uint8_t)v_code(v[j], (xv - 31u) << 23, bits_for_v(hash, place));
             } else {
                 ((float *)t.exp_avg)[i] = m[j];
                 ((float *)t.exp_avg_sq)[i] = v[j];
@@ -390,193 +490,199 @@ __device__ __forceinline__ void step_unit(const AdamwTensor &t, const AdamwScala
     }
 }
 
-// A workgroup's share in units is 16 (of 16 lanes) times UNROLL; a lane asks for all its units' data before it uses any.
+// A workgroup's share in units is 16 (32 with pairs) times UNROLL; a lane asks for all its units' data before it uses any.
+// Lanes past a row's end and units past the tensor's read their neighbours' data again (the same largest value) and store nothing.
 template <int UNROLL, int DT, bool MASTER, bool STATE8>
-__device__ __forceinline__ void step_fours(const AdamwTensor &t, const AdamwScalars &k, float scale, unsigned chunk) {
-    constexpr int GROUP = 16, PER_PASS = GS_BLOCK / GROUP;
-    const int unit_len = t.row_len > 0 ? t.row_len : UNIT;
-    const long long chunk_unit = (long long)chunk * (PER_PASS * UNROLL);
-    const long long unit0 = chunk_unit + threadIdx.x / GROUP;
-    const long long whole = t.numel / unit_len;         // units of full length
-    const int sub = threadIdx.x % GROUP;
-    Quad<DT, MASTER, STATE8> q[UNROLL];
-    uint32_t x[UNROLL];
+__device__ __forceinline__ void step_quads(const AdamwTensor &t, const AdamwScalars &k, float scale, unsigned chunk) {
+    typedef Share<DT, MASTER, STATE8> S;
+    constexpr int GROUP = S::GROUP, PER_PASS = GS_BLOCK / GROUP, SHARE = PER_PASS * UNROLL;
+    const uint32_t unit_len = t.row_len > 0 ? t.row_len : UNIT;
+    const long long chunk_unit = (long long)chunk * SHARE, whole = t.numel / unit_len;         // units of full length
+    const uint32_t units = (uint32_t)min((long long)SHARE, max(0LL, whole - chunk_unit));
+    const uint32_t sub = threadIdx.x % GROUP;
+    if (units > 0) {
+        const Buffers<DT, MASTER, STATE8> b(t, chunk_unit * unit_len, chunk_unit);
+        S q[UNROLL];
+        uint32_t x[UNROLL];
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-        const long long unit = unit0 + u * PER_PASS;
-        q[u].clear();
-        x[u] = 0u;
-        if (unit < whole && 4 * sub < unit_len) {
-            q[u].load(t, unit * unit_len + 4 * sub);
-            if (STATE8) x[u] = *(const uint16_t *)(t.exponents + 2 * unit);
+        for (int u = 0; u < UNROLL; ++u) {
+            const uint32_t unit = min(threadIdx.x / GROUP + u * PER_PASS, units - 1u);
+            q[u].place(unit * unit_len, unit_len, sub);
+            q[u].load(b);
+            x[u] = STATE8 ? *(const uint16_t *)(b.exponents + 2u * unit) : 0u;
         }
-    }
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-        const long long unit = unit0 + u * PER_PASS;
-        const long long i = unit * unit_len + 4 * sub;
-        f32x4 p;
-        // (a lane past its row's end holds zeros, and NaN only where the clipping coefficient makes NaN of all)
-        const uint32_t new_x = q[u].template step<GROUP>(p, x[u], 1.f, 1.f, i, scale, k);
-        if (unit < whole && 4 * sub < unit_len) {
-            q[u].store(t, i, p);
-            if (STATE8 && sub == 0) *(uint16_t *)(t.exponents + 2 * unit) = (uint16_t)new_x;
+        for (int u = 0; u < UNROLL; ++u) {
+            const uint32_t unit = threadIdx.x / GROUP + u * PER_PASS;
+            f32x4 p[S::Q];
+            const uint32_t new_x = q[u].template step<false>(p, x[u], 1.f, 1.f, b.quad, scale, k);
+            if (unit < units && S::inside(unit_len, sub)) {
+                q[u].store(b, p);
+                if (STATE8 && sub == 0) *(uint16_t *)(b.exponents + 2u * unit) = (uint16_t)new_x;
+            }
         }
     }
     // the last unit of a flat tensor, where it is shorter
-    if (whole * unit_len < t.numel && whole >= chunk_unit && whole < chunk_unit + PER_PASS * UNROLL && threadIdx.x < GS_WAVE)
-        step_unit<GROUP, DT, MASTER, STATE8>(t, k, scale, whole + threadIdx.x / GROUP, unit_len);
+    if (whole * unit_len < t.numel && whole >= chunk_unit && whole < chunk_unit + SHARE && threadIdx.x < GS_WAVE)
+        step_unit<16, DT, MASTER, STATE8>(t, k, scale, whole + threadIdx.x / 16, (int)unit_len);
 }
 
 // Rows under a mask: a wave reads the mask and the stamps of 64 rows, packs the live ones and steps them four at a time, so
 // that no lane waits beside a row without a point and none of such a row's data is asked for.
 template <int UNROLL, bool STATE8>
-__device__ __forceinline__ void step_fours_masked(const AdamwTensor &t, const AdamwScalars &k, float scale, unsigned chunk) {
-    constexpr int GROUP = 16;
-    const int row_len = t.row_len, lane = gs_lane(), sub = lane % GROUP;
-    const long long row0 = ((long long)chunk * (GS_BLOCK / GS_WAVE) + threadIdx.x / GS_WAVE) * GS_WAVE;
-    const long long mine = row0 + lane, rows = t.numel / row_len;
-    const bool live = mine < rows && ((const int8_t *)t.master_or_mask)[mine < rows ? mine : 0] == 0;
-    const u64 lives = __ballot(live);
+__device__ __forceinline__ void step_quads_masked(const AdamwTensor &t, const AdamwScalars &k, float scale, unsigned chunk) {
+    typedef Share<GS_DTYPE_F32, false, STATE8> S;
+    constexpr int GROUP = S::GROUP, PER_PASS = GS_WAVE / GROUP;
+    const uint32_t row_len = t.row_len, lane = gs_lane(), sub = lane % GROUP;
+    const long long row0 = ((long long)chunk * (GS_BLOCK / GS_WAVE) + __builtin_amdgcn_readfirstlane(threadIdx.x / GS_WAVE)) * GS_WAVE;
+    const long long rows = t.numel / row_len;
+    if (row0 >= rows) return;
+    const bool there = row0 + lane < rows;
+    const bool live = there && ((const int8_t *)t.master_or_mask)[there ? row0 + lane : row0] == 0;
+    const u64 lives = __ballot(live), below = (1ull << lane) - 1ull;
     if (lives == 0) return;
     float decay_m = 1.f, decay_v = 1.f;
     int x = 0;
     if (live) {
-        row_decay(k, t.last_step[mine], decay_m, decay_v);
-        t.last_step[mine] = k.step;
-        if (STATE8) x = *(const uint16_t *)(t.exponents + 2 * mine);
+        row_decay(k, t.last_step[row0 + lane], decay_m, decay_v);
+        t.last_step[row0 + lane] = k.step;
+        if (STATE8) x = *(const uint16_t *)(t.exponents + 2 * (row0 + lane));
     }
     // lane i learns which lane has the i-th live row
-    const int rank = __popcll(lives & ((1ull << lane) - 1ull)), n_live = __popcll(lives);
-    const int order = __builtin_amdgcn_ds_permute(4 * (live ? rank : 63 - __popcll(~lives & ((1ull << lane) - 1ull))), lane);
+    const int n_live = __popcll(lives);
+    const int order = __builtin_amdgcn_ds_permute(4 * (live ? __popcll(lives & below) : 63 - __popcll(~lives & below)), (int)lane);
     const bool any_late = __ballot(decay_m != 1.f || decay_v != 1.f) != 0;
-    for (int at = 0; at < n_live; at += 4 * UNROLL) {
-        Quad<GS_DTYPE_F32, false, STATE8> q[UNROLL];
+    const Buffers<GS_DTYPE_F32, false, STATE8> b(t, row0 * row_len, row0);
+    for (int at = 0; at < n_live; at += PER_PASS * UNROLL) {
+        S q[UNROLL];
         int from[UNROLL];
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
-            const int i = at + 4 * u + lane / GROUP;
-            from[u] = __shfl(order, i < n_live ? i : 0, GS_WAVE);
-            q[u].clear();
-            if (i < n_live && 4 * sub < row_len) q[u].load(t, (row0 + from[u]) * row_len + 4 * sub);
+            from[u] = __shfl(order, min(at + PER_PASS * u + (int)(lane / GROUP), n_live - 1), GS_WAVE);
+            q[u].place(from[u] * row_len, row_len, sub);
+            q[u].load(b);
         }
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
-            const long long i = (row0 + from[u]) * row_len + 4 * sub;
             const uint32_t old_x = STATE8 ? (uint32_t)__shfl(x, from[u], GS_WAVE) : 0u;
             const float dm = any_late ? __shfl(decay_m, from[u], GS_WAVE) : 1.f, dv = any_late ? __shfl(decay_v, from[u], GS_WAVE) : 1.f;
-            f32x4 p;
-            const uint32_t new_x = q[u].template step<GROUP>(p, old_x, dm, dv, i, scale, k);
-            if (at + 4 * u + lane / GROUP < n_live && 4 * sub < row_len) {
-                q[u].store(t, i, p);
-                if (STATE8 && sub == 0) *(uint16_t *)(t.exponents + 2 * (row0 + from[u])) = (uint16_t)new_x;
+            f32x4 p[S::Q];
+            const uint32_t new_x = q[u].template step<true>(p, old_x, dm, dv, b.quad, scale, k);
+            if (at + PER_PASS * u + (int)(lane / GROUP) < n_live && S::inside(row_len, sub)) {
+                q[u].store(b, p);
+                if (STATE8 && sub == 0) *(uint16_t *)(b.exponents + 2 * from[u]) = (uint16_t)new_x;
             }
         }
     }
 }
 
-// Float rows of L elements, four rows (L quads) a lane: every access is 16 bytes (4 for codes, 8 for exponents) although a row
-// is not.  Of rows under a mask the lane writes back what it read.
+// Float rows of L = 1..4 elements, as many rows a lane as make whole quads (rows of three: four rows, three quads): every access
+// is 16 bytes (4 for codes) although a row is not.  Of rows under a mask the lane writes back what it read.
+__host__ __device__ constexpr int narrow_rows(int row_len) { return row_len == 4 ? 1 : (row_len == 2 ? 2 : 4); }
+
 template <int L, bool STATE8>
 __device__ __forceinline__ void step_narrow(const AdamwTensor &t, const AdamwScalars &k, float scale, unsigned chunk) {
-    const long long rows = t.numel / L, row0 = 4 * ((long long)chunk * GS_BLOCK + threadIdx.x);
+    constexpr int R = narrow_rows(L), Q = R * L / 4;
+    const long long rows = t.numel / L, row0 = R * ((long long)chunk * GS_BLOCK + threadIdx.x);
     if (row0 >= rows) return;
-    if (row0 + 4 > rows) {
+    if (row0 + R > rows) {
         for (long long r = row0; r < rows; ++r) step_unit<1, GS_DTYPE_F32, false, STATE8>(t, k, scale, r, L);
         return;
     }
-    bool live[4] = {true, true, true, true};
-    float decay_m[4] = {1.f, 1.f, 1.f, 1.f}, decay_v[4] = {1.f, 1.f, 1.f, 1.f};
-    typedef int i32x4 __attribute__((ext_vector_type(4)));
-    typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
-    if (t.masked) {
-        const uint32_t mask = *(const uint32_t *)((const int8_t *)t.master_or_mask + row0);
-        i32x4 last = *(const i32x4 *)(t.last_step + row0);
+    bool live[R];
+    float decay_m[R], decay_v[R];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            live[r] = (mask >> (8 * r) & 255u) == 0u;
+    for (int r = 0; r < R; ++r) {
+        live[r] = true;
+        decay_m[r] = decay_v[r] = 1.f;
+    }
+    if (t.masked) {
+        int8_t mask[R];
+        int last[R];
+        __builtin_memcpy(mask, __builtin_assume_aligned((const int8_t *)t.master_or_mask + row0, R), R);
+        __builtin_memcpy(last, __builtin_assume_aligned(t.last_step + row0, 4 * R), 4 * R);
+        bool any = false;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            live[r] = mask[r] == 0;
+            any = any || live[r];
             if (live[r]) {
                 row_decay(k, last[r], decay_m[r], decay_v[r]);
                 last[r] = k.step;
             }
         }
-        if (!(live[0] || live[1] || live[2] || live[3])) return;
-        *(i32x4 *)(t.last_step + row0) = last;
+        if (!any) return;
+        __builtin_memcpy(__builtin_assume_aligned(t.last_step + row0, 4 * R), last, 4 * R);
     }
-    const long long base = row0 * L;
-    Quad<GS_DTYPE_F32, false, STATE8> q[L];
-    u16x4 x = {0, 0, 0, 0};
+    const Buffers<GS_DTYPE_F32, false, STATE8> b(t, row0 * L, row0);
+    Share<GS_DTYPE_F32, false, STATE8, false> q[Q];      // (cached: several accesses of the lane touch a line; 202 us, else 232)
+    uint16_t x[R];
 #pragma unroll
-    for (int c = 0; c < L; ++c) q[c].load(t, base + 4 * c);
-    if (STATE8) x = *(const u16x4 *)(t.exponents + 2 * row0);
-    f32x4 p[L];
-    float m[4 * L], v[4 * L];
-#pragma unroll
-    for (int e = 0; e < 4 * L; ++e) {
-        const int r = e / L, c = e / 4, j = e % 4;
-        if (STATE8) {
-            m[e] = decode_m((q[c].mc >> (8 * j)) & 255u, exponent_scale(x[r] & 255, 9, -8));
-            v[e] = decode_v((q[c].vc >> (8 * j)) & 255u, exponent_scale(x[r] >> 8, 32, -31));
-        } else {
-            m[e] = q[c].m[j];
-            v[e] = q[c].v[j];
-        }
-        const float old_p = q[c].p[j], old_m = m[e], old_v = v[e];
-        m[e] *= decay_m[r];
-        v[e] *= decay_v[r];
-        p[c][j] = update_one<STATE8, false>(old_p, scaled(q[c].g[j], scale), m[e], v[e], k);
-        if (!live[r]) {
-            p[c][j] = old_p;
-            m[e] = old_m;
-            v[e] = old_v;
-        }
+    for (int c = 0; c < Q; ++c) {
+        q[c].e = 4u * c;
+        q[c].load(b);
     }
-    if (STATE8) {
-        uint32_t hash[L];
+    if (STATE8) __builtin_memcpy(x, __builtin_assume_aligned(b.exponents, 2 * R), 2 * R);
+    f32x4 p[Q][1];
+    if constexpr (STATE8) {
+        uint32_t mc[Q] = {}, vc[Q] = {};
 #pragma unroll
-        for (int c = 0; c < L; ++c) hash[c] = mix32((uint32_t)((base + 4 * c) >> 2) ^ k.key);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
+        for (int r = 0; r < R; ++r) {
+            const OldBlock o(x[r], decay_m[r], decay_v[r], k);
+            float m[L], v[L];
             uint32_t top_m = 0u, top_v = 0u;
 #pragma unroll
-            for (int e = r * L; e < r * L + L; ++e) {
-                top_m = max(top_m, to_bits(m[e]) & 0x7FFFFFFFu);
-                top_v = max(top_v, to_bits(v[e]) & 0x7FFFFFFFu);
+            for (int i = 0; i < L; ++i) {
+                const int c = (r * L + i) / 4, j = (r * L + i) % 4;
+                const float out = update_coded<false>(q[c].p[0][j], scaled(q[c].g[0][j], scale), unit_at(q[c].mc[0], j), (q[c].vc[0] >> (8 * j)) & 255u, o, m[i], v[i], k);
+                p[c][0][j] = live[r] ? out : q[c].p[0][j];
+                top_m = max(top_m, to_bits(m[i]) & 0x7FFFFFFFu);
+                top_v = max(top_v, to_bits(v[i]) & 0x7FFFFFFFu);
             }
-            const int xm = block_exponent(top_m, 0x1FFFFFu, 9), xv = block_exponent(top_v, 0x0FFFFFu, 32);
+            const uint32_t xm = block_exponent(top_m, CARRY_M, LOW_M), xv = block_exponent(top_v, CARRY_V, LOW_V);
+#pragma unroll
+            for (int i = 0; i < L; ++i) {
+                const int c = (r * L + i) / 4, j = (r * L + i) % 4;
+                const uint32_t hash = mix32((b.quad + c) ^ k.key);
+                const uint32_t a = xm == 255u ? 0u : m_word(m[i], xm, bits_for_m(hash, j)) >> 24;
+                const uint32_t d = xv == 255u ? 0u : v_code(v[i], (xv - 31u) << 23, bits_for_v(hash, j));
+                mc[c] |= live[r] ? a << (8 * j) : q[c].mc[0] & (255u << (8 * j));
+                vc[c] |= live[r] ? d << (8 * j) : q[c].vc[0] & (255u << (8 * j));
+            }
             if (live[r]) x[r] = (uint16_t)(xm | xv << 8);
-#pragma unroll
-            for (int e = r * L; e < r * L + L; ++e) {
-                const int c = e / 4, j = e % 4;
-                const uint32_t bits = element_bits(hash[c], j), keep = ~(255u << (8 * j));
-                const uint32_t mc = (q[c].mc & keep) | encode_m(m[e], xm, bits) << (8 * j), vc = (q[c].vc & keep) | encode_v(v[e], xv, bits) << (8 * j);
-                q[c].mc = live[r] ? mc : q[c].mc;
-                q[c].vc = live[r] ? vc : q[c].vc;
-            }
         }
-        *(u16x4 *)(t.exponents + 2 * row0) = x;
+#pragma unroll
+        for (int c = 0; c < Q; ++c) {
+            q[c].mc[0] = mc[c];
+            q[c].vc[0] = vc[c];
+        }
+        __builtin_memcpy(__builtin_assume_aligned(b.exponents, 2 * R), x, 2 * R);
+    } else {
+#pragma unroll
+        for (int e = 0; e < R * L; ++e) {
+            const int r = e / L, c = e / 4, j = e % 4;
+            float m = q[c].m[0][j] * decay_m[r], v = q[c].v[0][j] * decay_v[r];
+            const float out = update_one<false>(q[c].p[0][j], scaled(q[c].g[0][j], scale), m, v, k);
+            p[c][0][j] = live[r] ? out : q[c].p[0][j];
+            q[c].m[0][j] = live[r] ? m : q[c].m[0][j];
+            q[c].v[0][j] = live[r] ? v : q[c].v[0][j];
+        }
     }
 #pragma unroll
-    for (int c = 0; c < L; ++c) {
-        if (!STATE8) {
-            q[c].m = f32x4{m[4 * c], m[4 * c + 1], m[4 * c + 2], m[4 * c + 3]};
-            q[c].v = f32x4{v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]};
-        }
-        q[c].store(t, base + 4 * c, p[c]);
-    }
+    for (int c = 0; c < Q; ++c) q[c].store(b, p[c]);
 }
 
 // Chunks that a form makes of a tensor (a workgroup each)
-__host__ __device__ inline long long form_chunks(int form, long long numel, int row_len, int unroll) {
+__host__ __device__ inline long long form_chunks(int form, long long numel, int row_len, int per_quads) {
     const long long units = row_len > 0 ? numel / row_len : (numel + UNIT - 1) / UNIT;
     const int group = row_len == 0 || row_len > 16 ? 16 : (row_len > 4 ? 4 : 1);
-    const int per = form == FOURS ? GS_BLOCK / 16 * unroll : form == FOURS_MASKED ? GS_BLOCK : form == NARROW ? 4 * GS_BLOCK : GS_BLOCK / group;
+    const int per = form == QUADS ? GS_BLOCK / 16 * per_quads : form == QUADS_MASKED ? GS_BLOCK : form == NARROW ? narrow_rows(row_len) * GS_BLOCK : GS_BLOCK / group;
     return (units + per - 1) / per;
 }
 
 // All tensors of one parameter type and one form of moments, whatever their shapes: the branches on `form` are uniform in a
-// workgroup, and one launch costs less than the idle lanes' registers.
-template <int UNROLL, int DT, bool MASTER, bool STATE8>
+// workgroup.  Masked tensors have a kernel of their own, whose registers would cost the others occupancy.
+template <int QUADS_A_LANE, int DT, bool MASTER, bool STATE8, bool MASKED>
 __global__ __launch_bounds__(GS_BLOCK) void adamw_kernel(AdamwBatch b) {
     const int ti = find_tensor<MAX_TENSORS>(b.first_chunk, b.n_tensors, blockIdx.x);
     const AdamwTensor &t = b.t[ti];
@@ -584,9 +690,12 @@ __global__ __launch_bounds__(GS_BLOCK) void adamw_kernel(AdamwBatch b) {
     if (!b.device_scalars) k.key = t.key;
     const float scale = b.grad_scale ? *b.grad_scale : 1.f;
     const unsigned chunk = blockIdx.x - b.first_chunk[ti];
-    if (t.form == FOURS) return step_fours<UNROLL, DT, MASTER, STATE8>(t, k, scale, chunk);
-    if constexpr (DT == GS_DTYPE_F32) {
-        if (t.form == FOURS_MASKED) return step_fours_masked<UNROLL, STATE8>(t, k, scale, chunk);
+    if constexpr (MASKED) {
+        if (t.form == QUADS_MASKED) return step_quads_masked<MASKED_ROWS / 4, STATE8>(t, k, scale, chunk);
+    } else {
+        if (t.form == QUADS) return step_quads<pairs(DT, MASTER, STATE8) ? (QUADS_A_LANE + 1) / 2 : QUADS_A_LANE, DT, MASTER, STATE8>(t, k, scale, chunk);
+    }
+    if constexpr (DT == GS_DTYPE_F32 && (MASKED || STATE8)) {
         if (t.form == NARROW) {
             if (t.row_len == 3) return step_narrow<3, STATE8>(t, k, scale, chunk);
             if (t.row_len == 1) return step_narrow<1, STATE8>(t, k, scale, chunk);
@@ -649,69 +758,75 @@ struct MomentsBatch {
 };
 static_assert(sizeof(MomentsBatch) <= 4000, "kernel arguments");
 
+__device__ __forceinline__ float v_value(uint32_t c, uint32_t x) { return v_is_nan(x) ? __builtin_nanf("") : v_of(c, v_base(x)); }
+
 template <int GROUP, int DT>
 __device__ __forceinline__ void read_unit(const MomentsTensor &t, long long unit, int unit_len) {
     const long long base = unit * unit_len, left = t.numel - base;
     const int len = left <= 0 ? 0 : (left < unit_len ? (int)left : unit_len);
     if (len == 0) return;
-    const float scale_m = exponent_scale(t.exponents[2 * unit], 9, -8), scale_v = exponent_scale(t.exponents[2 * unit + 1], 32, -31);
+    const uint32_t x = t.exponents[2 * unit] | (uint32_t)t.exponents[2 * unit + 1] << 8;
     for (int e = threadIdx.x % GROUP; e < len; e += GROUP) {
-        store_one<DT>(t.m_out, base + e, decode_m(t.m[base + e], scale_m));
-        store_one<DT>(t.v_out, base + e, decode_v(t.v[base + e], scale_v));
+        store_one<DT>(t.m_out, base + e, unit_of(t.m[base + e]) * m_scale(x));
+        store_one<DT>(t.v_out, base + e, v_value(t.v[base + e], x));
     }
 }
 
+template <int DT>
+__device__ __forceinline__ void read_four(uint32_t mc, uint32_t vc, uint32_t x, void *m_out, void *v_out, long long i) {
+    f32x4 v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = v_value((vc >> (8 * j)) & 255u, x);
+    store_four<DT>(m_out, i, units_of(mc) * m_scale(x));
+    store_four<DT>(v_out, i, v);
+}
+
 template <int UNROLL, int DT>
-__device__ __forceinline__ void read_fours(const MomentsTensor &t, unsigned chunk) {
-    constexpr int GROUP = 16, PER_PASS = GS_BLOCK / GROUP;
-    const int unit_len = t.row_len > 0 ? t.row_len : UNIT;
-    const long long chunk_unit = (long long)chunk * (PER_PASS * UNROLL), unit0 = chunk_unit + threadIdx.x / GROUP;
-    const long long whole = t.numel / unit_len;
-    const int sub = threadIdx.x % GROUP;
-    uint32_t mc[UNROLL], vc[UNROLL], x[UNROLL];
+__device__ __forceinline__ void read_quads(const MomentsTensor &t, unsigned chunk) {
+    constexpr int GROUP = 16, PER_PASS = GS_BLOCK / GROUP, SHARE = PER_PASS * UNROLL, BYTES = DT == GS_DTYPE_F32 ? 4 : 2;
+    const uint32_t unit_len = t.row_len > 0 ? t.row_len : UNIT;
+    const long long chunk_unit = (long long)chunk * SHARE, whole = t.numel / unit_len;
+    const uint32_t units = (uint32_t)min((long long)SHARE, max(0LL, whole - chunk_unit)), sub = threadIdx.x % GROUP;
+    if (units > 0) {
+        const uint8_t *m = t.m + chunk_unit * unit_len, *v = t.v + chunk_unit * unit_len, *exponents = t.exponents + 2 * chunk_unit;
+        char *m_out = (char *)t.m_out + chunk_unit * unit_len * BYTES, *v_out = (char *)t.v_out + chunk_unit * unit_len * BYTES;
+        uint32_t mc[UNROLL], vc[UNROLL], x[UNROLL], e[UNROLL];
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-        const long long unit = unit0 + u * PER_PASS;
-        mc[u] = vc[u] = x[u] = 0u;
-        if (unit < whole && 4 * sub < unit_len) {
-            mc[u] = *(const uint32_t *)(t.m + unit * unit_len + 4 * sub);
-            vc[u] = *(const uint32_t *)(t.v + unit * unit_len + 4 * sub);
-            x[u] = *(const uint16_t *)(t.exponents + 2 * unit);
+        for (int u = 0; u < UNROLL; ++u) {
+            const uint32_t unit = min(threadIdx.x / GROUP + u * PER_PASS, units - 1u);
+            e[u] = unit * unit_len + min(4u * sub, unit_len - 4u);
+            mc[u] = *(const uint32_t *)(m + e[u]);
+            vc[u] = *(const uint32_t *)(v + e[u]);
+            x[u] = *(const uint16_t *)(exponents + 2u * unit);
         }
-    }
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-        const long long unit = unit0 + u * PER_PASS;
-        f32x4 m, v;
-        decode_four(mc[u], vc[u], x[u], m, v);
-        if (unit < whole && 4 * sub < unit_len) {
-            store_four<DT>(t.m_out, unit * unit_len + 4 * sub, m);
-            store_four<DT>(t.v_out, unit * unit_len + 4 * sub, v);
-        }
+        for (int u = 0; u < UNROLL; ++u)
+            if (threadIdx.x / GROUP + u * PER_PASS < units && 4u * sub < unit_len) read_four<DT>(mc[u], vc[u], x[u], m_out, v_out, e[u]);
     }
-    if (whole * unit_len < t.numel && whole >= chunk_unit && whole < chunk_unit + PER_PASS * UNROLL && threadIdx.x < GROUP)
-        read_unit<GROUP, DT>(t, whole, unit_len);
+    if (whole * unit_len < t.numel && whole >= chunk_unit && whole < chunk_unit + SHARE && threadIdx.x < GROUP)
+        read_unit<GROUP, DT>(t, whole, (int)unit_len);
 }
 
 template <int L, int DT>
 __device__ __forceinline__ void read_narrow(const MomentsTensor &t, unsigned chunk) {
-    const long long rows = t.numel / L, row0 = 4 * ((long long)chunk * GS_BLOCK + threadIdx.x);
+    constexpr int R = narrow_rows(L), Q = R * L / 4;
+    const long long rows = t.numel / L, row0 = R * ((long long)chunk * GS_BLOCK + threadIdx.x);
     if (row0 >= rows) return;
-    if (row0 + 4 > rows) {
+    if (row0 + R > rows) {
         for (long long r = row0; r < rows; ++r) read_unit<1, DT>(t, r, L);
         return;
     }
-    typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
-    const u16x4 x = *(const u16x4 *)(t.exponents + 2 * row0);
+    uint16_t x[R];
+    __builtin_memcpy(x, __builtin_assume_aligned(t.exponents + 2 * row0, 2 * R), 2 * R);
 #pragma unroll
-    for (int c = 0; c < L; ++c) {
+    for (int c = 0; c < Q; ++c) {
         const uint32_t mc = *(const uint32_t *)(t.m + row0 * L + 4 * c), vc = *(const uint32_t *)(t.v + row0 * L + 4 * c);
-        f32x4 m, v;
+        f32x4 m = units_of(mc), v;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int r = (4 * c + j) / L;
-            m[j] = decode_m((mc >> (8 * j)) & 255u, exponent_scale(x[r] & 255, 9, -8));
-            v[j] = decode_v((vc >> (8 * j)) & 255u, exponent_scale(x[r] >> 8, 32, -31));
+            const uint32_t xr = x[(4 * c + j) / L];
+            m[j] *= m_scale(xr);
+            v[j] = v_value((vc >> (8 * j)) & 255u, xr);
         }
         store_four<DT>(t.m_out, row0 * L + 4 * c, m);
         store_four<DT>(t.v_out, row0 * L + 4 * c, v);
@@ -723,7 +838,7 @@ __global__ __launch_bounds__(GS_BLOCK) void read_moments_kernel(MomentsBatch b) 
     const int ti = find_tensor<MAX_TENSORS>(b.first_chunk, b.n_tensors, blockIdx.x);
     const MomentsTensor &t = b.t[ti];
     const unsigned chunk = blockIdx.x - b.first_chunk[ti];
-    if (t.form == FOURS) return read_fours<UNROLL, DT>(t, chunk);
+    if (t.form == QUADS) return read_quads<UNROLL, DT>(t, chunk);
     if (t.form == NARROW) {
         if (t.row_len == 3) return read_narrow<3, DT>(t, chunk);
         if (t.row_len == 1) return read_narrow<1, DT>(t, chunk);
@@ -995,24 +1110,24 @@ int element_bytes(int dtype) { return dtype == GS_DTYPE_F32 ? 4 : 2; }
 bool aligned_to(u64 p, u64 bytes) { return p % bytes == 0; }
 u64 entry(const uint64_t *column, int i) { return column ? column[i] : 0; }
 
-// Small totals get small shares, so that they still reach every compute unit: 2048 workgroups are eight for each.
-constexpr int UNROLL = 4;
-constexpr long long SMALL_CHUNKS = 2048;
+// Quads that a lane of step_quads takes.  8 bits: four, to have enough in flight; small totals one (a pair), so that they
+// still reach every compute unit.  32 bits: one, and at most four workgroups to a compute unit (OCCUPANCY_LDS bytes each of
+// shared memory that nothing uses): more requests to seven streams at once only lose the memory's open rows (1M points: four
+// quads 282 us, one 282, one with the limit 263, six streams of 1652 MB).
+constexpr int UNROLL = 4, UNROLL_READ = 4;
+constexpr int OCCUPANCY_LDS = 40960;
+constexpr long long SMALL_CHUNKS = 2048;    // of 16 units
 
-template <int U>
-void launch_step(int dtype, bool master, bool state8, const AdamwBatch &b, hipStream_t s) {
+template <int U, bool STATE8>
+void launch_step(int dtype, bool master, bool masked, const AdamwBatch &b, hipStream_t s) {
     const dim3 grid(b.first_chunk[b.n_tensors]), block(GS_BLOCK);
-#define GS_ADAMW_LAUNCH(DT, MASTER)                                                                                        \
-    do {                                                                                                                   \
-        if (state8) hipLaunchKernelGGL((adamw_kernel<U, DT, MASTER, true>), grid, block, 0, s, b);                         \
-        else hipLaunchKernelGGL((adamw_kernel<U, DT, MASTER, false>), grid, block, 0, s, b);                               \
-    } while (0)
-    if (dtype == GS_DTYPE_F32) GS_ADAMW_LAUNCH(GS_DTYPE_F32, false);
-    else if (dtype == GS_DTYPE_BF16 && master) GS_ADAMW_LAUNCH(GS_DTYPE_BF16, true);
-    else if (dtype == GS_DTYPE_BF16) GS_ADAMW_LAUNCH(GS_DTYPE_BF16, false);
-    else if (master) GS_ADAMW_LAUNCH(GS_DTYPE_F16, true);
-    else GS_ADAMW_LAUNCH(GS_DTYPE_F16, false);
-#undef GS_ADAMW_LAUNCH
+    const int lds = STATE8 ? 0 : OCCUPANCY_LDS;
+    if (masked) hipLaunchKernelGGL((adamw_kernel<1, GS_DTYPE_F32, false, STATE8, true>), grid, block, 0, s, b);
+    else if (dtype == GS_DTYPE_F32) hipLaunchKernelGGL((adamw_kernel<U, GS_DTYPE_F32, false, STATE8, false>), grid, block, lds, s, b);
+    else if (dtype == GS_DTYPE_BF16 && master) hipLaunchKernelGGL((adamw_kernel<U, GS_DTYPE_BF16, true, STATE8, false>), grid, block, lds, s, b);
+    else if (dtype == GS_DTYPE_BF16) hipLaunchKernelGGL((adamw_kernel<U, GS_DTYPE_BF16, false, STATE8, false>), grid, block, lds, s, b);
+    else if (master) hipLaunchKernelGGL((adamw_kernel<U, GS_DTYPE_F16, true, STATE8, false>), grid, block, lds, s, b);
+    else hipLaunchKernelGGL((adamw_kernel<U, GS_DTYPE_F16, false, STATE8, false>), grid, block, lds, s, b);
 }
 
 template <int U>
@@ -1075,7 +1190,7 @@ extern "C" int gs_adamw_step(int n_tensors, const uint64_t *host_param, const ui
         GS_REQUIRE(aligned_to(host_param[i] | host_grad[i], element_bytes(dt)) && aligned_to(state8 ? 0 : host_exp_avg[i] | host_exp_avg_sq[i], 4) &&
                        aligned_to(entry(host_master, i) | (entry(host_row_mask, i) ? host_last_step[i] : 0), 4),
                    "gs_adamw_step: an address is no multiple of its type's size");
-        units_of_16 += form_chunks(FOURS, n, row, 1);
+        units_of_16 += form_chunks(QUADS, n, row, 1);
     }
     {
         Range *r = (Range *)malloc((size_t)n_tensors * 7 * sizeof(Range));
@@ -1098,32 +1213,35 @@ extern "C" int gs_adamw_step(int n_tensors, const uint64_t *host_param, const ui
     }
     hipStream_t s = (hipStream_t)stream;
     AdamwScalars *device_scalars = (AdamwScalars *)workspace;
-    const int unroll = units_of_16 <= SMALL_CHUNKS ? 1 : UNROLL;
+    const int unroll = !state8 || units_of_16 <= SMALL_CHUNKS ? 1 : UNROLL;
     StepBatch q;
     q.b.grad_scale = grad_scale;
-    // one type after the other: (parameter type, master copy)
+    // one type after the other: float, float under a mask, 16 bits with and without a master copy
     for (int kind = 0; kind < 6; ++kind) {
         const int dtype = kind / 2;
-        const bool master = kind % 2 != 0;
+        const bool masked = kind == 1, master = kind > 1 && kind % 2 != 0;
         q.clear();
         for (int i = 0; i <= n_tensors; ++i) {
             const bool end = i == n_tensors;
-            if (!end && (host_numel[i] == 0 || host_dtype[i] != dtype || (entry(host_master, i) != 0) != master)) continue;
+            if (!end && (host_numel[i] == 0 || host_dtype[i] != dtype || (entry(host_master, i) != 0) != master ||
+                         (entry(host_row_mask, i) != 0) != masked)) continue;
             AdamwTensor t = {};
             long long chunks = 0;
             int set = 0;
             if (!end) {
                 const u64 mask = entry(host_row_mask, i);
                 const int row = mask || state8 ? host_row_len[i] : 0;      // (moments in 32 bits without a mask: units of 64 whatever the shape)
-                const bool fours = aligned_to(host_param[i] | host_grad[i], 4 * element_bytes(dtype)) &&
-                                   aligned_to(host_exp_avg[i] | host_exp_avg_sq[i], state8 ? 4 : 16) &&
-                                   aligned_to(master ? host_master[i] : 0, 16) && aligned_to(state8 ? host_exponents[i] : 0, 2);
-                const bool narrow = fours && dtype == GS_DTYPE_F32 && aligned_to(state8 ? host_exponents[i] : 0, 8) && aligned_to(mask, 4) &&
-                                    aligned_to(mask ? host_last_step[i] : 0, 16);
-                t.form = row >= 1 && row <= 4 && narrow ? NARROW : fours && (row == 0 || (row > 16 && row % 4 == 0)) ? (mask ? FOURS_MASKED : FOURS) : ELEMENTS;
+                const bool pair = pairs(dtype, master, state8);
+                const u64 moments = host_exp_avg[i] | host_exp_avg_sq[i];
+                const bool values = aligned_to(host_param[i] | host_grad[i], pair ? 16 : 4 * element_bytes(dtype)) && aligned_to(master ? host_master[i] : 0, 16);
+                const bool quads = values && (row == 0 || (row > 16 && row % (pair ? 8 : 4) == 0)) &&
+                                   aligned_to(moments, pair ? 8 : state8 ? 4 : 16) && aligned_to(entry(host_exponents, i), 2);
+                const bool narrow = values && dtype == GS_DTYPE_F32 && row >= 1 && row <= 4 && aligned_to(moments, state8 ? 4 : 16) &&
+                                    aligned_to(entry(host_exponents, i), 8) && aligned_to(mask, 4) && aligned_to(mask ? host_last_step[i] : 0, 16);
+                t.form = narrow ? NARROW : quads ? (mask ? QUADS_MASKED : QUADS) : ELEMENTS;
                 t.row_len = (uint8_t)row;
                 t.masked = mask != 0;
-                chunks = form_chunks(t.form, host_numel[i], row, unroll);
+                chunks = form_chunks(t.form, host_numel[i], row, pair ? std::max(2, unroll) : unroll);
                 while (!on_device && set < q.n_sets &&
                        (q.step[set] != host_step[i] || memcmp(q.hyper[set], host_hyper + 5 * (size_t)i, 5 * sizeof(double)) != 0)) ++set;
             }
@@ -1136,8 +1254,9 @@ extern "C" int gs_adamw_step(int n_tensors, const uint64_t *host_param, const ui
                     hipLaunchKernelGGL(adamw_prepare_kernel, dim3(1), dim3(GS_WAVE), 0, s, q.prep, device_scalars);
                     device_scalars += q.b.n_tensors;      // (every batch has its own part: n_tensors in all)
                 }
-                if (unroll == 1) launch_step<1>(dtype, master, state8, q.b, s);
-                else launch_step<UNROLL>(dtype, master, state8, q.b, s);
+                if (!state8) launch_step<1, false>(dtype, master, masked, q.b, s);
+                else if (unroll == 1) launch_step<1, true>(dtype, master, masked, q.b, s);
+                else launch_step<UNROLL, true>(dtype, master, masked, q.b, s);
                 if (const int status = launch_status("gs_adamw_step")) return status;
                 q.clear();
                 set = 0;
@@ -1190,9 +1309,9 @@ extern "C" int gs_read_moments(int n_tensors, const uint64_t *host_exp_avg, cons
         GS_REQUIRE(n == 0 || (host_exp_avg[i] && host_exp_avg_sq[i] && host_exponents[i] && host_m_out[i] && host_v_out[i]),
                    "gs_read_moments: null tensor");
         GS_REQUIRE(aligned_to(host_m_out[i] | host_v_out[i], element_bytes(out_dtype)), "gs_read_moments: misaligned output");
-        units_of_16 += form_chunks(FOURS, n, row, 1);
+        units_of_16 += form_chunks(QUADS, n, row, 1);
     }
-    const int unroll = units_of_16 <= SMALL_CHUNKS ? 1 : UNROLL;
+    const int unroll = units_of_16 <= SMALL_CHUNKS ? 1 : UNROLL_READ;
     MomentsBatch b;
     b.n_tensors = 0;
     b.first_chunk[0] = 0;
@@ -1207,12 +1326,12 @@ extern "C" int gs_read_moments(int n_tensors, const uint64_t *host_exp_avg, cons
                                aligned_to(host_exponents[i], 2);
             t = {(const uint8_t *)host_exp_avg[i], (const uint8_t *)host_exp_avg_sq[i], (const uint8_t *)host_exponents[i],
                  (void *)host_m_out[i], (void *)host_v_out[i], host_numel[i], row, 0};
-            t.form = row >= 1 && row <= 4 && fours && aligned_to(host_exponents[i], 8) ? NARROW : fours && (row == 0 || (row > 16 && row % 4 == 0)) ? FOURS : ELEMENTS;
+            t.form = row >= 1 && row <= 4 && fours && aligned_to(host_exponents[i], 8) ? NARROW : fours && (row == 0 || (row > 16 && row % 4 == 0)) ? QUADS : ELEMENTS;
             chunks = form_chunks(t.form, host_numel[i], row, unroll);
         }
         if (b.n_tensors > 0 && (end || b.n_tensors == MAX_TENSORS || (long long)b.first_chunk[b.n_tensors] + chunks >= 0x7fffffffLL)) {
             if (unroll == 1) launch_moments<1>(out_dtype, b, (hipStream_t)stream);
-            else launch_moments<UNROLL>(out_dtype, b, (hipStream_t)stream);
+            else launch_moments<UNROLL_READ>(out_dtype, b, (hipStream_t)stream);
             if (const int status = launch_status("gs_read_moments")) return status;
             b.n_tensors = 0;
         }
