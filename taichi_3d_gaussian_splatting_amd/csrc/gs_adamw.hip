@@ -21,8 +21,12 @@ typedef unsigned long long u64;
 constexpr int UNIT = 64;            // elements of a block where blocks are not rows
 constexpr int MAX_TENSORS = 48;     // a batch's table is 3.9 KB of kernel arguments
 constexpr int MAX_SETS = 4;         // different (learning rate, step, ...) in a batch
-constexpr int MAX_NORM_TENSORS = 160, MAX_NORM_MASKED = 64;
-constexpr int NORM_PARTIALS = 4096; // most workgroups that the norm's first pass aims at, beyond one for each tensor
+constexpr int MAX_NORM_TENSORS = 192, MAX_NORM_MASKED = 64;
+// Most workgroups that the norm's first pass aims at, beyond one for each tensor: a round of eight to a compute unit.
+constexpr int NORM_PARTIALS = 2000;
+// Gradients of more bytes than this pass the caches by: what is read next (a clipped step's first gradients) is gone by
+// then.  Below, the step finds them there.  (944 MB: 205 -> 185 us by, 109 MB and a step: 273 us through, 285 by.)
+constexpr long long NORM_STREAM_BYTES = 128LL << 20;
 
 // What a step needs besides the tensors; key and step belong to one tensor
 struct AdamwScalars {
@@ -777,8 +781,10 @@ __device__ __forceinline__ void read_four(uint32_t mc, uint32_t vc, uint32_t x, 
     f32x4 v;
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = v_value((vc >> (8 * j)) & 255u, x);
-    store_four<DT>(m_out, i, units_of(mc) * m_scale(x));
-    store_four<DT>(v_out, i, v);
+    // (whole cache lines, not read again soon: 240 -> 227 us for a step of 1M points and this, the codes from the caches)
+    typedef typename Four<DT>::type Value;
+    stream_store((char *)m_out + i * (long long)(sizeof(Value) / 4), __builtin_convertvector(units_of(mc) * m_scale(x), Value));
+    stream_store((char *)v_out + i * (long long)(sizeof(Value) / 4), __builtin_convertvector(v, Value));
 }
 
 template <int UNROLL, int DT>
@@ -861,9 +867,9 @@ struct NormTensor {
 };
 struct NormBatch {              // tensors without a row mask
     int n_tensors;
-    unsigned chunk;             // elements, a multiple of 1024
+    unsigned chunk;             // elements, a multiple of NORM_STEP
+    int first_id;               // of the first tensor in the caller's list; the others follow it
     unsigned first_block[MAX_NORM_TENSORS + 1];
-    int id[MAX_NORM_TENSORS];   // place in the caller's list
     NormTensor t[MAX_NORM_TENSORS];
 };
 struct NormMaskedTensor {
@@ -881,10 +887,12 @@ struct NormMaskedBatch {
 };
 static_assert(sizeof(NormBatch) <= 4000 && sizeof(NormMaskedBatch) <= 4000, "kernel arguments");
 
+constexpr int NORM_STEP = 4096;     // what a workgroup has in flight of float gradients
+
 // Rows of a masked tensor that a workgroup of the first pass takes: at least a chunk's elements, so that there are no more
-// parts than without a mask; whole waves' worth of rows
+// parts than without a mask; whole workgroups' worth of rows
 __host__ __device__ __forceinline__ long long norm_rows(long long chunk, int row_len) {
-    return ((chunk + row_len - 1) / row_len + 63) / 64 * 64;
+    return ((chunk + row_len - 1) / row_len + GS_BLOCK - 1) / GS_BLOCK * GS_BLOCK;
 }
 
 __device__ __forceinline__ double wave_sum(double x) {
@@ -911,25 +919,26 @@ __device__ __forceinline__ double add_squares(double s, V x) {
     return s;
 }
 
-// Elements begin..end (begin is a multiple of 1024: the chunk is aligned where the tensor is): 16 bytes a lane, four requests
-// in flight.
-template <int DT>
+// Elements begin..end (begin is a multiple of 16 bytes: the chunk is aligned where the tensor is): 16 bytes a lane, AHEAD
+// requests in flight, past the end none.
+template <int DT, bool STREAM>
 __device__ __forceinline__ double flat_squares(const void *grad, long long begin, long long end) {
     typedef typename Wide<DT>::type V;
     constexpr int N = 16 / (DT == GS_DTYPE_F32 ? 4 : 2), AHEAD = 4;
     double s = 0.0;
-    const long long wide = ((uintptr_t)grad & 15) == 0 ? (end - begin) / N : 0;
+    const unsigned wide = ((uintptr_t)grad & 15) == 0 ? (unsigned)((end - begin) / N) : 0u;
     const V *g = (const V *)((const char *)grad + begin * (16 / N));
-    long long q = threadIdx.x;
-    for (; q + (AHEAD - 1) * GS_BLOCK < wide; q += AHEAD * GS_BLOCK) {
+    for (unsigned q = threadIdx.x; q < wide; q += AHEAD * GS_BLOCK) {
         V x[AHEAD];
 #pragma unroll
-        for (int a = 0; a < AHEAD; ++a) x[a] = g[q + a * GS_BLOCK];
+        for (int a = 0; a < AHEAD; ++a) {
+            x[a] = {};
+            if (q + a * GS_BLOCK < wide) x[a] = STREAM ? __builtin_nontemporal_load(g + q + a * GS_BLOCK) : g[q + a * GS_BLOCK];
+        }
 #pragma unroll
         for (int a = 0; a < AHEAD; ++a) s = add_squares<N>(s, x[a]);
     }
-    for (; q < wide; q += GS_BLOCK) s = add_squares<N>(s, g[q]);
-    for (long long i = begin + N * wide + threadIdx.x; i < end; i += GS_BLOCK) {
+    for (long long i = begin + (long long)N * wide + threadIdx.x; i < end; i += GS_BLOCK) {
         const double x = (double)load_one<DT>(grad, i);
         s = fma(x, x, s);
     }
@@ -1030,6 +1039,7 @@ __device__ __forceinline__ void leave_partial(double s, unsigned base, unsigned 
     }
 }
 
+template <bool STREAM>
 __global__ __launch_bounds__(GS_BLOCK) void norm_partial_kernel(NormBatch b, unsigned base, double *__restrict__ partials, uint2 *__restrict__ spans) {
     const int ti = find_tensor<MAX_NORM_TENSORS>(b.first_block, b.n_tensors, blockIdx.x);
     const unsigned part = blockIdx.x - b.first_block[ti];
@@ -1038,10 +1048,10 @@ __global__ __launch_bounds__(GS_BLOCK) void norm_partial_kernel(NormBatch b, uns
     const long long end = min(numel, begin + (long long)b.chunk);
     const int type = (int)(b.t[ti].numel_type & 3);
     double s;
-    if (type == GS_DTYPE_F32) s = flat_squares<GS_DTYPE_F32>(grad, begin, end);
-    else if (type == GS_DTYPE_BF16) s = flat_squares<GS_DTYPE_BF16>(grad, begin, end);
-    else s = flat_squares<GS_DTYPE_F16>(grad, begin, end);
-    leave_partial(s, base, part, b.first_block[ti + 1] - b.first_block[ti], b.id[ti], partials, spans);
+    if (type == GS_DTYPE_F32) s = flat_squares<GS_DTYPE_F32, STREAM>(grad, begin, end);
+    else if (type == GS_DTYPE_BF16) s = flat_squares<GS_DTYPE_BF16, STREAM>(grad, begin, end);
+    else s = flat_squares<GS_DTYPE_F16, STREAM>(grad, begin, end);
+    leave_partial(s, base, part, b.first_block[ti + 1] - b.first_block[ti], b.first_id + ti, partials, spans);
 }
 
 __global__ __launch_bounds__(GS_BLOCK) void norm_masked_kernel(NormMaskedBatch b, unsigned base, double *__restrict__ partials, uint2 *__restrict__ spans) {
@@ -1353,7 +1363,7 @@ extern "C" int gs_grad_norm(int n_tensors, const uint64_t *host_grad, const uint
     GS_REQUIRE(n_tensors >= 1 && n_tensors <= (1 << 20), "gs_grad_norm: 1 to 2^20 tensors");
     GS_REQUIRE(host_grad && host_numel && host_row_len && host_dtype && sq_sum && norm && clip && workspace, "gs_grad_norm: null pointer");
     GS_REQUIRE(((uintptr_t)workspace & 7) == 0, "gs_grad_norm: the workspace must be 8-byte aligned");
-    long long total = 0;
+    long long total = 0, bytes = 0;
     for (int i = 0; i < n_tensors; ++i) {
         const long long n = host_numel[i];
         const int dt = host_dtype[i];
@@ -1362,10 +1372,11 @@ extern "C" int gs_grad_norm(int n_tensors, const uint64_t *host_grad, const uint
         GS_REQUIRE(n == 0 || (host_grad[i] && aligned_to(host_grad[i], element_bytes(dt))), "gs_grad_norm: null or misaligned tensor");
         GS_REQUIRE(!entry(host_row_mask, i) || (host_row_len[i] > 0 && host_row_len[i] <= UNIT && n % host_row_len[i] == 0), "gs_grad_norm: a row mask needs rows");
         total += n;
+        bytes += n * element_bytes(dt);
     }
-    // chunks of a multiple of 1024 elements, so that there are at most NORM_PARTIALS of them and one more for each tensor
+    // chunks of a multiple of NORM_STEP elements, so that there are at most NORM_PARTIALS of them and one more for each tensor
     long long chunk = (total + NORM_PARTIALS - 1) / NORM_PARTIALS;
-    chunk = chunk < 4096 ? 4096 : (chunk + 1023) / 1024 * 1024;
+    chunk = chunk < NORM_STEP ? NORM_STEP : (chunk + NORM_STEP - 1) / NORM_STEP * NORM_STEP;
     GS_REQUIRE(chunk < 0x7fffffffLL, "gs_grad_norm: too many elements");
     hipStream_t s = (hipStream_t)stream;
     double *partials = (double *)workspace;
@@ -1377,18 +1388,20 @@ extern "C" int gs_grad_norm(int n_tensors, const uint64_t *host_grad, const uint
     b.n_tensors = 0;
     b.first_block[0] = 0;
     for (int i = 0; i <= n_tensors; ++i) {
-        const bool end = i == n_tensors;
-        if (!end && entry(host_row_mask, i)) continue;
-        if (b.n_tensors > 0 && (end || b.n_tensors == MAX_NORM_TENSORS)) {
-            hipLaunchKernelGGL(norm_partial_kernel, dim3(b.first_block[b.n_tensors]), dim3(GS_BLOCK), 0, s, b, n_partials, partials, spans);
+        const bool end = i == n_tensors, other = !end && entry(host_row_mask, i);
+        if (b.n_tensors > 0 && (end || other || b.n_tensors == MAX_NORM_TENSORS)) {
+            const dim3 grid(b.first_block[b.n_tensors]), block(GS_BLOCK);
+            if (bytes > NORM_STREAM_BYTES) hipLaunchKernelGGL(norm_partial_kernel<true>, grid, block, 0, s, b, n_partials, partials, spans);
+            else hipLaunchKernelGGL(norm_partial_kernel<false>, grid, block, 0, s, b, n_partials, partials, spans);
             GS_CHECK_LAUNCH();
             n_partials += b.first_block[b.n_tensors];
             b.n_tensors = 0;
         }
         if (end) break;
+        if (other) continue;
+        if (b.n_tensors == 0) b.first_id = i;
         const long long parts = host_numel[i] == 0 ? 1 : (host_numel[i] + chunk - 1) / chunk;
         b.t[b.n_tensors] = {(const void *)host_grad[i], (u64)host_numel[i] << 2 | (u64)host_dtype[i]};
-        b.id[b.n_tensors] = i;
         b.first_block[b.n_tensors + 1] = b.first_block[b.n_tensors] + (unsigned)parts;
         ++b.n_tensors;
     }

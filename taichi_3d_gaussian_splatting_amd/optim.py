@@ -145,23 +145,27 @@ def _on(device_index: int):
     return contextlib.nullcontext() if torch.cuda.current_device() == device_index else torch.cuda.device(device_index)
 
 
-def _norm_of(collected, masks, max_norm: float, each: bool, group=None):
-    """(norm, clip, each | None) of collected gradients, on their device's current stream."""
+def _stream(device_index: int) -> int:
+    """Handle of the current stream (``_lib.current_stream`` without the stream object: a step is 13 us in all)."""
+    return torch._C._cuda_getCurrentRawStream(device_index)
+
+
+def _norm_of(collected, masks, max_norm: float, each: bool, group=None) -> torch.Tensor:
+    """[norm, clip, each ...] of collected gradients, on their device's current stream."""
     (grads, *_), numel, rows, types, index, _ = collected
     device, n = torch.device("cuda", index), len(numel) // 8
     out = torch.empty(2 + (n if each else 0), dtype=torch.float32, device=device)
     floats = out.data_ptr()
-    bytes_needed = int(_lib.load().gs_grad_norm_workspace_bytes(n))
-    workspace = torch.empty(1 + (bytes_needed + 7) // 8, dtype=torch.float64, device=device)     # [0]: the sum of squares
-    sq_sum = workspace.data_ptr()
+    workspace = torch.empty(1 + (_lib.load().gs_grad_norm_workspace_bytes(n) + 7) // 8, dtype=torch.float64, device=device)
+    sq_sum = workspace.data_ptr()       # the sum of squares, then the library's own
     with _on(index):
-        stream = current_stream(device)
+        stream = _stream(index)
         call("gs_grad_norm", n, grads, masks, numel, rows, types, max_norm, sq_sum, floats, floats + 4,
              floats + 8 if each else None, sq_sum + 8, stream)
         if group is not None:
             _sum_over_ranks(workspace[:1], group)
             call("gs_clip_coefficient", sq_sum, max_norm, floats, floats + 4, stream)
-    return out[0], out[1], out[2:] if each else None
+    return out
 
 
 def _sum_over_ranks(value: torch.Tensor, group) -> None:
@@ -185,8 +189,8 @@ def grad_norm(grads: Sequence[torch.Tensor], row_masks: Optional[Sequence[Option
         raise ValueError("grad_norm: no gradients")
     host = _lib.host()
     collected = host.collect(("grads", grads, host.GRADS), ("row_masks", row_masks, host.MASK))
-    norm, _, each = _norm_of(collected, collected[0][1], 0.0, per_tensor)
-    return (norm, each) if per_tensor else norm
+    out = _norm_of(collected, collected[0][1], 0.0, per_tensor)
+    return (out[0], out[2:]) if per_tensor else out[0]
 
 
 @torch.no_grad()
@@ -255,20 +259,20 @@ def adamw_step_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], e
     if numbers and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("a captured step needs its step count in a device tensor: a number would be the same at every replay")
 
-    norm = clip = None
+    norms = clip = None
     if max_grad_norm is not None:
-        norm, clip, _ = _norm_of((columns[1:2], numel, rows, types, index, kept), columns[6], float(max_grad_norm), False, norm_group)
+        norms = _norm_of((columns[1:2], numel, rows, types, index, kept), columns[6], float(max_grad_norm), False, norm_group)
+        clip = norms.data_ptr() + 4
     elif grad_scale is not None:
-        clip = grad_scale
+        clip = grad_scale.data_ptr()
     ids = array("i", range(n) if tensor_ids is None else tensor_ids)
     workspace = None
     if step_tensors is not None or rate_tensors is not None:
         workspace = torch.empty(int(_lib.load().gs_adamw_workspace_bytes(n)), dtype=torch.uint8, device=device)
     with _on(index):
         call("gs_adamw_step", n, *columns, numel, rows, types, ids.buffer_info()[0], hyper, counts, step_tensors, rate_tensors,
-             None if clip is None else clip.data_ptr(), seed & 0xFFFFFFFF,
-             None if workspace is None else workspace.data_ptr(), current_stream(device))
-    return norm
+             clip, seed & 0xFFFFFFFF, None if workspace is None else workspace.data_ptr(), _stream(index))
+    return None if norms is None else norms[0]
 
 
 @torch.no_grad()
@@ -297,7 +301,7 @@ def read_moments(exp_avgs: Sequence[torch.Tensor], exp_avg_sqs: Sequence[torch.T
         if out[1][0].dtype is not dtype:
             raise TypeError("out: both lists have one type")
     with _on(index):
-        call("gs_read_moments", n, m, v, x, m_out, v_out, numel, rows, _DTYPES[dtype], current_stream(torch.device("cuda", index)))
+        call("gs_read_moments", n, m, v, x, m_out, v_out, numel, rows, _DTYPES[dtype], _stream(index))
     return out
 
 
@@ -412,8 +416,9 @@ class AdamW(torch.optim.Optimizer):
         host = _lib.host()
         grads, masks = [g for columns in parts for g in columns[1]], [mask for columns in parts for mask in columns[6]]
         collected = host.collect(("grads", grads, host.GRADS), ("row_masks", masks, host.MASK))
-        self.last_grad_norm, clip, _ = _norm_of(collected, collected[0][1], float(self.max_grad_norm), False, self.norm_group)
-        return clip
+        norms = _norm_of(collected, collected[0][1], float(self.max_grad_norm), False, self.norm_group)
+        self.last_grad_norm = norms[0]
+        return norms[1]
 
     def moments(self, param: torch.Tensor, dtype: torch.dtype = torch.float32) -> Tuple[torch.Tensor, torch.Tensor]:
         """Values of a parameter's first and second moment, whatever they are held in."""

@@ -163,4 +163,4 @@ def test_c_entries_with_nothing_to_do_or_missing_arguments():
     assert lib.gs_grad_norm(0, *[None] * 5, 0.0, *[None] * 6) == -1
     assert lib.gs_clip_coefficient(None, 1.0, None, None, None) == -1
     assert lib.gs_adamw_workspace_bytes(3) >= 3 * 40 and lib.gs_adamw_workspace_bytes(-1) == 0
-    assert lib.gs_grad_norm_workspace_bytes(3) >= 8 * 4099 and lib.gs_grad_norm_workspace_bytes(-1) == 0
+    assert lib.gs_grad_norm_workspace_bytes(3) >= 8 * 2003 and lib.gs_grad_norm_workspace_bytes(-1) == 0
