@@ -198,6 +198,9 @@ def host():
         except ImportError as e:
             raise RuntimeError(f"_gs_host is missing or does not load ({e}): build it with `make -C {os.path.join(_HERE, 'csrc')}` "
                                "(or __graft_entry__.build()).  There is no fallback path.") from e
+        lib = load()
+        _gs_host.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
+                        for name in ("gs_adamw_step", "gs_grad_norm", "gs_read_moments")))
         _host = _gs_host
     return _host
 

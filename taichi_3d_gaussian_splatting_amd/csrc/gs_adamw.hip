@@ -1321,6 +1321,22 @@ extern "C" int gs_read_moments(int n_tensors, const uint64_t *host_exp_avg, cons
         GS_REQUIRE(aligned_to(host_m_out[i] | host_v_out[i], element_bytes(out_dtype)), "gs_read_moments: misaligned output");
         units_of_16 += form_chunks(QUADS, n, row, 1);
     }
+    {
+        Range *r = (Range *)malloc((size_t)n_tensors * 5 * sizeof(Range));
+        GS_REQUIRE(r != nullptr, "gs_read_moments: out of host memory");
+        size_t k = 0;
+        for (int i = 0; i < n_tensors; ++i) {
+            const u64 n = (u64)host_numel[i], oe = n * element_bytes(out_dtype), row = (u64)host_row_len[i], blocks = row > 0 ? n / row : (n + UNIT - 1) / UNIT;
+            r[k++] = {host_exp_avg[i], host_exp_avg[i] + n, 0};
+            r[k++] = {host_exp_avg_sq[i], host_exp_avg_sq[i] + n, 0};
+            r[k++] = {host_exponents[i], host_exponents[i] + 2 * blocks, 0};
+            r[k++] = {host_m_out[i], host_m_out[i] + oe, 1};
+            r[k++] = {host_v_out[i], host_v_out[i] + oe, 1};
+        }
+        const bool meet = ranges_meet(r, k);
+        free(r);
+        GS_REQUIRE(!meet, "gs_read_moments: an output overlaps another buffer");
+    }
     const int unroll = units_of_16 <= SMALL_CHUNKS ? 1 : UNROLL_READ;
     MomentsBatch b;
     b.n_tensors = 0;

@@ -1,8 +1,9 @@
-// gs_host.cpp -- argument checks and address columns for the operators on lists of tensors (optim.py), as a CPython module.
+// gs_host.cpp -- argument checks, address columns and the library calls of the operators on lists of tensors (optim.py), as a
+// CPython module.
 //
 // A step of 180 tensors looks at five to eight properties of some 900 tensor objects.  Python spends 0.3 us on each object
-// (0.25 ms a step, as long as the kernels run); reading the same fields from C++ takes 0.03 us.  The module keeps nothing
-// between calls.
+// (0.25 ms a step, as long as the kernels run); reading the same fields from C++ takes 0.03 us, and a call
+// of twenty arguments 0.1 us where ctypes takes 3.  The module keeps nothing between calls but the library's addresses.
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
@@ -11,6 +12,8 @@
 
 #include <string>
 #include <vector>
+
+#include "../../include/gsplat_hip.h"
 
 namespace {
 
@@ -243,6 +246,91 @@ PyObject *scalars_checked(PyObject *args) {
     return Py_BuildValue("(OOOOO)", a.o, b.o, c.o, d.o, number ? Py_True : Py_False);
 }
 
+// The library's entry points: it is loaded by the package (which checks its version), not linked here.
+decltype(&gs_adamw_step) adamw_step = nullptr;
+decltype(&gs_grad_norm) grad_norm = nullptr;
+decltype(&gs_read_moments) read_moments = nullptr;
+
+PyObject *bind(PyObject *args) {
+    unsigned long long a, b, c;
+    if (!PyArg_ParseTuple(args, "KKK", &a, &b, &c)) return nullptr;
+    adamw_step = reinterpret_cast<decltype(adamw_step)>(a);
+    grad_norm = reinterpret_cast<decltype(grad_norm)>(b);
+    read_moments = reinterpret_cast<decltype(read_moments)>(c);
+    Py_RETURN_NONE;
+}
+
+// The data of a column (bytes), null for None
+template <typename T>
+const T *column(PyObject *o) {
+    if (o == Py_None) return nullptr;
+    if (!PyBytes_Check(o)) throw Refused{PyExc_TypeError, "a column of collect() or scalars()"};
+    return reinterpret_cast<const T *>(PyBytes_AS_STRING(o));
+}
+template <typename T>
+const T *column(PyObject *tuple, Py_ssize_t i) { return column<T>(PyTuple_GET_ITEM(tuple, i)); }
+
+PyObject *tuple_of(PyObject *o, Py_ssize_t n) {
+    if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) < n) throw Refused{PyExc_TypeError, "a tuple of collect() or scalars()"};
+    return o;
+}
+
+// step(collected, scalars, ids or None, grad scale address, seed, workspace address, stream): status of gs_adamw_step.
+// `collected`: params, grads, exp_avgs, exp_avg_sqs, exponents, masters, row masks, last steps.
+PyObject *step(PyObject *args) {
+    PyObject *collected, *numbers, *ids;
+    unsigned long long scale, workspace, stream;
+    unsigned int seed;
+    if (!PyArg_ParseTuple(args, "OOOKIKK", &collected, &numbers, &ids, &scale, &seed, &workspace, &stream)) return nullptr;
+    PyObject *c = tuple_of(PyTuple_GET_ITEM(tuple_of(collected, 4), 0), 8);
+    tuple_of(numbers, 4);
+    const Py_ssize_t n = PyBytes_GET_SIZE(PyTuple_GET_ITEM(collected, 1)) / 8;
+    std::vector<int32_t> id(n);
+    if (ids != Py_None) {
+        Holder fast(PySequence_Fast(ids, "tensor_ids: a sequence of numbers"));
+        if (!fast.o) return nullptr;
+        if (PySequence_Fast_GET_SIZE(fast.o) != n) throw Refused{PyExc_ValueError, "tensor_ids: one for each tensor"};
+        for (Py_ssize_t i = 0; i < n; ++i) {
+            id[i] = (int32_t)PyLong_AsLong(PySequence_Fast_GET_ITEM(fast.o, i));
+            if (id[i] == -1 && PyErr_Occurred()) return nullptr;
+        }
+    } else {
+        for (Py_ssize_t i = 0; i < n; ++i) id[i] = (int32_t)i;
+    }
+    if (!adamw_step) throw Refused{PyExc_RuntimeError, "the library is not bound"};
+    typedef uint64_t U;
+    return PyLong_FromLong(adamw_step((int)n, column<U>(c, 0), column<U>(c, 1), column<U>(c, 2), column<U>(c, 3), column<U>(c, 4), column<U>(c, 5),
+                                      column<U>(c, 6), column<U>(c, 7), column<int64_t>(collected, 1), column<int32_t>(collected, 2), column<int32_t>(collected, 3),
+                                      id.data(), column<double>(numbers, 0), column<int64_t>(numbers, 1), column<U>(numbers, 2), column<U>(numbers, 3),
+                                      (const float *)scale, seed, (void *)workspace, (void *)stream));
+}
+
+// norm(grads column, row mask column, collected, max_norm, sq_sum, norm, clip, each or 0, workspace, stream): status of gs_grad_norm
+PyObject *norm(PyObject *args) {
+    PyObject *grads, *masks, *collected;
+    double max_norm;
+    unsigned long long sq_sum, total, clip, each, workspace, stream;
+    if (!PyArg_ParseTuple(args, "OOOdKKKKKK", &grads, &masks, &collected, &max_norm, &sq_sum, &total, &clip, &each, &workspace, &stream)) return nullptr;
+    tuple_of(collected, 4);
+    if (!grad_norm) throw Refused{PyExc_RuntimeError, "the library is not bound"};
+    return PyLong_FromLong(grad_norm((int)(PyBytes_GET_SIZE(PyTuple_GET_ITEM(collected, 1)) / 8), column<uint64_t>(grads), column<uint64_t>(masks),
+                                     column<int64_t>(collected, 1), column<int32_t>(collected, 2), column<int32_t>(collected, 3), max_norm, (double *)sq_sum,
+                                     (float *)total, (float *)clip, (float *)each, (void *)workspace, (void *)stream));
+}
+
+// read(collected, type code, stream): status of gs_read_moments.  `collected`: exp_avgs, exp_avg_sqs, exponents and the two outputs.
+PyObject *read(PyObject *args) {
+    PyObject *collected;
+    int dtype;
+    unsigned long long stream;
+    if (!PyArg_ParseTuple(args, "OiK", &collected, &dtype, &stream)) return nullptr;
+    PyObject *c = tuple_of(PyTuple_GET_ITEM(tuple_of(collected, 4), 0), 5);
+    if (!read_moments) throw Refused{PyExc_RuntimeError, "the library is not bound"};
+    typedef uint64_t U;
+    return PyLong_FromLong(read_moments((int)(PyBytes_GET_SIZE(PyTuple_GET_ITEM(collected, 1)) / 8), column<U>(c, 0), column<U>(c, 1), column<U>(c, 2),
+                                        column<U>(c, 3), column<U>(c, 4), column<int64_t>(collected, 1), column<int32_t>(collected, 2), dtype, (void *)stream));
+}
+
 template <PyObject *(*F)(PyObject *)>
 PyObject *guarded(PyObject *, PyObject *args) {
     try {
@@ -258,6 +346,10 @@ PyObject *guarded(PyObject *, PyObject *args) {
 PyMethodDef methods[] = {
     {"collect", guarded<collect_checked>, METH_VARARGS, "collect((name, tensors or None, kind), ...): checked address columns"},
     {"scalars", guarded<scalars_checked>, METH_VARARGS, "scalars(n, step, lr, weight_decay, beta1, beta2, eps, device): checked number columns"},
+    {"bind", guarded<bind>, METH_VARARGS, "bind(gs_adamw_step, gs_grad_norm, gs_read_moments): the library's addresses"},
+    {"step", guarded<step>, METH_VARARGS, "gs_adamw_step on collected columns"},
+    {"norm", guarded<norm>, METH_VARARGS, "gs_grad_norm on collected columns"},
+    {"read", guarded<read>, METH_VARARGS, "gs_read_moments on collected columns"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_gs_host", "argument columns of the operators on lists of tensors", -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -12,13 +12,12 @@ are functions on lists of tensors: ``adamw_step_``, ``grad_norm``, ``read_moment
 from __future__ import annotations
 
 import contextlib
-from array import array
 from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
 from . import _lib
-from ._lib import call, current_stream, ptr
+from ._lib import call, check, current_stream, ptr
 
 
 class Adam(torch.optim.Optimizer):
@@ -150,18 +149,17 @@ def _stream(device_index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(device_index)
 
 
-def _norm_of(collected, masks, max_norm: float, each: bool, group=None) -> torch.Tensor:
+def _norm_of(host, collected, grads, masks, max_norm: float, each: bool, group=None) -> torch.Tensor:
     """[norm, clip, each ...] of collected gradients, on their device's current stream."""
-    (grads, *_), numel, rows, types, index, _ = collected
-    device, n = torch.device("cuda", index), len(numel) // 8
+    index = collected[4]
+    device, n = torch.device("cuda", index), len(collected[1]) // 8
     out = torch.empty(2 + (n if each else 0), dtype=torch.float32, device=device)
-    floats = out.data_ptr()
     workspace = torch.empty(1 + (_lib.load().gs_grad_norm_workspace_bytes(n) + 7) // 8, dtype=torch.float64, device=device)
-    sq_sum = workspace.data_ptr()       # the sum of squares, then the library's own
+    floats, sq_sum = out.data_ptr(), workspace.data_ptr()       # (the sum of squares, then the library's own)
     with _on(index):
         stream = _stream(index)
-        call("gs_grad_norm", n, grads, masks, numel, rows, types, max_norm, sq_sum, floats, floats + 4,
-             floats + 8 if each else None, sq_sum + 8, stream)
+        check(host.norm(grads, masks, collected, max_norm, sq_sum, floats, floats + 4, floats + 8 if each else 0, sq_sum + 8, stream),
+              "gs_grad_norm")
         if group is not None:
             _sum_over_ranks(workspace[:1], group)
             call("gs_clip_coefficient", sq_sum, max_norm, floats, floats + 4, stream)
@@ -178,7 +176,6 @@ def _sum_over_ranks(value: torch.Tensor, group) -> None:
     value.copy_(host)
 
 
-@torch.no_grad()
 def grad_norm(grads: Sequence[torch.Tensor], row_masks: Optional[Sequence[Optional[torch.Tensor]]] = None, *,
               per_tensor: bool = False):
     """2-norm of all ``grads`` together (float32 scalar on their device, no host wait); with ``per_tensor`` also the norms of
@@ -189,11 +186,10 @@ def grad_norm(grads: Sequence[torch.Tensor], row_masks: Optional[Sequence[Option
         raise ValueError("grad_norm: no gradients")
     host = _lib.host()
     collected = host.collect(("grads", grads, host.GRADS), ("row_masks", row_masks, host.MASK))
-    out = _norm_of(collected, collected[0][1], 0.0, per_tensor)
+    out = _norm_of(host, collected, *collected[0], 0.0, per_tensor)
     return (out[0], out[2:]) if per_tensor else out[0]
 
 
-@torch.no_grad()
 def adamw_step_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence[torch.Tensor],
                 exp_avg_sqs: Sequence[torch.Tensor], *, step: Union[int, torch.Tensor, Sequence[Union[int, torch.Tensor]]],
                 lr: Union[Scalar, Sequence[Scalar]] = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
@@ -251,31 +247,28 @@ def adamw_step_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], e
         if max_grad_norm is not None:
             raise ValueError("the norm of no gradients")
         return None
-    columns, numel, rows, types, index, kept = collected
-    device = torch.device("cuda", index)
+    columns, index = collected[0], collected[4]
     if grad_scale is not None and (grad_scale.get_device() != index or grad_scale.dtype is not torch.float32 or grad_scale.numel() != 1):
         raise ValueError("grad_scale: one float32 on the parameters' device")
-    hyper, counts, step_tensors, rate_tensors, numbers = host.scalars(n, step, lr, weight_decay, beta1, beta2, eps, index)
-    if numbers and torch.cuda.is_current_stream_capturing():
+    numbers = host.scalars(n, step, lr, weight_decay, beta1, beta2, eps, index)
+    if numbers[4] and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("a captured step needs its step count in a device tensor: a number would be the same at every replay")
 
-    norms = clip = None
+    norms, clip = None, 0
     if max_grad_norm is not None:
-        norms = _norm_of((columns[1:2], numel, rows, types, index, kept), columns[6], float(max_grad_norm), False, norm_group)
+        norms = _norm_of(host, collected, columns[1], columns[6], float(max_grad_norm), False, norm_group)
         clip = norms.data_ptr() + 4
     elif grad_scale is not None:
         clip = grad_scale.data_ptr()
-    ids = array("i", range(n) if tensor_ids is None else tensor_ids)
-    workspace = None
-    if step_tensors is not None or rate_tensors is not None:
-        workspace = torch.empty(int(_lib.load().gs_adamw_workspace_bytes(n)), dtype=torch.uint8, device=device)
+    workspace, workspace_at = None, 0
+    if numbers[2] is not None or numbers[3] is not None:
+        workspace = torch.empty(int(_lib.load().gs_adamw_workspace_bytes(n)), dtype=torch.uint8, device=torch.device("cuda", index))
+        workspace_at = workspace.data_ptr()
     with _on(index):
-        call("gs_adamw_step", n, *columns, numel, rows, types, ids.buffer_info()[0], hyper, counts, step_tensors, rate_tensors,
-             clip, seed & 0xFFFFFFFF, None if workspace is None else workspace.data_ptr(), _stream(index))
+        check(host.step(collected, numbers, tensor_ids, clip, seed & 0xFFFFFFFF, workspace_at, _stream(index)), "gs_adamw_step")
     return None if norms is None else norms[0]
 
 
-@torch.no_grad()
 def read_moments(exp_avgs: Sequence[torch.Tensor], exp_avg_sqs: Sequence[torch.Tensor], exponents: Sequence[torch.Tensor], *,
                  dtype: torch.dtype = torch.float32, out: Optional[Tuple[Sequence[torch.Tensor], Sequence[torch.Tensor]]] = None
                  ) -> Tuple[Sequence[torch.Tensor], Sequence[torch.Tensor]]:
@@ -287,21 +280,17 @@ def read_moments(exp_avgs: Sequence[torch.Tensor], exp_avg_sqs: Sequence[torch.T
     if out is None:
         if dtype not in (torch.float32, torch.bfloat16):
             raise TypeError("read_moments: float32 or bfloat16 values")
-        collected = host.collect(*inputs)
+        host.collect(*inputs)
         out = tuple([torch.empty(t.shape, dtype=dtype, device=t.device) for t in exp_avgs] for _ in range(2))
-        if n == 0:
-            return out
-        (_, m_out, v_out), *_ = host.collect(inputs[0], ("out", out[0], host.VALUE), ("out", out[1], host.VALUE))
-        (m, v, x), numel, rows, _, index, _ = collected
-    else:
-        (m, v, x, m_out, v_out), numel, rows, _, index, _ = host.collect(*inputs, ("out", out[0], host.VALUE), ("out", out[1], host.VALUE))
-        if n == 0:
-            return out
-        dtype = out[0][0].dtype
-        if out[1][0].dtype is not dtype:
-            raise TypeError("out: both lists have one type")
+    collected = host.collect(*inputs, ("out", out[0], host.VALUE), ("out", out[1], host.VALUE))
+    if n == 0:
+        return out
+    dtype = out[0][0].dtype
+    if out[1][0].dtype is not dtype:
+        raise TypeError("out: both lists have one type")
+    index = collected[4]
     with _on(index):
-        call("gs_read_moments", n, m, v, x, m_out, v_out, numel, rows, _DTYPES[dtype], _stream(index))
+        check(host.read(collected, _DTYPES[dtype], _stream(index)), "gs_read_moments")
     return out
 
 
@@ -416,7 +405,7 @@ class AdamW(torch.optim.Optimizer):
         host = _lib.host()
         grads, masks = [g for columns in parts for g in columns[1]], [mask for columns in parts for mask in columns[6]]
         collected = host.collect(("grads", grads, host.GRADS), ("row_masks", masks, host.MASK))
-        norms = _norm_of(collected, collected[0][1], float(self.max_grad_norm), False, self.norm_group)
+        norms = _norm_of(host, collected, *collected[0], float(self.max_grad_norm), False, self.norm_group)
         self.last_grad_norm = norms[0]
         return norms[1]
 
