@@ -42,7 +42,7 @@ from .GaussianPointCloudRasterisation import GaussianPointCloudRasterisation
 from .GaussianPointCloudScene import GaussianPointCloudScene
 from .ImagePoseDataset import ImagePoseDataset
 from .LossFunction import LossFunction, ssim
-from .optim import Adam
+from .optim import Adam, AdamW
 from .yaml_config import YAMLConfig
 
 _log = logging.getLogger(__name__)
@@ -197,6 +197,13 @@ class GaussianPointCloudTrainer:
         # additions (not in the reference)
         num_data_loader_workers: int = 4
         seed: int = 0
+        # "adam": the reference's two Adam optimisers.  "adamw": one optim.AdamW over features and positions (same rates and
+        # schedule) with decoupled weight decay, moments in 32 or 8 bits (8: 118 instead of 472 bytes a Gaussian) and
+        # clipping by the global gradient norm (0: off)
+        optimizer: str = "adam"
+        optimizer_state_bits: int = 32
+        weight_decay: float = 0.0
+        max_grad_norm: float = 0.0
         # multi-GPU (torch.distributed initialised): "replicated" = every rank holds the whole point cloud and the rasteriser
         # is sharded over tile rows (distributed.py; loss, optimiser and controller run replicated and bit-identical);
         # "owner" = every rank OWNS a contiguous block of the point cloud -- its parameters, its Adam state, its share of
@@ -214,6 +221,10 @@ class GaussianPointCloudTrainer:
     def __init__(self, config: "GaussianPointCloudTrainer.TrainConfig", device: Optional[torch.device] = None):
         if not torch.cuda.is_available():
             raise RuntimeError("GaussianPointCloudTrainer needs a HIP device: the rasteriser has no CPU path")
+        if config.optimizer not in ("adam", "adamw"):
+            raise ValueError(f"optimizer {config.optimizer!r}: 'adam' or 'adamw'")
+        if config.optimizer == "adam" and (config.optimizer_state_bits != 32 or config.weight_decay or config.max_grad_norm):
+            raise ValueError("optimizer_state_bits, weight_decay and max_grad_norm need optimizer 'adamw'")
         self.config = config
         self.device = device or torch.device("cuda", torch.cuda.current_device())
         self.rank = torch.distributed.get_rank() if torch.distributed.is_initialized() else 0
@@ -385,6 +396,35 @@ class GaussianPointCloudTrainer:
             self._live_share_cache = cached
         return cached[1]
 
+    def _adamw(self):
+        """One AdamW for features and positions and the schedule of the positions' rate."""
+        cfg, scene = self.config, self.scene
+        optimizer = AdamW([dict(params=[scene.point_cloud_features], lr=cfg.feature_learning_rate),
+                           dict(params=[scene.point_cloud], lr=cfg.position_learning_rate)],
+                          betas=(0.9, 0.999), weight_decay=cfg.weight_decay, state_bits=cfg.optimizer_state_bits,
+                          max_grad_norm=cfg.max_grad_norm or None,
+                          # (replicated ranks hold the same gradients; owners have different points: the norm is that of all)
+                          norm_group=torch.distributed.group.WORLD if self.owner_sharded and cfg.max_grad_norm else None,
+                          seed=cfg.seed + (self.rank if self.owner_sharded else 0))
+        for p in (scene.point_cloud_features, scene.point_cloud):
+            optimizer.set_row_mask(p, scene.point_invalid_mask)
+        gamma = cfg.position_learning_rate_decay_rate
+        scheduler = torch.optim.lr_scheduler.LambdaLR(optimizer, [lambda n: 1.0, lambda n: gamma ** n])
+        return [optimizer], scheduler
+
+    def _add_regulariser_gradient(self) -> None:
+        """The scale regulariser's gradient, added to the features' (the mean is over all live Gaussians of all ranks)."""
+        from . import hip_ops
+        scene = self.scene
+        if scene.point_cloud_features.grad is None:
+            scene.point_cloud_features.grad = torch.zeros_like(scene.point_cloud_features)
+        weight = float(self.loss_function.config.regularization_weight)
+        if self.owner_sharded:
+            weight *= self._local_live_share()
+        with torch.no_grad():
+            hip_ops.scale_regulariser(scene.point_cloud_features, scene.point_invalid_mask, weight,
+                                      grad_features=scene.point_cloud_features.grad)
+
     # ------------------------------------------------------------------ training (TRN:120-272)
     def train(self):
         cfg = self.config
@@ -394,19 +434,23 @@ class GaussianPointCloudTrainer:
             train_loader = DeviceResidentSamples(train_loader, self.device, cfg.seed)
             _log.info("training set resident on %s: %d images", self.device, len(train_loader))
         batches = cycle(train_loader)
-        feature_optimizer = Adam([self.scene.point_cloud_features], lr=cfg.feature_learning_rate, betas=(0.9, 0.999))
-        position_optimizer = Adam([self.scene.point_cloud], lr=cfg.position_learning_rate, betas=(0.9, 0.999))
-        # fixed-capacity tensors (max_num_points_ratio): the rows without a point are not stepped
-        feature_optimizer.set_row_mask(self.scene.point_cloud_features, self.scene.point_invalid_mask)
-        position_optimizer.set_row_mask(self.scene.point_cloud, self.scene.point_invalid_mask)
         regularised = self.loss_function.config.enable_regularization
-        if regularised:
-            feature_optimizer.set_scale_regulariser(self.scene.point_cloud_features,
-                                                    self.loss_function.config.regularization_weight,
-                                                    self.scene.point_invalid_mask,
-                                                    local_share=self._local_live_share if self.owner_sharded else None)
-        scheduler = torch.optim.lr_scheduler.ExponentialLR(position_optimizer,
-                                                           gamma=cfg.position_learning_rate_decay_rate)
+        if cfg.optimizer == "adamw":
+            optimizers, scheduler = self._adamw()
+        else:
+            feature_optimizer = Adam([self.scene.point_cloud_features], lr=cfg.feature_learning_rate, betas=(0.9, 0.999))
+            position_optimizer = Adam([self.scene.point_cloud], lr=cfg.position_learning_rate, betas=(0.9, 0.999))
+            optimizers = [feature_optimizer, position_optimizer]
+            # fixed-capacity tensors (max_num_points_ratio): the rows without a point are not stepped
+            feature_optimizer.set_row_mask(self.scene.point_cloud_features, self.scene.point_invalid_mask)
+            position_optimizer.set_row_mask(self.scene.point_cloud, self.scene.point_invalid_mask)
+            if regularised:
+                feature_optimizer.set_scale_regulariser(self.scene.point_cloud_features,
+                                                        self.loss_function.config.regularization_weight,
+                                                        self.scene.point_invalid_mask,
+                                                        local_share=self._local_live_share if self.owner_sharded else None)
+            scheduler = torch.optim.lr_scheduler.ExponentialLR(position_optimizer,
+                                                               gamma=cfg.position_learning_rate_decay_rate)
         downsample_factor = cfg.initial_downsample_factor
         recent_losses = deque(maxlen=100)
         last_problematic = -1000
@@ -418,8 +462,8 @@ class GaussianPointCloudTrainer:
                 break
             if iteration > 0 and iteration % cfg.half_downsample_factor_interval == 0 and downsample_factor > 1:
                 downsample_factor //= 2
-            feature_optimizer.zero_grad(set_to_none=True)
-            position_optimizer.zero_grad(set_to_none=True)
+            for optimizer in optimizers:
+                optimizer.zero_grad(set_to_none=True)
             image_gt, q, t, info = next(batches)
             image_gt, q, t, info = self._to_device((image_gt, q, t, info))   # no-op for resident samples
             if downsample_factor > 1:   # on the device (the reference resizes on the host before the copy)
@@ -444,8 +488,10 @@ class GaussianPointCloudTrainer:
                 loss = loss + reg_value
             raw_pred = image_pred.detach()
             image_pred = None   # the clamped CHW copy is only materialised on logging iterations (below)
-            feature_optimizer.step()
-            position_optimizer.step()
+            if regularised and cfg.optimizer == "adamw":   # (there it is part of the gradient that is clipped)
+                self._add_regulariser_gradient()
+            for optimizer in optimizers:
+                optimizer.step()
             if iteration % cfg.position_learning_rate_decay_interval == 0:
                 scheduler.step()
 

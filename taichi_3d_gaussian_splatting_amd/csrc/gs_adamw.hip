@@ -1131,7 +1131,7 @@ constexpr long long SMALL_CHUNKS = 2048;    // of 16 units
 template <int U, bool STATE8>
 void launch_step(int dtype, bool master, bool masked, const AdamwBatch &b, hipStream_t s) {
     const dim3 grid(b.first_chunk[b.n_tensors]), block(GS_BLOCK);
-    const int lds = STATE8 ? 0 : OCCUPANCY_LDS;
+    const int lds = STATE8 || masked ? 0 : OCCUPANCY_LDS;
     if (masked) hipLaunchKernelGGL((adamw_kernel<1, GS_DTYPE_F32, false, STATE8, true>), grid, block, 0, s, b);
     else if (dtype == GS_DTYPE_F32) hipLaunchKernelGGL((adamw_kernel<U, GS_DTYPE_F32, false, STATE8, false>), grid, block, lds, s, b);
     else if (dtype == GS_DTYPE_BF16 && master) hipLaunchKernelGGL((adamw_kernel<U, GS_DTYPE_BF16, true, STATE8, false>), grid, block, lds, s, b);

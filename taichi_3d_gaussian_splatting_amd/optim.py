@@ -381,6 +381,10 @@ class AdamW(torch.optim.Optimizer):
                                                    group["weight_decay"], place)):
                     column.append(value)
         if not work:
+            if self.max_grad_norm is not None and self.norm_group is not None:     # (the other ranks wait for this one's share)
+                share = torch.zeros(1, dtype=torch.float64, device=self.param_groups[0]["params"][0].device)
+                _sum_over_ranks(share, self.norm_group)
+                self.last_grad_norm = share.sqrt().float()[0]
             return loss
         clip = None
         if self.max_grad_norm is not None:
