@@ -153,15 +153,16 @@ def _norm_of(host, collected, grads, masks, max_norm: float, each: bool, group=N
     """[norm, clip, each ...] of collected gradients, on their device's current stream."""
     index = collected[4]
     device, n = torch.device("cuda", index), len(collected[1]) // 8
-    out = torch.empty(2 + (n if each else 0), dtype=torch.float32, device=device)
-    workspace = torch.empty(1 + (_lib.load().gs_grad_norm_workspace_bytes(n) + 7) // 8, dtype=torch.float64, device=device)
-    floats, sq_sum = out.data_ptr(), workspace.data_ptr()       # (the sum of squares, then the library's own)
+    words = (2 + (n if each else 0) + 1) // 2 * 2       # behind them: the sum of squares (double), the library's workspace
+    out = torch.empty(words + 2 + (_lib.load().gs_grad_norm_workspace_bytes(n) + 3) // 4, dtype=torch.float32, device=device)
+    floats = out.data_ptr()
+    sq_sum = floats + 4 * words
     with _on(index):
         stream = _stream(index)
         check(host.norm(grads, masks, collected, max_norm, sq_sum, floats, floats + 4, floats + 8 if each else 0, sq_sum + 8, stream),
               "gs_grad_norm")
         if group is not None:
-            _sum_over_ranks(workspace[:1], group)
+            _sum_over_ranks(out[words:words + 2].view(torch.float64), group)
             call("gs_clip_coefficient", sq_sum, max_norm, floats, floats + 4, stream)
     return out
 
@@ -187,7 +188,7 @@ def grad_norm(grads: Sequence[torch.Tensor], row_masks: Optional[Sequence[Option
     host = _lib.host()
     collected = host.collect(("grads", grads, host.GRADS), ("row_masks", row_masks, host.MASK))
     out = _norm_of(host, collected, *collected[0], 0.0, per_tensor)
-    return (out[0], out[2:]) if per_tensor else out[0]
+    return (out[0], out[2:2 + len(grads)]) if per_tensor else out[0]
 
 
 def adamw_step_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence[torch.Tensor],
@@ -351,35 +352,7 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        work = {}           # (state_bits, betas, eps, device) -> columns of adamw_step_
-        place = -1
-        for group in self.param_groups:
-            for p in group["params"]:
-                place += 1
-                if p.grad is None:
-                    continue
-                if p.grad.is_sparse:
-                    raise RuntimeError("AdamW does not take sparse gradients")
-                if not p.is_cuda or not p.is_contiguous():
-                    raise RuntimeError("optim.AdamW needs contiguous parameters on the HIP device")
-                state = self.state[p]
-                mask = self._row_mask.get(id(p))
-                if not state or (mask is not None and "last_step" not in state):
-                    if torch.cuda.is_current_stream_capturing():
-                        raise RuntimeError("run one step of AdamW before capturing one: its state is made there")
-                if not state:
-                    state.update(self._new_state(p, group))
-                if mask is not None and "last_step" not in state:
-                    # moments from a state_dict without row masks are current as of the previous step
-                    state["last_step"] = torch.full((p.shape[0],), int(state["step"]), dtype=torch.int32, device=p.device)
-                if not self.capturable:
-                    state["step"] += 1
-                bits = 8 if "exponents" in state else 32
-                columns = work.setdefault((bits, group["betas"], group["eps"], p.device), tuple([] for _ in range(12)))
-                for column, value in zip(columns, (p, p.grad, state["exp_avg"], state["exp_avg_sq"], state.get("exponents"),
-                                                   state.get("master"), mask, state.get("last_step"), state["step"], group["lr"],
-                                                   group["weight_decay"], place)):
-                    column.append(value)
+        work = self._work()
         if not work:
             if self.max_grad_norm is not None and self.norm_group is not None:     # (the other ranks wait for this one's share)
                 share = torch.zeros(1, dtype=torch.float64, device=self.param_groups[0]["params"][0].device)
@@ -391,23 +364,69 @@ class AdamW(torch.optim.Optimizer):
             if len({key[3] for key in work}) > 1:
                 raise RuntimeError("max_grad_norm: all parameters belong on one device")
             clip = self._clip(list(work.values()))
-        for (bits, betas, eps, _), columns in work.items():
-            params, grads, ms, vs, exponents, masters, masks, stamps, steps, rates, decays, places = columns
+        for (eight, betas, eps, _), (params, grads, states, masks, rates, decays, ids) in work.items():
             if self.capturable:
+                steps = [s["step"] for s in states]
                 torch._foreach_add_(steps, 1)
+            else:
+                steps = [s["step"] + 1 for s in states]
+            masters = [s.get("master") for s in states] if self.master_weights else None
             masked = any(mask is not None for mask in masks)
-            adamw_step_(params, grads, ms, vs, step=steps, lr=rates, betas=betas, eps=eps, weight_decay=decays,
-                        exponents=exponents if bits == 8 else None,
-                        masters=masters if any(c is not None for c in masters) else None,
+            adamw_step_(params, grads, [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states], step=steps, lr=rates,
+                        betas=betas, eps=eps, weight_decay=decays,
+                        exponents=[s["exponents"] for s in states] if eight else None, masters=masters,
                         row_masks=masks if masked else None,
-                        last_steps=[s if mask is not None else None for s, mask in zip(stamps, masks)] if masked else None,
-                        grad_scale=clip, seed=self.seed, tensor_ids=places)
+                        last_steps=[None if mask is None else s["last_step"] for s, mask in zip(states, masks)] if masked else None,
+                        grad_scale=clip, seed=self.seed, tensor_ids=ids)
+            if not self.capturable:
+                for state, count in zip(states, steps):
+                    state["step"] = count
         return loss
+
+    def _work(self) -> dict:
+        """What a step has to do, by what one call of ``adamw_step_`` shares: (8-bit moments, betas, eps, device index) -> lists of
+        parameters, gradients, states, row masks, rates, decays and the parameters' places in the optimiser."""
+        work, place = {}, 0
+        for group in self.param_groups:
+            params, first = group["params"], place
+            place += len(params)
+            grads = [p.grad for p in params]
+            ids = list(range(first, place))
+            if any(g is None for g in grads):
+                kept = [i for i, g in enumerate(grads) if g is not None]
+                params, grads, ids = ([column[i] for i in kept] for column in (params, grads, ids))
+            states = [self.state[p] for p in params]
+            masks = [self._row_mask.get(id(p)) for p in params] if self._row_mask else [None] * len(params)
+            for p, state, mask in zip(params, states, masks):
+                if not state or (mask is not None and "last_step" not in state):
+                    self._complete(p, state, mask, group)
+            kinds = [("exponents" in s, p.get_device()) for p, s in zip(params, states)]
+            for kind in sorted(set(kinds)):
+                columns = params, grads, states, masks, ids
+                if any(k != kind for k in kinds):
+                    columns = tuple([x for x, k in zip(column, kinds) if k == kind] for column in columns)
+                n = len(columns[0])
+                rows = work.setdefault((kind[0], tuple(group["betas"]), group["eps"], kind[1]), tuple([] for _ in range(7)))
+                for row, column in zip(rows, (*columns[:4], [group["lr"]] * n, [group["weight_decay"]] * n, columns[4])):
+                    row.extend(column)
+        return work
+
+    def _complete(self, p: torch.Tensor, state: dict, mask: Optional[torch.Tensor], group: dict) -> None:
+        """The state of a parameter that has none, or none for its row mask yet."""
+        if not p.is_cuda:
+            raise RuntimeError("optim.AdamW needs parameters on the HIP device: there is no CPU path")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("run one step of AdamW before capturing one: its state is made there")
+        if not state:
+            state.update(self._new_state(p, group))
+        if mask is not None:
+            # moments from a state_dict without row masks are current as of the previous step
+            state["last_step"] = torch.full((p.shape[0],), int(state["step"]), dtype=torch.int32, device=p.device)
 
     def _clip(self, parts) -> torch.Tensor:
         """The clipping coefficient of all gradients (and ``last_grad_norm``)."""
         host = _lib.host()
-        grads, masks = [g for columns in parts for g in columns[1]], [mask for columns in parts for mask in columns[6]]
+        grads, masks = [g for columns in parts for g in columns[1]], [mask for columns in parts for mask in columns[3]]
         collected = host.collect(("grads", grads, host.GRADS), ("row_masks", masks, host.MASK))
         norms = _norm_of(host, collected, *collected[0], float(self.max_grad_norm), False, self.norm_group)
         self.last_grad_norm = norms[0]
@@ -454,7 +473,9 @@ class AdamW(torch.optim.Optimizer):
                     state[name] = value.detach().to(device=p.device, dtype=types[name], copy=True).contiguous()
             if not {"step", "exp_avg", "exp_avg_sq"} <= set(state):
                 raise ValueError("state_dict: no AdamW state")
-            if self.master_weights and p.dtype != torch.float32 and "master" not in state:
+            if not self.master_weights:
+                state.pop("master", None)
+            elif p.dtype != torch.float32 and "master" not in state:
                 state["master"] = p.detach().to(torch.float32)
             group["state_bits"] = 8 if eight else 32
             self.state[p] = state
