@@ -31,6 +31,7 @@ constexpr long long NORM_STREAM_BYTES = 128LL << 20;
 // What a step needs besides the tensors; key and step belong to one tensor
 struct AdamwScalars {
     float rate, root, keep, one_minus_beta1, beta2, one_minus_beta2, eps, beta1;   // rate = lr / (1 - b1^t), root = 1 / sqrt(1 - b2^t)
+    float log_beta1[2], log_beta2[2];       // log2 of the betas, each a float and what it lacks
     int step;
     uint32_t key;
 };
@@ -39,12 +40,15 @@ struct AdamwScalars {
 // where the parameter has 16 bits, its moments 8 and there is no master copy: 16 bytes of the parameter again, and half the
 // instructions an element for a block's largest value, exponents and scales, which bound that case.
 constexpr bool pairs(int dtype, bool master, bool state8) { return state8 && dtype != GS_DTYPE_F32 && !master; }
-constexpr int MASKED_ROWS = 32;     // packed rows that a wave has in flight (8, 16, 32: 206, 202, 196 us for 1.2M rows, 30 % live)
+// Rows under a mask that a wave packs, all of them in flight.  us of a step of 1.2M rows, all live / 30 % at random / the first
+// 30 %: 32 bits: 16 rows 335 / 175 / 114, 32: 362 / 182 / 117, 64: 376 / 173 / 128; 8 bits: 196 / 118 / 76, 203 / 122 / 73,
+// 215 / 127 / 74, and 132, 120, 121 of the second where a tenth of the rows comes back late.
+constexpr int masked_rows(bool state8) { return state8 ? 32 : 16; }
 
 // How a tensor is cut among lanes
 enum Form : int {
     QUADS,          // units of 64, or long rows: 16 lanes a unit, or 8 with pairs of quads
-    QUADS_MASKED,   // the same rows under a mask: a wave packs the live ones of 64 rows
+    QUADS_MASKED,   // the same rows under a mask: a wave packs the live ones
     NARROW,         // float rows of 1 to 4 elements: whole quads of rows a lane
     ELEMENTS        // anything else, unaligned tensors: element by element
 };
@@ -251,12 +255,21 @@ __device__ __forceinline__ float update_coded(float p, float g, float m_unit, ui
     return moved<MASTER>(p, m * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v) * k.root + k.eps), k);
 }
 
+// beta^d = 2^(d log2 beta): the product's rounding error and what the logarithm lacks follow as a factor, so that long gaps
+// lose nothing.
+__device__ __forceinline__ float beta_power(int d, const float (&log_beta)[2]) {
+    const float n = (float)d, x = n * log_beta[0];
+    const float rest = fmaf(n, log_beta[1], fmaf(n, log_beta[0], -x));
+    const float y = __builtin_amdgcn_exp2f(x);
+    return fmaf(y, 0.693147180559945f * rest, y);
+}
+
 // What a row that was last stepped at `last` has to be multiplied with before this step
 __device__ __forceinline__ void row_decay(const AdamwScalars &k, int last, float &decay_m, float &decay_v) {
     const int gap = k.step - 1 - last;
     if (gap > 0) {
-        decay_m = powf(k.beta1, (float)gap);
-        decay_v = powf(k.beta2, (float)gap);
+        decay_m = beta_power(gap, k.log_beta1);
+        decay_v = beta_power(gap, k.log_beta2);
     }
 }
 
@@ -531,17 +544,17 @@ __device__ __forceinline__ void step_quads(const AdamwTensor &t, const AdamwScal
         step_unit<16, DT, MASTER, STATE8>(t, k, scale, whole + threadIdx.x / 16, (int)unit_len);
 }
 
-// Rows under a mask: a wave reads the mask and the stamps of 64 rows, packs the live ones and steps them four at a time, so
+// Rows under a mask: a wave reads the mask and the stamps of its rows, packs the live ones and steps them four at a time, so
 // that no lane waits beside a row without a point and none of such a row's data is asked for.
 template <int UNROLL, bool STATE8>
 __device__ __forceinline__ void step_quads_masked(const AdamwTensor &t, const AdamwScalars &k, float scale, unsigned chunk) {
     typedef Share<GS_DTYPE_F32, false, STATE8> S;
-    constexpr int GROUP = S::GROUP, PER_PASS = GS_WAVE / GROUP;
+    constexpr int GROUP = S::GROUP, PER_PASS = GS_WAVE / GROUP, WAVE_ROWS = PER_PASS * UNROLL;
     const uint32_t row_len = t.row_len, lane = gs_lane(), sub = lane % GROUP;
-    const long long row0 = ((long long)chunk * (GS_BLOCK / GS_WAVE) + __builtin_amdgcn_readfirstlane(threadIdx.x / GS_WAVE)) * GS_WAVE;
+    const long long row0 = ((long long)chunk * (GS_BLOCK / GS_WAVE) + __builtin_amdgcn_readfirstlane(threadIdx.x / GS_WAVE)) * WAVE_ROWS;
     const long long rows = t.numel / row_len;
     if (row0 >= rows) return;
-    const bool there = row0 + lane < rows;
+    const bool there = lane < WAVE_ROWS && row0 + lane < rows;
     const bool live = there && ((const int8_t *)t.master_or_mask)[there ? row0 + lane : row0] == 0;
     const u64 lives = __ballot(live), below = (1ull << lane) - 1ull;
     if (lives == 0) return;
@@ -557,25 +570,25 @@ __device__ __forceinline__ void step_quads_masked(const AdamwTensor &t, const Ad
     const int order = __builtin_amdgcn_ds_permute(4 * (live ? __popcll(lives & below) : 63 - __popcll(~lives & below)), (int)lane);
     const bool any_late = __ballot(decay_m != 1.f || decay_v != 1.f) != 0;
     const Buffers<GS_DTYPE_F32, false, STATE8> b(t, row0 * row_len, row0);
-    for (int at = 0; at < n_live; at += PER_PASS * UNROLL) {
-        S q[UNROLL];
-        int from[UNROLL];
+    S q[UNROLL];
+    int from[UNROLL];
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            from[u] = __shfl(order, min(at + PER_PASS * u + (int)(lane / GROUP), n_live - 1), GS_WAVE);
-            q[u].place(from[u] * row_len, row_len, sub);
-            q[u].load(b);
-        }
+    for (int u = 0; u < UNROLL; ++u) {
+        if (PER_PASS * u >= n_live) break;      // (the same for the wave)
+        from[u] = __shfl(order, min(PER_PASS * u + (int)(lane / GROUP), n_live - 1), GS_WAVE);
+        q[u].place(from[u] * row_len, row_len, sub);
+        q[u].load(b);
+    }
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            const uint32_t old_x = STATE8 ? (uint32_t)__shfl(x, from[u], GS_WAVE) : 0u;
-            const float dm = any_late ? __shfl(decay_m, from[u], GS_WAVE) : 1.f, dv = any_late ? __shfl(decay_v, from[u], GS_WAVE) : 1.f;
-            f32x4 p[S::Q];
-            const uint32_t new_x = q[u].template step<true>(p, old_x, dm, dv, b.quad, scale, k);
-            if (at + PER_PASS * u + (int)(lane / GROUP) < n_live && S::inside(row_len, sub)) {
-                q[u].store(b, p);
-                if (STATE8 && sub == 0) *(uint16_t *)(b.exponents + 2 * from[u]) = (uint16_t)new_x;
-            }
+    for (int u = 0; u < UNROLL; ++u) {
+        if (PER_PASS * u >= n_live) break;
+        const uint32_t old_x = STATE8 ? (uint32_t)__shfl(x, from[u], GS_WAVE) : 0u;
+        const float dm = any_late ? __shfl(decay_m, from[u], GS_WAVE) : 1.f, dv = any_late ? __shfl(decay_v, from[u], GS_WAVE) : 1.f;
+        f32x4 p[S::Q];
+        const uint32_t new_x = q[u].template step<true>(p, old_x, dm, dv, b.quad, scale, k);
+        if (PER_PASS * u + (int)(lane / GROUP) < n_live && S::inside(row_len, sub)) {
+            q[u].store(b, p);
+            if (STATE8 && sub == 0) *(uint16_t *)(b.exponents + 2 * from[u]) = (uint16_t)new_x;
         }
     }
 }
@@ -677,10 +690,10 @@ __device__ __forceinline__ void step_narrow(const AdamwTensor &t, const AdamwSca
 }
 
 // Chunks that a form makes of a tensor (a workgroup each)
-__host__ __device__ inline long long form_chunks(int form, long long numel, int row_len, int per_quads) {
+__host__ __device__ inline long long form_chunks(int form, long long numel, int row_len, int per_quads, bool state8) {
     const long long units = row_len > 0 ? numel / row_len : (numel + UNIT - 1) / UNIT;
     const int group = row_len == 0 || row_len > 16 ? 16 : (row_len > 4 ? 4 : 1);
-    const int per = form == QUADS ? GS_BLOCK / 16 * per_quads : form == QUADS_MASKED ? GS_BLOCK : form == NARROW ? narrow_rows(row_len) * GS_BLOCK : GS_BLOCK / group;
+    const int per = form == QUADS ? GS_BLOCK / 16 * per_quads : form == QUADS_MASKED ? GS_BLOCK / GS_WAVE * masked_rows(state8) : form == NARROW ? narrow_rows(row_len) * GS_BLOCK : GS_BLOCK / group;
     return (units + per - 1) / per;
 }
 
@@ -695,7 +708,7 @@ __global__ __launch_bounds__(GS_BLOCK) void adamw_kernel(AdamwBatch b) {
     const float scale = b.grad_scale ? *b.grad_scale : 1.f;
     const unsigned chunk = blockIdx.x - b.first_chunk[ti];
     if constexpr (MASKED) {
-        if (t.form == QUADS_MASKED) return step_quads_masked<MASKED_ROWS / 4, STATE8>(t, k, scale, chunk);
+        if (t.form == QUADS_MASKED) return step_quads_masked<masked_rows(STATE8) / 4, STATE8>(t, k, scale, chunk);
     } else {
         if (t.form == QUADS) return step_quads<pairs(DT, MASTER, STATE8) ? (QUADS_A_LANE + 1) / 2 : QUADS_A_LANE, DT, MASTER, STATE8>(t, k, scale, chunk);
     }
@@ -735,6 +748,12 @@ __host__ __device__ AdamwScalars adamw_scalars(double lr, double beta1, double b
     k.one_minus_beta2 = (float)(1.0 - beta2);
     k.eps = (float)eps;
     k.beta1 = (float)beta1;
+    // (a beta of zero: any power is far below float's range)
+    const double l1 = beta1 > 0.0 ? log2(beta1) : -1e6, l2 = beta2 > 0.0 ? log2(beta2) : -1e6;
+    k.log_beta1[0] = (float)l1;
+    k.log_beta1[1] = (float)(l1 - (double)k.log_beta1[0]);
+    k.log_beta2[0] = (float)l2;
+    k.log_beta2[1] = (float)(l2 - (double)k.log_beta2[0]);
     k.key = tensor_key(seed, tensor, (uint32_t)step);
     k.step = (int)step;
     return k;
@@ -1190,7 +1209,7 @@ extern "C" int gs_adamw_step(int n_tensors, const uint64_t *host_param, const ui
         GS_REQUIRE(n >= 0 && n < (1LL << 46) && row >= 0 && row <= UNIT && (row == 0 || n % row == 0),
                    "gs_adamw_step: numel in [0, 2^46), too large else, rows of 1..64 elements");
         GS_REQUIRE(dt == GS_DTYPE_F32 || dt == GS_DTYPE_BF16 || dt == GS_DTYPE_F16, "gs_adamw_step: unknown dtype");
-        GS_REQUIRE(form_chunks(ELEMENTS, n, row, 1) < 0x7fffffffLL, "gs_adamw_step: tensor too large");
+        GS_REQUIRE(form_chunks(ELEMENTS, n, row, 1, false) < 0x7fffffffLL, "gs_adamw_step: tensor too large");
         GS_REQUIRE(n == 0 || (host_param[i] && host_grad[i] && host_exp_avg[i] && host_exp_avg_sq[i] && (!state8 || host_exponents[i])),
                    "gs_adamw_step: null tensor");
         GS_REQUIRE(!entry(host_row_mask, i) || (row > 0 && dt == GS_DTYPE_F32 && host_last_step[i]), "gs_adamw_step: a row mask needs float rows and last steps");
@@ -1200,7 +1219,7 @@ extern "C" int gs_adamw_step(int n_tensors, const uint64_t *host_param, const ui
         GS_REQUIRE(aligned_to(host_param[i] | host_grad[i], element_bytes(dt)) && aligned_to(state8 ? 0 : host_exp_avg[i] | host_exp_avg_sq[i], 4) &&
                        aligned_to(entry(host_master, i) | (entry(host_row_mask, i) ? host_last_step[i] : 0), 4),
                    "gs_adamw_step: an address is no multiple of its type's size");
-        units_of_16 += form_chunks(QUADS, n, row, 1);
+        units_of_16 += form_chunks(QUADS, n, row, 1, false);
     }
     {
         Range *r = (Range *)malloc((size_t)n_tensors * 7 * sizeof(Range));
@@ -1251,7 +1270,7 @@ extern "C" int gs_adamw_step(int n_tensors, const uint64_t *host_param, const ui
                 t.form = narrow ? NARROW : quads ? (mask ? QUADS_MASKED : QUADS) : ELEMENTS;
                 t.row_len = (uint8_t)row;
                 t.masked = mask != 0;
-                chunks = form_chunks(t.form, host_numel[i], row, pair ? std::max(2, unroll) : unroll);
+                chunks = form_chunks(t.form, host_numel[i], row, pair ? std::max(2, unroll) : unroll, state8);
                 while (!on_device && set < q.n_sets &&
                        (q.step[set] != host_step[i] || memcmp(q.hyper[set], host_hyper + 5 * (size_t)i, 5 * sizeof(double)) != 0)) ++set;
             }
@@ -1315,11 +1334,11 @@ extern "C" int gs_read_moments(int n_tensors, const uint64_t *host_exp_avg, cons
         const int row = host_row_len[i];
         GS_REQUIRE(n >= 0 && n < (1LL << 46) && row >= 0 && row <= UNIT && (row == 0 || n % row == 0),
                    "gs_read_moments: numel in [0, 2^46), rows of 1..64 elements");
-        GS_REQUIRE(form_chunks(ELEMENTS, n, row, 1) < 0x7fffffffLL, "gs_read_moments: tensor too large");
+        GS_REQUIRE(form_chunks(ELEMENTS, n, row, 1, false) < 0x7fffffffLL, "gs_read_moments: tensor too large");
         GS_REQUIRE(n == 0 || (host_exp_avg[i] && host_exp_avg_sq[i] && host_exponents[i] && host_m_out[i] && host_v_out[i]),
                    "gs_read_moments: null tensor");
         GS_REQUIRE(aligned_to(host_m_out[i] | host_v_out[i], element_bytes(out_dtype)), "gs_read_moments: misaligned output");
-        units_of_16 += form_chunks(QUADS, n, row, 1);
+        units_of_16 += form_chunks(QUADS, n, row, 1, false);
     }
     {
         Range *r = (Range *)malloc((size_t)n_tensors * 5 * sizeof(Range));
@@ -1353,7 +1372,7 @@ extern "C" int gs_read_moments(int n_tensors, const uint64_t *host_exp_avg, cons
             t = {(const uint8_t *)host_exp_avg[i], (const uint8_t *)host_exp_avg_sq[i], (const uint8_t *)host_exponents[i],
                  (void *)host_m_out[i], (void *)host_v_out[i], host_numel[i], row, 0};
             t.form = row >= 1 && row <= 4 && fours && aligned_to(host_exponents[i], 8) ? NARROW : fours && (row == 0 || (row > 16 && row % 4 == 0)) ? QUADS : ELEMENTS;
-            chunks = form_chunks(t.form, host_numel[i], row, unroll);
+            chunks = form_chunks(t.form, host_numel[i], row, unroll, true);
         }
         if (b.n_tensors > 0 && (end || b.n_tensors == MAX_TENSORS || (long long)b.first_chunk[b.n_tensors] + chunks >= 0x7fffffffLL)) {
             if (unroll == 1) launch_moments<1>(out_dtype, b, (hipStream_t)stream);
