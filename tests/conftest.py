@@ -15,6 +15,11 @@ def pytest_configure(config):
 def pytest_collection_modifyitems(config, items):
     """Without a HIP device the gpu-marked tests are skipped (a CPU-only run then still reports CPU-side regressions)
     -- except on a gpurun box (GRAFT_REPO_ROOT is set there), where a missing device must fail loudly."""
+    if not os.path.isdir("/root/reference/taichi_3d_gaussian_splatting"):
+        # an empty folder in their place is no reference sources either
+        for item in items:
+            if any("reference sources" in str(m.kwargs.get("reason")) for m in item.iter_markers("skipif")):
+                item.add_marker(pytest.mark.skip(reason="no reference sources here"))
     import torch
     if torch.cuda.is_available() or os.environ.get("GRAFT_REPO_ROOT"):
         return
