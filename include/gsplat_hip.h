@@ -683,7 +683,7 @@ int gs_adam_step_rows(float *param, const float *grad, float *exp_avg, float *ex
  *   host_step[i]    : t;  host_step_device (nullable, entries too): device int64 that holds t instead
  *   host_lr_device  : (nullable, entries too) device float that holds lr instead
  *   host_row_mask   : (nullable, entries too; float tensors with row_len 1..64) int8[rows]: rows with a value other than 0
- *                     are neither read nor written; host_last_step[i] int32[rows] = the last step that updated the row, a
+ *                     are left as they are; host_last_step[i] int32[rows] = the last step that updated the row, a
  *                     row that missed d steps starts from m beta1^d, v beta2^d
  *   workspace       : gs_adamw_workspace_bytes(n_tensors), needed where host_step_device or host_lr_device is given
  * No written range may overlap another range of the call. */

@@ -1222,7 +1222,7 @@ extern "C" int gs_adamw_step(int n_tensors, const uint64_t *host_param, const ui
         units_of_16 += form_chunks(QUADS, n, row, 1, false);
     }
     {
-        Range *r = (Range *)malloc((size_t)n_tensors * 7 * sizeof(Range));
+        Range *r = (Range *)malloc((size_t)n_tensors * 8 * sizeof(Range));
         GS_REQUIRE(r != nullptr, "gs_adamw_step: out of host memory");
         size_t k = 0;
         for (int i = 0; i < n_tensors; ++i) {
@@ -1234,7 +1234,10 @@ extern "C" int gs_adamw_step(int n_tensors, const uint64_t *host_param, const ui
             r[k++] = {host_exp_avg_sq[i], host_exp_avg_sq[i] + se, 1};
             if (state8) r[k++] = {host_exponents[i], host_exponents[i] + 2 * blocks, 1};
             if (entry(host_master, i)) r[k++] = {host_master[i], host_master[i] + 4 * n, 1};
-            if (entry(host_row_mask, i)) r[k++] = {host_last_step[i], host_last_step[i] + 4 * blocks, 1};
+            if (entry(host_row_mask, i)) {
+                r[k++] = {host_last_step[i], host_last_step[i] + 4 * blocks, 1};
+                r[k++] = {host_row_mask[i], host_row_mask[i] + blocks, 0};
+            }
         }
         const bool meet = ranges_meet(r, k);
         free(r);

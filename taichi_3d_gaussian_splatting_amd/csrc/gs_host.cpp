@@ -160,10 +160,10 @@ PyObject *collect_checked(PyObject *lists) {
             else right_shape = k == 0 || t.sizes() == ref.sizes();
             if (!right_shape)
                 throw Refused{PyExc_ValueError, at_place(name, i) + " has shape " + shape_text(t.sizes()) + ", which does not fit a tensor of shape " + shape_text(ref.sizes())};
-            if (t.is_contiguous()) {
+            if (t.is_contiguous() && !t.is_neg()) {
                 address[i] = (uint64_t)(uintptr_t)t.const_data_ptr();
             } else if (kind == GRAD || kind == GRADS) {
-                const at::Tensor copy = t.detach().contiguous();
+                const at::Tensor copy = t.detach().resolve_neg().contiguous();
                 Holder wrapped(THPVariable_Wrap(copy));
                 if (!wrapped.o || PyList_Append(kept.o, wrapped.o) < 0) return nullptr;
                 address[i] = (uint64_t)(uintptr_t)copy.const_data_ptr();

@@ -218,10 +218,11 @@ def adamw_step_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], e
       ``lr``: a number or a device tensor (float32, one element); each for all tensors or one per tensor.  While a graph is
       captured ``step`` has to be a tensor: a number would be the same at every replay.
     * ``row_masks`` / ``last_steps``: for float32 tensors ``[N, 1..64]``, int8 ``[N]`` and int32 ``[N]``: rows with a mask
-      other than 0 are neither read nor written, and a row that missed ``d`` steps starts from ``m b1^d``, ``v b2^d``.
+      other than 0 are left as they are, and a row that missed ``d`` steps starts from ``m b1^d``, ``v b2^d``.
     * ``max_grad_norm``: gradients are scaled by ``min(1, max_grad_norm / (norm + 1e-6))`` as they are read; the norm is that of
-      all gradients of the call (masked rows apart), over all ranks of ``norm_group`` where one is given, and is returned as a
-      float32 scalar on the device.  ``grads`` themselves stay as they are.
+      all gradients of the call (masked rows apart), over all ranks of ``norm_group`` where one is given (each of them calls
+      with one tensor at least), and is returned as a float32 scalar on the device.  ``grads`` themselves stay as they are.  An
+      infinite norm scales by 0, a NaN makes NaN of everything, as torch.nn.utils.clip_grad_norm_ does.
     * ``grad_scale``: a float32 device scalar to multiply the gradients with instead.
 
     Nothing waits for the device (but for a ``norm_group`` whose back end takes host memory).  Written buffers must not
@@ -301,7 +302,8 @@ class AdamW(torch.optim.Optimizer):
 
     * ``state_bits`` (also per group): 32 (float32 moments) or 8 (a code and a share of two exponents each: 2.03 bytes for an
       element's two moments instead of 8), see ``new_moments``; ``moments(param)`` reads either.
-    * ``master_weights``: 16-bit parameters are stepped through a float32 copy (``state["master"]``).
+    * ``master_weights``: 16-bit parameters are stepped through a float32 copy (``state["master"]``, made at the first step; who
+      changes such a parameter afterwards changes the copy too).
     * ``max_grad_norm``: the gradients of all groups are clipped by their global norm; ``last_grad_norm`` holds it (a device
       scalar) after a step.  ``norm_group``: a process group whose ranks hold different parameters: the norm is that of all.
     * ``capturable``: step counts live on the device, so a step can be captured into a graph and replayed; ``lr`` may then be a
@@ -433,49 +435,74 @@ class AdamW(torch.optim.Optimizer):
         return norms[1]
 
     def moments(self, param: torch.Tensor, dtype: torch.dtype = torch.float32) -> Tuple[torch.Tensor, torch.Tensor]:
-        """Values of a parameter's first and second moment, whatever they are held in."""
+        """Copies of a parameter's first and second moment, whatever they are held in (of rows that miss steps under a row mask:
+        as of the last step that reached them)."""
         state = self.state.get(param)
         if not state:
             raise KeyError("the parameter has no state yet")
         if "exponents" not in state:
-            return state["exp_avg"].to(dtype), state["exp_avg_sq"].to(dtype)
+            return state["exp_avg"].to(dtype, copy=True), state["exp_avg_sq"].to(dtype, copy=True)
         m, v = read_moments([state["exp_avg"]], [state["exp_avg_sq"]], [state["exponents"]], dtype=dtype)
         return m[0], v[0]
 
+    _OPTIONS = ("master_weights", "max_grad_norm", "norm_group", "capturable", "seed", "last_grad_norm")
+
+    def __getstate__(self) -> dict:
+        places = {id(p): i for i, p in enumerate(p for group in self.param_groups for p in group["params"])}
+        return {**super().__getstate__(), **{name: getattr(self, name) for name in self._OPTIONS},
+                "row_masks": {places[i]: mask for i, mask in self._row_mask.items() if i in places}}
+
+    def __setstate__(self, state: dict) -> None:
+        state = dict(state)
+        masks = state.pop("row_masks", None)
+        super().__setstate__(state)
+        if masks is not None:       # (a copy or an unpickled optimiser; load_state_dict brings none)
+            params = [p for group in self.param_groups for p in group["params"]]
+            self._row_mask = {id(params[i]): mask for i, mask in masks.items()}
+
     def load_state_dict(self, state_dict) -> None:
         """As in torch, but the state keeps its own types (torch would cast codes, counts and float32 moments of 16-bit
-        parameters to the parameter's type).  Whether moments have 8 or 32 bits is what was saved."""
-        super().load_state_dict(state_dict)
-        saved = [i for group in state_dict["param_groups"] for i in group["params"]]
-        params = [(p, group) for group in self.param_groups for p in group["params"]]
+        parameters to the parameter's type).  Whether moments have 8 or 32 bits is what was saved; amsgrad and maximize are not
+        known here.  A state_dict that does not fit is refused and changes nothing."""
+        saved_groups = state_dict["param_groups"]
+        for group in saved_groups:
+            if group.get("amsgrad") or group.get("maximize"):
+                raise ValueError("state_dict: AdamW here has neither amsgrad nor maximize")
+        saved = [i for group in saved_groups for i in group["params"]]
+        params = [p for group in self.param_groups for p in group["params"]]
+        held = [state_dict["state"].get(i) for i in saved]
+        states = [self._loaded(p, h) if h else None for p, h in zip(params, held)]
+        super().load_state_dict({"state": {}, "param_groups": saved_groups})       # (refuses other groups)
+        self.state.clear()
+        for p, state in zip(params, states):
+            if state is not None:
+                self.state[p] = state
         for group in self.param_groups:
             group.setdefault("state_bits", self.defaults["state_bits"])
-            group["betas"] = tuple(group["betas"])
-        for i, (p, group) in zip(saved, params):
-            held = state_dict["state"].get(i)
-            if not held:
+            for p in group["params"]:
+                if p in self.state:
+                    group["state_bits"] = 8 if "exponents" in self.state[p] else 32
+
+    def _loaded(self, p: torch.Tensor, held: dict) -> dict:
+        """A saved state as this optimiser's, on the parameter's device."""
+        shapes = {"exp_avg": p.shape, "exp_avg_sq": p.shape, "master": p.shape, "exponents": (_num_blocks(p.shape), 2),
+                  "last_step": p.shape[:1]}
+        eight = "exponents" in held
+        moment = torch.uint8 if eight else torch.float32
+        types = {"exp_avg": moment, "exp_avg_sq": moment, "exponents": torch.uint8, "master": torch.float32, "last_step": torch.int32}
+        if not {"step", "exp_avg", "exp_avg_sq"} <= set(held):
+            raise ValueError("state_dict: no AdamW state")
+        count = int(held["step"])
+        state = dict(step=torch.full((), count, dtype=torch.int64, device=p.device) if self.capturable else count)
+        for name, shape in shapes.items():
+            if name not in held or (name == "master" and (not self.master_weights or p.dtype == torch.float32)):
                 continue
-            shapes = {"exp_avg": p.shape, "exp_avg_sq": p.shape, "master": p.shape, "exponents": (_num_blocks(p.shape), 2),
-                      "last_step": p.shape[:1]}
-            eight = "exponents" in held
-            types = {"exp_avg": torch.uint8 if eight else torch.float32, "exponents": torch.uint8, "master": torch.float32,
-                     "last_step": torch.int32}
-            types["exp_avg_sq"] = types["exp_avg"]
-            state = {}
-            for name, value in held.items():
-                if name == "step":
-                    state[name] = torch.full((), int(value), dtype=torch.int64, device=p.device) if self.capturable else int(value)
-                elif name in shapes:
-                    if tuple(value.shape) != tuple(shapes[name]):
-                        raise ValueError(f"state_dict: {name} has shape {tuple(value.shape)}, not {tuple(shapes[name])}")
-                    if eight and name.startswith("exp_avg") and value.dtype != torch.uint8:
-                        raise TypeError(f"state_dict: {name} with exponents is uint8, not {value.dtype}")
-                    state[name] = value.detach().to(device=p.device, dtype=types[name], copy=True).contiguous()
-            if not {"step", "exp_avg", "exp_avg_sq"} <= set(state):
-                raise ValueError("state_dict: no AdamW state")
-            if not self.master_weights:
-                state.pop("master", None)
-            elif p.dtype != torch.float32 and "master" not in state:
-                state["master"] = p.detach().to(torch.float32)
-            group["state_bits"] = 8 if eight else 32
-            self.state[p] = state
+            value = held[name]
+            if tuple(value.shape) != tuple(shape):
+                raise ValueError(f"state_dict: {name} has shape {tuple(value.shape)}, not {tuple(shape)}")
+            if (value.dtype == torch.uint8) != (types[name] == torch.uint8):
+                raise TypeError(f"state_dict: {name} is {value.dtype}, not {types[name]}")
+            state[name] = value.detach().to(device=p.device, dtype=types[name], copy=True).contiguous()
+        if self.master_weights and p.dtype != torch.float32 and "master" not in state:
+            state["master"] = p.detach().to(torch.float32)
+        return state

@@ -644,3 +644,116 @@ def test_offsets_beyond_32_bits():
             assert (got[s].cpu().numpy() == want).mean() > 1 - 1e-3
     total = float(o.grad_norm([g]))
     assert abs(total / n ** 0.5 - 1) < 1e-3
+
+
+def test_late_rows_of_long_gaps_against_64_bits():
+    """Gaps from 1 to 20000 steps: beta^d is right to 4 units of 2^-24 however large d is (hardware's exponential 2, the
+    correction and the product one each), so v', sums of positive terms, is right to 12 of them; below 2^-126 it may be zero."""
+    o = _optim()
+    shape = (4000, 56)
+    p, g, m, v, _ = _inputs(shape, torch.float32, 32, 6)
+    gaps = torch.cat([torch.arange(1, 2001), torch.randint(1, 20_000, (2000,), generator=torch.Generator().manual_seed(0))])
+    stamps = (30_000 - 1 - gaps).to(torch.int32).to(DEV)
+    before = [_np(t) for t in (p, g, m, v)]
+    o.adamw_step_([p], [g], [m], [v], step=30_000, row_masks=[torch.zeros(4000, dtype=torch.int8, device=DEV)], last_steps=[stamps], **HYPER)
+    _, wm, wv = plain.update(*before, step=30_000, missed=gaps.numpy(), **HYPER)
+    _assert_near(_np(v), wv, 12 * 2.0 ** -24 * wv + 2.0 ** -126, "exp_avg_sq")
+    _assert_near(_np(m), wm, 8 * 2.0 ** -24 * (np.abs(before[1]) + 0.9 ** gaps.numpy()[:, None] * np.abs(before[2])) + 2.0 ** -126, "exp_avg")
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_steps_and_rates_for_each_tensor_as_numbers_and_device_tensors_mixed(bits):
+    o = _optim()
+    kinds = [torch.float32, torch.bfloat16, torch.float32]
+    shapes = [(300, 3), (1000,), (77, 56)]
+    counts, rates = [3, 900, 17], [1e-3, 2e-3, 5e-4]
+    def run(as_tensor):
+        tensors = [_inputs(s, d, bits, 40 + i) for i, (s, d) in enumerate(zip(shapes, kinds))]
+        step = [torch.tensor(c, device=DEV) if as_tensor[0][i] else c for i, c in enumerate(counts)]
+        lr = [torch.tensor(r, device=DEV) if as_tensor[1][i] else float(np.float32(r)) for i, r in enumerate(rates)]
+        o.adamw_step_(*[[t[k] for t in tensors] for k in range(4)], step=step, lr=lr, weight_decay=[0.0, 0.1, 0.01],
+                      exponents=[t[4] for t in tensors] if bits == 8 else None, tensor_ids=[5, 1, 9], seed=-3)
+        return [x for t in tensors for x in t if x is not None]
+    want = run([[0] * 3, [0] * 3])
+    for as_tensor in ([[1, 0, 1], [0, 0, 0]], [[0, 0, 0], [0, 1, 1]], [[1, 1, 1], [1, 1, 1]]):
+        got = run(as_tensor)
+        # (the device's exponentials and logarithms in double precision may differ in their last bit: one unit of a float)
+        for a, b in zip(got, want):
+            if a.dtype == torch.uint8:
+                assert (a != b).float().mean() <= 1e-3
+            else:
+                assert ((a.float() - b.float()).abs() <= (2.0 ** -7 if a.dtype == torch.bfloat16 else 2.0 ** -22) * b.float().abs() + 1e-9).all()
+
+
+def test_gradients_that_are_not_contiguous_are_taken_as_they_are():
+    o = _optim()
+    def run(g):
+        p, _, m, v, _ = _inputs((120, 56), torch.float32, 32, 1)
+        norm = o.adamw_step_([p], [g], [m], [v], step=2, max_grad_norm=0.1, **HYPER)
+        return p, m, v, norm
+    base = torch.randn(56, 120, device=DEV)
+    wide = torch.randn(120, 70, device=DEV)
+    for g in (base.t(), wide[:, 7:63], torch.randn(1, 56, device=DEV).expand(120, 56), torch._neg_view(torch.randn(120, 56, device=DEV))):
+        for a, b in zip(run(g), run(g.clone(memory_format=torch.contiguous_format))):
+            assert torch.equal(a, b)
+
+
+def test_copies_of_an_optimiser_keep_what_it_was_told():
+    import copy
+    import pickle
+    o = _optim()
+    ps = _parameters(3)
+    mask = (torch.arange(1001, device=DEV) % 2).to(torch.int8)
+    opt = o.AdamW(ps, state_bits=8, max_grad_norm=0.5, seed=4)
+    opt.set_row_mask(ps[0], mask)
+    _feed(ps, 1)
+    opt.step()
+    twins = [copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))]
+    _feed(ps, 2)
+    opt.step()
+    for twin in twins:
+        qs = [q for group in twin.param_groups for q in group["params"]]
+        _feed(qs, 2)
+        twin.step()
+        assert torch.equal(twin.last_grad_norm, opt.last_grad_norm) and twin.seed == 4
+        for p, q in zip(ps, qs):
+            assert torch.equal(p, q) and torch.equal(opt.state[p]["exp_avg_sq"], twin.state[q]["exp_avg_sq"])
+
+
+def test_a_refused_state_dict_changes_nothing_and_moments_are_copies():
+    o = _optim()
+    ps = _parameters(2)
+    opt = o.AdamW(ps, state_bits=8)
+    _feed(ps, 0)
+    opt.step()
+    before = {k: t.clone() for k, t in opt.state[ps[1]].items() if isinstance(t, torch.Tensor)}
+    saved = opt.state_dict()
+    for change in (dict(amsgrad=True), dict(maximize=True)):
+        bad = {"state": saved["state"], "param_groups": [{**g, **change} for g in saved["param_groups"]]}
+        with pytest.raises(ValueError, match="amsgrad"):
+            opt.load_state_dict(bad)
+    broken = {"state": {k: dict(s) for k, s in saved["state"].items()}, "param_groups": saved["param_groups"]}
+    broken["state"][3].pop("exp_avg_sq")
+    with pytest.raises(ValueError, match="no AdamW state"):
+        opt.load_state_dict(broken)
+    with pytest.raises(ValueError):
+        opt.load_state_dict({"state": {}, "param_groups": saved["param_groups"] * 2})
+    for name, t in before.items():
+        assert torch.equal(opt.state[ps[1]][name], t) and opt.state[ps[1]][name].dtype == t.dtype
+    plain32 = o.AdamW(_parameters(2))
+    qs = plain32.param_groups[0]["params"]
+    _feed(qs, 0)
+    plain32.step()
+    m, _ = plain32.moments(qs[0])
+    m.zero_()
+    assert plain32.state[qs[0]]["exp_avg"].any()
+
+
+def test_reading_moments_into_overlapping_buffers_is_refused():
+    o = _optim()
+    m, v, x = o.new_moments(torch.zeros(640, device=DEV), 8)
+    out = torch.zeros(1000, device=DEV)
+    with pytest.raises(RuntimeError, match="overlaps"):
+        o.read_moments([m], [v], [x], out=([out[:640]], [out[300:940]]))
+    with pytest.raises(RuntimeError, match="overlaps"):
+        o.read_moments([m], [v], [x], out=([out[:640]], [out[:640]]))
