@@ -50,7 +50,7 @@ enum Form : int {
     QUADS,          // units of 64, or long rows: 16 lanes a unit, or 8 with pairs of quads
     QUADS_MASKED,   // the same rows under a mask: a wave packs the live ones
     NARROW,         // float rows of 1 to 4 elements: whole quads of rows a lane
-    ELEMENTS        // anything else, unaligned tensors: element by element
+    ELEMENTS        // rows of 5 to 16, or of lengths that are no multiple: element by element
 };
 
 struct AdamwTensor {
@@ -113,6 +113,13 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
+// A type at any address: the wide accesses need no alignment here, so views at odd offsets take the same code.
+template <typename T> struct Anywhere { typedef T type __attribute__((aligned(1))); };
+template <typename T>
+__device__ __forceinline__ T load_at(const void *p) { return *(const typename Anywhere<T>::type *)p; }
+template <typename T>
+__device__ __forceinline__ void store_at(void *p, T x) { *(typename Anywhere<T>::type *)p = x; }
+
 template <int DT> struct Four;
 template <> struct Four<GS_DTYPE_F32> { typedef f32x4 type; };
 template <> struct Four<GS_DTYPE_BF16> { typedef bf16x4 type; };
@@ -126,9 +133,8 @@ template <> struct Wide<GS_DTYPE_F16> { typedef f16x8 type; };
 
 template <int DT>
 __device__ __forceinline__ void store_four(void *p, long long i, f32x4 x) {
-    if (DT == GS_DTYPE_F32) *(f32x4 *)((float *)p + i) = x;
-    else if (DT == GS_DTYPE_BF16) *(bf16x4 *)((__bf16 *)p + i) = __builtin_convertvector(x, bf16x4);
-    else *(f16x4 *)((_Float16 *)p + i) = __builtin_convertvector(x, f16x4);
+    typedef typename Four<DT>::type V;
+    store_at((char *)p + i * (long long)(sizeof(V) / 4), __builtin_convertvector(x, V));
 }
 
 // ------------------------------------------------------------------ 8-bit moments
@@ -325,9 +331,9 @@ struct Buffers {
 // Parameter, gradient and moments are read once and written once a step, and the next reader of most of them is the next step:
 // they pass the caches by.
 template <typename T>
-__device__ __forceinline__ T stream_load(const char *p) { return __builtin_nontemporal_load((const T *)p); }
+__device__ __forceinline__ T stream_load(const void *p) { return __builtin_nontemporal_load((const typename Anywhere<T>::type *)p); }
 template <typename T>
-__device__ __forceinline__ void stream_store(char *p, T x) { __builtin_nontemporal_store(x, (T *)p); }
+__device__ __forceinline__ void stream_store(void *p, T x) { __builtin_nontemporal_store(x, (typename Anywhere<T>::type *)p); }
 
 // One or two quads of consecutive elements a lane: what a lane reads before the step and writes after it.  (Two float quads
 // a lane are no gain: an access of the wave then covers half of each cache line, and every line is asked for twice.)
@@ -351,11 +357,11 @@ struct Share {
     static __device__ __forceinline__ bool inside(uint32_t len, uint32_t sub) { return 4u * Q * sub < len; }
 
     template <typename T>
-    static __device__ __forceinline__ T get(const char *p) { return STREAM ? stream_load<T>(p) : *(const T *)p; }
+    static __device__ __forceinline__ T get(const char *p) { return STREAM ? stream_load<T>(p) : load_at<T>(p); }
     template <typename T>
     static __device__ __forceinline__ void put(char *p, T x) {
         if (STREAM) stream_store(p, x);
-        else *(T *)p = x;
+        else store_at(p, x);
     }
     __device__ __forceinline__ void load(const B &b) {
         if constexpr (PAIR) {
@@ -526,7 +532,7 @@ __device__ __forceinline__ void step_quads(const AdamwTensor &t, const AdamwScal
             const uint32_t unit = min(threadIdx.x / GROUP + u * PER_PASS, units - 1u);
             q[u].place(unit * unit_len, unit_len, sub);
             q[u].load(b);
-            x[u] = STATE8 ? *(const uint16_t *)(b.exponents + 2u * unit) : 0u;
+            x[u] = STATE8 ? load_at<uint16_t>(b.exponents + 2u * unit) : 0u;
         }
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
@@ -535,7 +541,7 @@ __device__ __forceinline__ void step_quads(const AdamwTensor &t, const AdamwScal
             const uint32_t new_x = q[u].template step<false>(p, x[u], 1.f, 1.f, b.quad, scale, k);
             if (unit < units && S::inside(unit_len, sub)) {
                 q[u].store(b, p);
-                if (STATE8 && sub == 0) *(uint16_t *)(b.exponents + 2u * unit) = (uint16_t)new_x;
+                if (STATE8 && sub == 0) store_at(b.exponents + 2u * unit, (uint16_t)new_x);
             }
         }
     }
@@ -563,7 +569,7 @@ __device__ __forceinline__ void step_quads_masked(const AdamwTensor &t, const Ad
     if (live) {
         row_decay(k, t.last_step[row0 + lane], decay_m, decay_v);
         t.last_step[row0 + lane] = k.step;
-        if (STATE8) x = *(const uint16_t *)(t.exponents + 2 * (row0 + lane));
+        if (STATE8) x = load_at<uint16_t>(t.exponents + 2 * (row0 + lane));
     }
     // lane i learns which lane has the i-th live row
     const int n_live = __popcll(lives);
@@ -588,7 +594,7 @@ __device__ __forceinline__ void step_quads_masked(const AdamwTensor &t, const Ad
         const uint32_t new_x = q[u].template step<true>(p, old_x, dm, dv, b.quad, scale, k);
         if (PER_PASS * u + (int)(lane / GROUP) < n_live && S::inside(row_len, sub)) {
             q[u].store(b, p);
-            if (STATE8 && sub == 0) *(uint16_t *)(b.exponents + 2 * from[u]) = (uint16_t)new_x;
+            if (STATE8 && sub == 0) store_at(b.exponents + 2 * from[u], (uint16_t)new_x);
         }
     }
 }
@@ -616,8 +622,8 @@ __device__ __forceinline__ void step_narrow(const AdamwTensor &t, const AdamwSca
     if (t.masked) {
         int8_t mask[R];
         int last[R];
-        __builtin_memcpy(mask, __builtin_assume_aligned((const int8_t *)t.master_or_mask + row0, R), R);
-        __builtin_memcpy(last, __builtin_assume_aligned(t.last_step + row0, 4 * R), 4 * R);
+        __builtin_memcpy(mask, (const int8_t *)t.master_or_mask + row0, R);
+        __builtin_memcpy(last, t.last_step + row0, 4 * R);
         bool any = false;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
@@ -629,7 +635,7 @@ __device__ __forceinline__ void step_narrow(const AdamwTensor &t, const AdamwSca
             }
         }
         if (!any) return;
-        __builtin_memcpy(__builtin_assume_aligned(t.last_step + row0, 4 * R), last, 4 * R);
+        __builtin_memcpy(t.last_step + row0, last, 4 * R);
     }
     const Buffers<GS_DTYPE_F32, false, STATE8> b(t, row0 * L, row0);
     Share<GS_DTYPE_F32, false, STATE8, false> q[Q];      // (cached: several accesses of the lane touch a line; 202 us, else 232)
@@ -639,7 +645,7 @@ __device__ __forceinline__ void step_narrow(const AdamwTensor &t, const AdamwSca
         q[c].e = 4u * c;
         q[c].load(b);
     }
-    if (STATE8) __builtin_memcpy(x, __builtin_assume_aligned(b.exponents, 2 * R), 2 * R);
+    if (STATE8) __builtin_memcpy(x, b.exponents, 2 * R);
     f32x4 p[Q][1];
     if constexpr (STATE8) {
         uint32_t mc[Q] = {}, vc[Q] = {};
@@ -673,7 +679,7 @@ __device__ __forceinline__ void step_narrow(const AdamwTensor &t, const AdamwSca
             q[c].mc[0] = mc[c];
             q[c].vc[0] = vc[c];
         }
-        __builtin_memcpy(__builtin_assume_aligned(b.exponents, 2 * R), x, 2 * R);
+        __builtin_memcpy(b.exponents, x, 2 * R);
     } else {
 #pragma unroll
         for (int e = 0; e < R * L; ++e) {
@@ -820,9 +826,9 @@ __device__ __forceinline__ void read_quads(const MomentsTensor &t, unsigned chun
         for (int u = 0; u < UNROLL; ++u) {
             const uint32_t unit = min(threadIdx.x / GROUP + u * PER_PASS, units - 1u);
             e[u] = unit * unit_len + min(4u * sub, unit_len - 4u);
-            mc[u] = *(const uint32_t *)(m + e[u]);
-            vc[u] = *(const uint32_t *)(v + e[u]);
-            x[u] = *(const uint16_t *)(exponents + 2u * unit);
+            mc[u] = load_at<uint32_t>(m + e[u]);
+            vc[u] = load_at<uint32_t>(v + e[u]);
+            x[u] = load_at<uint16_t>(exponents + 2u * unit);
         }
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u)
@@ -842,10 +848,10 @@ __device__ __forceinline__ void read_narrow(const MomentsTensor &t, unsigned chu
         return;
     }
     uint16_t x[R];
-    __builtin_memcpy(x, __builtin_assume_aligned(t.exponents + 2 * row0, 2 * R), 2 * R);
+    __builtin_memcpy(x, t.exponents + 2 * row0, 2 * R);
 #pragma unroll
     for (int c = 0; c < Q; ++c) {
-        const uint32_t mc = *(const uint32_t *)(t.m + row0 * L + 4 * c), vc = *(const uint32_t *)(t.v + row0 * L + 4 * c);
+        const uint32_t mc = load_at<uint32_t>(t.m + row0 * L + 4 * c), vc = load_at<uint32_t>(t.v + row0 * L + 4 * c);
         f32x4 m = units_of(mc), v;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -938,21 +944,20 @@ __device__ __forceinline__ double add_squares(double s, V x) {
     return s;
 }
 
-// Elements begin..end (begin is a multiple of 16 bytes: the chunk is aligned where the tensor is): 16 bytes a lane, AHEAD
-// requests in flight, past the end none.
+// Elements begin..end: 16 bytes a lane, AHEAD requests in flight, past the end none.
 template <int DT, bool STREAM>
 __device__ __forceinline__ double flat_squares(const void *grad, long long begin, long long end) {
     typedef typename Wide<DT>::type V;
     constexpr int N = 16 / (DT == GS_DTYPE_F32 ? 4 : 2), AHEAD = 4;
     double s = 0.0;
-    const unsigned wide = ((uintptr_t)grad & 15) == 0 ? (unsigned)((end - begin) / N) : 0u;
-    const V *g = (const V *)((const char *)grad + begin * (16 / N));
+    const unsigned wide = (unsigned)((end - begin) / N);
+    const char *g = (const char *)grad + begin * (16 / N);
     for (unsigned q = threadIdx.x; q < wide; q += AHEAD * GS_BLOCK) {
         V x[AHEAD];
 #pragma unroll
         for (int a = 0; a < AHEAD; ++a) {
             x[a] = {};
-            if (q + a * GS_BLOCK < wide) x[a] = STREAM ? __builtin_nontemporal_load(g + q + a * GS_BLOCK) : g[q + a * GS_BLOCK];
+            if (q + a * GS_BLOCK < wide) x[a] = STREAM ? stream_load<V>(g + 16ll * (q + a * GS_BLOCK)) : load_at<V>(g + 16ll * (q + a * GS_BLOCK));
         }
 #pragma unroll
         for (int a = 0; a < AHEAD; ++a) s = add_squares<N>(s, x[a]);
@@ -981,7 +986,7 @@ __device__ __forceinline__ double row_squares(const NormMaskedTensor &t, long lo
     return s;
 }
 
-// The same rows with aligned quads, rows of 20 to 64 elements: a wave packs the live ones of 64 rows and reads them four at a
+// The same for rows of 20, 24 .. 64 elements: a wave packs the live ones of 64 rows and reads them four at a
 // time, AHEAD of them in flight.
 template <int DT>
 __device__ __forceinline__ double packed_row_squares(const NormMaskedTensor &t, long long begin, long long end) {
@@ -1000,7 +1005,7 @@ __device__ __forceinline__ double packed_row_squares(const NormMaskedTensor &t, 
                 const int i = at + 4 * a + lane / GROUP;
                 const long long row = row0 + __shfl(order, i < n_live ? i : 0, GS_WAVE);
                 x[a] = {};
-                if (i < n_live && 4 * sub < len) x[a] = *(const decltype(+x[a]) *)((const char *)t.grad + (row * len + 4 * sub) * BYTES);
+                if (i < n_live && 4 * sub < len) x[a] = load_at<typename Four<DT>::type>((const char *)t.grad + (row * len + 4 * sub) * BYTES);
             }
 #pragma unroll
             for (int a = 0; a < AHEAD; ++a) s = add_squares<4>(s, x[a]);
@@ -1021,10 +1026,10 @@ __device__ __forceinline__ double narrow_squares(const NormMaskedTensor &t, long
                 for (int j = 0; j < L && t.row_mask[r] == 0; ++j) s = fma((double)grad[r * L + j], (double)grad[r * L + j], s);
             break;
         }
-        const uint32_t mask = *(const uint32_t *)(t.row_mask + row0);
+        const uint32_t mask = load_at<uint32_t>(t.row_mask + row0);
         f32x4 x[L];
 #pragma unroll
-        for (int c = 0; c < L; ++c) x[c] = *(const f32x4 *)(grad + row0 * L + 4 * c);
+        for (int c = 0; c < L; ++c) x[c] = load_at<f32x4>(grad + row0 * L + 4 * c);
 #pragma unroll
         for (int e = 0; e < 4 * L; ++e)
             if ((mask >> (8 * (e / L)) & 255u) == 0u) s = fma((double)x[e / 4][e % 4], (double)x[e / 4][e % 4], s);
@@ -1036,16 +1041,14 @@ template <int DT>
 __device__ __forceinline__ double masked_squares(const NormMaskedTensor &t, unsigned part, unsigned chunk) {
     const long long rows = t.numel / t.row_len, per = norm_rows(chunk, t.row_len);
     const long long begin = part * per, end = min(rows, begin + per);
-    const bool aligned = ((uintptr_t)t.grad & (DT == GS_DTYPE_F32 ? 15 : 7)) == 0;
-    if (t.row_len > 16) return aligned && t.row_len % 4 == 0 ? packed_row_squares<DT>(t, begin, end) : row_squares<16, DT>(t, begin, end);
+    if (t.row_len > 16) return t.row_len % 4 == 0 ? packed_row_squares<DT>(t, begin, end) : row_squares<16, DT>(t, begin, end);
     if (t.row_len > 4) return row_squares<4, DT>(t, begin, end);
-    if constexpr (DT == GS_DTYPE_F32)
-        if (aligned && ((uintptr_t)t.row_mask & 3) == 0) {
-            if (t.row_len == 3) return narrow_squares<3>(t, begin, end);
-            if (t.row_len == 1) return narrow_squares<1>(t, begin, end);
-            if (t.row_len == 2) return narrow_squares<2>(t, begin, end);
-            return narrow_squares<4>(t, begin, end);
-        }
+    if constexpr (DT == GS_DTYPE_F32) {
+        if (t.row_len == 3) return narrow_squares<3>(t, begin, end);
+        if (t.row_len == 1) return narrow_squares<1>(t, begin, end);
+        if (t.row_len == 2) return narrow_squares<2>(t, begin, end);
+        return narrow_squares<4>(t, begin, end);
+    }
     return row_squares<1, DT>(t, begin, end);
 }
 
@@ -1264,12 +1267,7 @@ extern "C" int gs_adamw_step(int n_tensors, const uint64_t *host_param, const ui
                 const u64 mask = entry(host_row_mask, i);
                 const int row = mask || state8 ? host_row_len[i] : 0;      // (moments in 32 bits without a mask: units of 64 whatever the shape)
                 const bool pair = pairs(dtype, master, state8);
-                const u64 moments = host_exp_avg[i] | host_exp_avg_sq[i];
-                const bool values = aligned_to(host_param[i] | host_grad[i], pair ? 16 : 4 * element_bytes(dtype)) && aligned_to(master ? host_master[i] : 0, 16);
-                const bool quads = values && (row == 0 || (row > 16 && row % (pair ? 8 : 4) == 0)) &&
-                                   aligned_to(moments, pair ? 8 : state8 ? 4 : 16) && aligned_to(entry(host_exponents, i), 2);
-                const bool narrow = values && dtype == GS_DTYPE_F32 && row >= 1 && row <= 4 && aligned_to(moments, state8 ? 4 : 16) &&
-                                    aligned_to(entry(host_exponents, i), 8) && aligned_to(mask, 4) && aligned_to(mask ? host_last_step[i] : 0, 16);
+                const bool quads = row == 0 || (row > 16 && row % (pair ? 8 : 4) == 0), narrow = dtype == GS_DTYPE_F32 && row >= 1 && row <= 4;
                 t.form = narrow ? NARROW : quads ? (mask ? QUADS_MASKED : QUADS) : ELEMENTS;
                 t.row_len = (uint8_t)row;
                 t.masked = mask != 0;
@@ -1370,11 +1368,9 @@ extern "C" int gs_read_moments(int n_tensors, const uint64_t *host_exp_avg, cons
         long long chunks = 0;
         if (!end) {
             const int row = host_row_len[i];
-            const bool fours = aligned_to(host_exp_avg[i] | host_exp_avg_sq[i], 4) && aligned_to(host_m_out[i] | host_v_out[i], 4 * element_bytes(out_dtype)) &&
-                               aligned_to(host_exponents[i], 2);
             t = {(const uint8_t *)host_exp_avg[i], (const uint8_t *)host_exp_avg_sq[i], (const uint8_t *)host_exponents[i],
                  (void *)host_m_out[i], (void *)host_v_out[i], host_numel[i], row, 0};
-            t.form = row >= 1 && row <= 4 && fours && aligned_to(host_exponents[i], 8) ? NARROW : fours && (row == 0 || (row > 16 && row % 4 == 0)) ? QUADS : ELEMENTS;
+            t.form = row >= 1 && row <= 4 ? NARROW : row == 0 || (row > 16 && row % 4 == 0) ? QUADS : ELEMENTS;
             chunks = form_chunks(t.form, host_numel[i], row, unroll, true);
         }
         if (b.n_tensors > 0 && (end || b.n_tensors == MAX_TENSORS || (long long)b.first_chunk[b.n_tensors] + chunks >= 0x7fffffffLL)) {
