@@ -30,8 +30,7 @@ constexpr long long NORM_STREAM_BYTES = 128LL << 20;
 
 // What a step needs besides the tensors; key and step belong to one tensor
 struct AdamwScalars {
-    float rate, root, keep, one_minus_beta1, beta2, one_minus_beta2, eps, beta1;   // rate = lr / (1 - b1^t), root = 1 / sqrt(1 - b2^t)
-    float log_beta1[2], log_beta2[2];       // log2 of the betas, each a float and what it lacks
+    float rate, root, keep, one_minus_beta1, beta2, one_minus_beta2, eps, beta1;    // rate = lr / (1 - b1^t), root = 1 / sqrt(1 - b2^t)
     int step;
     uint32_t key;
 };
@@ -247,35 +246,34 @@ __device__ __forceinline__ float update_one(float p, float g, float &m, float &v
 }
 
 // Moments in 8 bits are bound by their arithmetic: what is the same for a block goes into two factors, and the square root
-// and the reciprocal are the hardware's (one unit in the last place each; the codes do not depend on them).
+// and the reciprocal are the hardware's (one unit in the last place each; the codes do not depend on them).  The moments
+// themselves are computed one rounding an operation, as the formulas are written: a code is decided by the last bits of a
+// moment, and this way they are those of any other float implementation.
 struct OldBlock {
-    float m_factor, v_factor;       // beta1 2^(X - 135) and beta2, times what late rows lost; NaN for 255
+    float m_factor, v_factor;       // 2^(X - 135) and 1, times what late rows lost; NaN for 255
     uint32_t base;
-    __device__ __forceinline__ OldBlock(uint32_t x, float decay_m, float decay_v, const AdamwScalars &k)
-        : m_factor(k.beta1 * decay_m * m_scale(x)), v_factor(v_is_nan(x) ? __builtin_nanf("") : k.beta2 * decay_v), base(v_base(x)) {}
+    __device__ __forceinline__ OldBlock(uint32_t x, float decay_m, float decay_v)
+        : m_factor(decay_m * m_scale(x)), v_factor(v_is_nan(x) ? __builtin_nanf("") : decay_v), base(v_base(x)) {}
 };
-template <bool MASTER>
+// LATE: the row may have a decay.  (Without, beta2 joins the factor that is 1 or NaN: an operation less.)
+template <bool MASTER, bool LATE>
 __device__ __forceinline__ float update_coded(float p, float g, float m_unit, uint32_t v_old, const OldBlock &o, float &m, float &v, const AdamwScalars &k) {
-    m = fmaf(k.one_minus_beta1, g, o.m_factor * m_unit);
-    v = fmaf(k.one_minus_beta2 * g, g, o.v_factor * v_of(v_old, o.base));
+    {
+#pragma clang fp contract(off)
+        m = o.m_factor * m_unit;
+        m = m + k.one_minus_beta1 * (g - m);
+        const float old = v_of(v_old, o.base);
+        v = (LATE ? k.beta2 * (o.v_factor * old) : (k.beta2 * o.v_factor) * old) + k.one_minus_beta2 * g * g;
+    }
     return moved<MASTER>(p, m * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v) * k.root + k.eps), k);
-}
-
-// beta^d = 2^(d log2 beta): the product's rounding error and what the logarithm lacks follow as a factor, so that long gaps
-// lose nothing.
-__device__ __forceinline__ float beta_power(int d, const float (&log_beta)[2]) {
-    const float n = (float)d, x = n * log_beta[0];
-    const float rest = fmaf(n, log_beta[1], fmaf(n, log_beta[0], -x));
-    const float y = __builtin_amdgcn_exp2f(x);
-    return fmaf(y, 0.693147180559945f * rest, y);
 }
 
 // What a row that was last stepped at `last` has to be multiplied with before this step
 __device__ __forceinline__ void row_decay(const AdamwScalars &k, int last, float &decay_m, float &decay_v) {
     const int gap = k.step - 1 - last;
     if (gap > 0) {
-        decay_m = beta_power(gap, k.log_beta1);
-        decay_v = beta_power(gap, k.log_beta2);
+        decay_m = powf(k.beta1, (float)gap);
+        decay_v = powf(k.beta2, (float)gap);
     }
 }
 
@@ -410,14 +408,14 @@ struct Share {
 #pragma unroll
         for (int c = 0; c < Q; ++c) out[c] = __builtin_convertvector(p[c], f32x4);
         if constexpr (STATE8) {
-            const OldBlock o(x, decay_m, decay_v, k);
+            const OldBlock o(x, decay_m, decay_v);
 #pragma unroll
             for (int c = 0; c < Q; ++c) {
                 const f32x4 units = units_of(mc[c]), grad = __builtin_convertvector(g[c], f32x4);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     float mj, vj;
-                    out[c][j] = update_coded<MASTER>(out[c][j], scaled(grad[j], scale), units[j], (vc[c] >> (8 * j)) & 255u, o, mj, vj, k);
+                    out[c][j] = update_coded<MASTER, LATE>(out[c][j], scaled(grad[j], scale), units[j], (vc[c] >> (8 * j)) & 255u, o, mj, vj, k);
                     m[c][j] = mj;
                     v[c][j] = vj;
                 }
@@ -461,7 +459,7 @@ __device__ __forceinline__ void step_unit(const AdamwTensor &t, const AdamwScala
     const int count = live ? max(0, (len - sub + GROUP - 1) / GROUP) : 0;     // element j of this lane exists for j < count
     float p[4], m[4], v[4];
     const uint32_t x = STATE8 && live ? t.exponents[2 * unit] | (uint32_t)t.exponents[2 * unit + 1] << 8 : 0u;
-    const OldBlock o(x, decay_m, decay_v, k);
+    const OldBlock o(x, decay_m, decay_v);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         p[j] = m[j] = v[j] = 0.f;
@@ -470,7 +468,7 @@ __device__ __forceinline__ void step_unit(const AdamwTensor &t, const AdamwScala
             p[j] = MASTER ? ((const float *)t.master_or_mask)[i] : load_one<DT>(t.param, i);
             const float g = scaled(load_one<DT>(t.grad, i), scale);
             if (STATE8) {
-                p[j] = update_coded<MASTER>(p[j], g, unit_of(((const uint8_t *)t.exp_avg)[i]), ((const uint8_t *)t.exp_avg_sq)[i], o, m[j], v[j], k);
+                p[j] = update_coded<MASTER, true>(p[j], g, unit_of(((const uint8_t *)t.exp_avg)[i]), ((const uint8_t *)t.exp_avg_sq)[i], o, m[j], v[j], k);
             } else {
                 m[j] = ((const float *)t.exp_avg)[i] * decay_m;
                 v[j] = ((const float *)t.exp_avg_sq)[i] * decay_v;
@@ -651,13 +649,13 @@ __device__ __forceinline__ void step_narrow(const AdamwTensor &t, const AdamwSca
         uint32_t mc[Q] = {}, vc[Q] = {};
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const OldBlock o(x[r], decay_m[r], decay_v[r], k);
+            const OldBlock o(x[r], decay_m[r], decay_v[r]);
             float m[L], v[L];
             uint32_t top_m = 0u, top_v = 0u;
 #pragma unroll
             for (int i = 0; i < L; ++i) {
                 const int c = (r * L + i) / 4, j = (r * L + i) % 4;
-                const float out = update_coded<false>(q[c].p[0][j], scaled(q[c].g[0][j], scale), unit_at(q[c].mc[0], j), (q[c].vc[0] >> (8 * j)) & 255u, o, m[i], v[i], k);
+                const float out = update_coded<false, true>(q[c].p[0][j], scaled(q[c].g[0][j], scale), unit_at(q[c].mc[0], j), (q[c].vc[0] >> (8 * j)) & 255u, o, m[i], v[i], k);
                 p[c][0][j] = live[r] ? out : q[c].p[0][j];
                 top_m = max(top_m, to_bits(m[i]) & 0x7FFFFFFFu);
                 top_v = max(top_v, to_bits(v[i]) & 0x7FFFFFFFu);
@@ -754,12 +752,6 @@ __host__ __device__ AdamwScalars adamw_scalars(double lr, double beta1, double b
     k.one_minus_beta2 = (float)(1.0 - beta2);
     k.eps = (float)eps;
     k.beta1 = (float)beta1;
-    // (a beta of zero: any power is far below float's range)
-    const double l1 = beta1 > 0.0 ? log2(beta1) : -1e6, l2 = beta2 > 0.0 ? log2(beta2) : -1e6;
-    k.log_beta1[0] = (float)l1;
-    k.log_beta1[1] = (float)(l1 - (double)k.log_beta1[0]);
-    k.log_beta2[0] = (float)l2;
-    k.log_beta2[1] = (float)(l2 - (double)k.log_beta2[0]);
     k.key = tensor_key(seed, tensor, (uint32_t)step);
     k.step = (int)step;
     return k;
@@ -1145,7 +1137,7 @@ u64 entry(const uint64_t *column, int i) { return column ? column[i] : 0; }
 // Quads that a lane of step_quads takes.  8 bits: four, to have enough in flight; small totals one (a pair), so that they
 // still reach every compute unit.  32 bits: one, and at most four workgroups to a compute unit (OCCUPANCY_LDS bytes each of
 // shared memory that nothing uses): more requests to seven streams at once only lose the memory's open rows (1M points: four
-// quads 282 us, one 282, one with the limit 263, six streams of 1652 MB).
+// quads 282 us, one 282, one with the limit 263, seven streams of 1652 MB in all).
 constexpr int UNROLL = 4, UNROLL_READ = 4;
 constexpr int OCCUPANCY_LDS = 40960;
 constexpr long long SMALL_CHUNKS = 2048;    // of 16 units

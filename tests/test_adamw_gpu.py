@@ -647,8 +647,9 @@ def test_offsets_beyond_32_bits():
 
 
 def test_late_rows_of_long_gaps_against_64_bits():
-    """Gaps from 1 to 20000 steps: beta^d is right to 4 units of 2^-24 however large d is (hardware's exponential 2, the
-    correction and the product one each), so v', sums of positive terms, is right to 12 of them; below 2^-126 it may be zero."""
+    """Gaps from 1 to 20000 steps.  The power is that of beta rounded to float, so its relative error is d times that rounding's
+    (known: e1, e2), with 2 units of 2^-24 for the power and one for the product; the step adds 8 of v' (sums of positive
+    terms) and 4 of the parts of m'.  Below 2^-126 either may be zero."""
     o = _optim()
     shape = (4000, 56)
     p, g, m, v, _ = _inputs(shape, torch.float32, 32, 6)
@@ -657,8 +658,12 @@ def test_late_rows_of_long_gaps_against_64_bits():
     before = [_np(t) for t in (p, g, m, v)]
     o.adamw_step_([p], [g], [m], [v], step=30_000, row_masks=[torch.zeros(4000, dtype=torch.int8, device=DEV)], last_steps=[stamps], **HYPER)
     _, wm, wv = plain.update(*before, step=30_000, missed=gaps.numpy(), **HYPER)
-    _assert_near(_np(v), wv, 12 * 2.0 ** -24 * wv + 2.0 ** -126, "exp_avg_sq")
-    _assert_near(_np(m), wm, 8 * 2.0 ** -24 * (np.abs(before[1]) + 0.9 ** gaps.numpy()[:, None] * np.abs(before[2])) + 2.0 ** -126, "exp_avg")
+    d = gaps.numpy()[:, None].astype(np.float64)
+    e1, e2 = (abs(float(np.float32(b)) / b - 1) for b in HYPER["betas"])
+    u = 2.0 ** -24
+    _assert_near(_np(v), wv, (11 * u + np.expm1(d * e2)) * wv + 2.0 ** -126, "exp_avg_sq")
+    old = 0.9 ** d * np.abs(before[2])
+    _assert_near(_np(m), wm, 4 * u * np.abs(before[1]) + (7 * u + np.expm1(d * e1)) * old + 2.0 ** -126, "exp_avg")
 
 
 @pytest.mark.parametrize("bits", [32, 8])
