@@ -198,7 +198,7 @@ class GaussianPointCloudTrainer:
         num_data_loader_workers: int = 4
         seed: int = 0
         # "adam": the reference's two Adam optimisers.  "adamw": one optim.AdamW over features and positions (same rates and
-        # schedule) with decoupled weight decay, moments in 32 or 8 bits (8: 118 instead of 472 bytes a Gaussian) and
+        # schedule) with decoupled weight decay, moments in 32 or 8 bits (8: 122 instead of 472 bytes a Gaussian) and
         # clipping by the global gradient norm (0: off)
         optimizer: str = "adam"
         optimizer_state_bits: int = 32

@@ -5,9 +5,9 @@
 // launches the small ones.  Hence: one launch for many tensors (their addresses travel as kernel arguments: no table to
 // upload, nothing to keep, capturable), a workgroup finds its tensor from its block index.
 //
-// A tensor is cut into units: a row (1..64 elements) or 64 consecutive elements.  GROUP lanes (1, 4 or 16, the least that
-// hold a unit at four elements a lane) work on a unit, so the largest value of a block -- the 8-bit moments' exponent -- is
-// a reduction inside a DPP row: no shared memory, no barrier.
+// A tensor is cut into units: a row (1..64 elements) or 64 consecutive elements.  GROUP lanes (up to 16) work on a unit, so
+// the largest value of a block -- the 8-bit moments' exponent -- is a reduction inside a DPP row: no shared memory, no
+// barrier.
 #include "gs_common.h"
 
 #include <stdlib.h>
@@ -113,7 +113,7 @@ typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
 // A type at any address: the wide accesses need no alignment here, so views at odd offsets take the same code.
-template <typename T> struct Anywhere { typedef T type __attribute__((aligned(1))); };
+template <typename T> struct Anywhere { typedef T type __attribute__((aligned(1), may_alias)); };
 template <typename T>
 __device__ __forceinline__ T load_at(const void *p) { return *(const typename Anywhere<T>::type *)p; }
 template <typename T>
