@@ -282,7 +282,7 @@ PyObject *step(PyObject *args) {
     unsigned long long scale, workspace, stream;
     unsigned int seed;
     if (!PyArg_ParseTuple(args, "OOOKIKK", &collected, &numbers, &ids, &scale, &seed, &workspace, &stream)) return nullptr;
-    PyObject *c = tuple_of(PyTuple_GET_ITEM(tuple_of(collected, 4), 0), 8);
+    PyObject *c = tuple_of(PyTuple_GET_ITEM(tuple_of(collected, 6), 0), 8);
     tuple_of(numbers, 4);
     const Py_ssize_t n = PyBytes_GET_SIZE(PyTuple_GET_ITEM(collected, 1)) / 8;
     std::vector<int32_t> id(n);
@@ -299,10 +299,17 @@ PyObject *step(PyObject *args) {
     }
     if (!adamw_step) throw Refused{PyExc_RuntimeError, "the library is not bound"};
     typedef uint64_t U;
-    return PyLong_FromLong(adamw_step((int)n, column<U>(c, 0), column<U>(c, 1), column<U>(c, 2), column<U>(c, 3), column<U>(c, 4), column<U>(c, 5),
-                                      column<U>(c, 6), column<U>(c, 7), column<int64_t>(collected, 1), column<int32_t>(collected, 2), column<int32_t>(collected, 3),
-                                      id.data(), column<double>(numbers, 0), column<int64_t>(numbers, 1), column<U>(numbers, 2), column<U>(numbers, 3),
-                                      (const float *)scale, seed, (void *)workspace, (void *)stream));
+    const int status = adamw_step((int)n, column<U>(c, 0), column<U>(c, 1), column<U>(c, 2), column<U>(c, 3), column<U>(c, 4), column<U>(c, 5),
+                                  column<U>(c, 6), column<U>(c, 7), column<int64_t>(collected, 1), column<int32_t>(collected, 2), column<int32_t>(collected, 3),
+                                  id.data(), column<double>(numbers, 0), column<int64_t>(numbers, 1), column<U>(numbers, 2), column<U>(numbers, 3),
+                                  (const float *)scale, seed, (void *)workspace, (void *)stream);
+    // A graph that has kept a parameter for its backward pass must notice that it changed, as after any operation in place.
+    PyObject *params = PyList_GET_ITEM(PyTuple_GET_ITEM(collected, 5), 0);
+    for (Py_ssize_t i = 0; status == 0 && i < PySequence_Fast_GET_SIZE(params); ++i) {
+        PyObject *p = PySequence_Fast_GET_ITEM(params, i);
+        if (THPVariable_Check(p) && !THPVariable_Unpack(p).is_inference()) THPVariable_Unpack(p).unsafeGetTensorImpl()->bump_version();
+    }
+    return PyLong_FromLong(status);
 }
 
 // norm(grads column, row mask column, collected, max_norm, sq_sum, norm, clip, each or 0, workspace, stream): status of gs_grad_norm

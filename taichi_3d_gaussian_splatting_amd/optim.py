@@ -374,12 +374,17 @@ class AdamW(torch.optim.Optimizer):
                 steps = [s["step"] + 1 for s in states]
             masters = [s.get("master") for s in states] if self.master_weights else None
             masked = any(mask is not None for mask in masks)
-            adamw_step_(params, grads, [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states], step=steps, lr=rates,
-                        betas=betas, eps=eps, weight_decay=decays,
-                        exponents=[s["exponents"] for s in states] if eight else None, masters=masters,
-                        row_masks=masks if masked else None,
-                        last_steps=[None if mask is None else s["last_step"] for s, mask in zip(states, masks)] if masked else None,
-                        grad_scale=clip, seed=self.seed, tensor_ids=ids)
+            try:
+                adamw_step_(params, grads, [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states], step=steps, lr=rates,
+                            betas=betas, eps=eps, weight_decay=decays,
+                            exponents=[s["exponents"] for s in states] if eight else None, masters=masters,
+                            row_masks=masks if masked else None,
+                            last_steps=[None if mask is None else s["last_step"] for s, mask in zip(states, masks)] if masked else None,
+                            grad_scale=clip, seed=self.seed, tensor_ids=ids)
+            except Exception:
+                if self.capturable:         # (a refused step has not happened)
+                    torch._foreach_add_(steps, -1)
+                raise
             if not self.capturable:
                 for state, count in zip(states, steps):
                     state["step"] = count

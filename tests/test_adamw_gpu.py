@@ -762,3 +762,58 @@ def test_reading_moments_into_overlapping_buffers_is_refused():
         o.read_moments([m], [v], [x], out=([out[:640]], [out[300:940]]))
     with pytest.raises(RuntimeError, match="overlaps"):
         o.read_moments([m], [v], [x], out=([out[:640]], [out[:640]]))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_graph_that_kept_a_parameter_notices_the_step(dtype):
+    p = torch.nn.Parameter(torch.randn(100, device=DEV).to(dtype))
+    opt = _optim().AdamW([p], lr=1e-2)
+    y = (p * p).sum()
+    p.grad = torch.ones_like(p)
+    before = p._version
+    opt.step()
+    assert p._version > before
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        y.backward()
+    (p * p).sum().backward()
+
+
+def test_a_refused_capturable_step_does_not_count():
+    p = torch.nn.Parameter(torch.randn(6, 8, device=DEV))
+    opt = _optim().AdamW([p], lr=1e-2, capturable=True)
+    p.grad = torch.ones_like(p)
+    opt.step()
+    kept, version = p.detach().clone(), p._version
+    p.grad = torch.sparse_coo_tensor([[1], [2]], [1.0], p.shape, device=DEV)
+    with pytest.raises(RuntimeError, match="sparse"):
+        opt.step()
+    assert int(opt.state[p]["step"]) == 1 and torch.equal(p, kept) and p._version == version
+
+
+def test_steps_from_two_threads_equal_steps_from_one():
+    import threading
+    optim = _optim()
+
+    def run(seed, out):
+        gen = torch.Generator().manual_seed(seed)
+        params = [torch.randn(n, generator=gen).to(DEV) for n in (1, 100, 5000, 300000)]
+        opt = optim.AdamW(params, lr=1e-2, state_bits=8, max_grad_norm=1.0, seed=seed)
+        with torch.cuda.stream(torch.cuda.Stream()):
+            torch.cuda.current_stream().wait_stream(torch.cuda.default_stream())
+            for _ in range(20):
+                for p in params:
+                    p.grad = torch.randn(p.shape, generator=gen).to(DEV)
+                opt.step()
+            torch.cuda.current_stream().synchronize()
+        out[seed] = params
+
+    alone, together = {}, {}
+    for seed in (1, 2):
+        run(seed, alone)
+    threads = [threading.Thread(target=run, args=(seed, together)) for seed in (1, 2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    for seed in (1, 2):
+        assert all(torch.equal(a, b) for a, b in zip(alone[seed], together[seed])), seed
