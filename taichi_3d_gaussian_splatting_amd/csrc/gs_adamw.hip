@@ -42,15 +42,24 @@ constexpr bool pairs(int dtype, bool master, bool state8) { return state8 && dty
 // Rows under a mask that a wave packs, all of them in flight.  us of a step of 1.2M rows, all live / 30 % at random / the first
 // 30 %: 32 bits: 16 rows 335 / 175 / 114, 32: 362 / 182 / 117, 64: 376 / 173 / 128; 8 bits: 196 / 118 / 76, 203 / 122 / 73,
 // 215 / 127 / 74, and 132, 120, 121 of the second where a tenth of the rows comes back late.
-constexpr int masked_rows(bool state8) { return state8 ? 32 : 16; }
+// Shorter rows: as many quads in flight, up to a row a lane.
+__host__ __device__ constexpr int masked_rows(int lanes, bool state8) { return lanes <= 4 || (lanes == 8 && state8) ? GS_WAVE : GS_WAVE / lanes * (state8 ? 8 : 4); }
 
 // How a tensor is cut among lanes
 enum Form : int {
-    QUADS,          // units of 64, or long rows: 16 lanes a unit, or 8 with pairs of quads
-    QUADS_MASKED,   // the same rows under a mask: a wave packs the live ones
+    QUADS,          // units of 64, or rows of 36, 40 .. 64 (of 40, 48 .. with pairs of quads): 16 lanes a unit, or 8 with pairs
+    ROWS,           // other rows from five elements on: 2, 4, 8 or 16 lanes a row
+    QUADS_MASKED,   // the rows of QUADS under a mask: a wave packs the live ones
+    ROWS_MASKED,    // the rows of ROWS under a mask, the same way
     NARROW,         // float rows of 1 to 4 elements: whole quads of rows a lane
-    ELEMENTS        // rows of 5 to 16, or of lengths that are no multiple: element by element
+    ELEMENTS        // 16-bit rows of 1 to 4 elements: a row a lane, element by element
 };
+// Passes of a lane over its workgroup's units, of a quad each, or of a pair where QUADS has pairs (ROWS has none)
+constexpr int passes(int quads, bool pair) { return pair ? (quads + 1) / 2 : quads; }
+// Lanes for a row of ROWS.  40M floats with 8-bit moments in rows of 5 / 8 / 17 / 24 / 45: 128 / 107 / 139 / 110 / 127 us (element by
+// element 404 / 278 / 461 / 178 / 235; 16 lanes for all would idle most of them), rows of 56 as QUADS 113; all live under a mask
+// 205 / 134 / 159 / 121 / 139 (646 / 426 / 715 / 176 / 325), rows of 56 118.
+__host__ __device__ constexpr int lanes_of(int row_len) { return row_len == 0 || row_len > 32 ? 16 : (row_len > 16 ? 8 : (row_len > 8 ? 4 : 2)); }
 
 struct AdamwTensor {
     void *param;
@@ -192,13 +201,13 @@ __device__ __forceinline__ uint32_t pack_top_bytes(uint32_t a, uint32_t b, uint3
     return __builtin_amdgcn_perm(b, a, 0x0c0c0703u) | __builtin_amdgcn_perm(d, c, 0x07030c0cu);
 }
 
-// Largest of GROUP consecutive lanes, in all of them (GROUP = 4: quad permutations, 8: and a mirrored half row, 16: rotations
+// Largest of GROUP consecutive lanes, in all of them (GROUP = 2, 4: quad permutations, 8: and a mirrored half row, 16: rotations
 // of a DPP row)
 template <int GROUP>
 __device__ __forceinline__ uint32_t group_max(uint32_t x) {
-    if (GROUP == 4 || GROUP == 8) {
+    if (GROUP == 2 || GROUP == 4 || GROUP == 8) {
         x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0xB1, 0xF, 0xF, true));
-        x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x4E, 0xF, 0xF, true));
+        if (GROUP > 2) x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x4E, 0xF, 0xF, true));
         if (GROUP == 8) x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x141, 0xF, 0xF, true));
     } else if (GROUP == 16) {
         x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x128, 0xF, 0xF, true));
@@ -277,9 +286,10 @@ __device__ __forceinline__ void row_decay(const AdamwScalars &k, int last, float
     }
 }
 
-// Codes and exponent bytes of a block from the lanes that share it: Q quads of consecutive elements a lane
-template <int GROUP, int Q>
-__device__ __forceinline__ uint32_t encode(const f32x4 (&m)[Q], const f32x4 (&v)[Q], uint32_t quad, uint32_t key, uint32_t (&mc)[Q], uint32_t (&vc)[Q]) {
+// Codes and exponent bytes of a block from the lanes that share it: Q quads of consecutive elements a lane, the first of
+// which begins at element 4 quad + shift; SHIFTED: shift may be other than 0, so that a quad's elements meet two hashes.
+template <int GROUP, bool SHIFTED, int Q>
+__device__ __forceinline__ uint32_t encode(const f32x4 (&m)[Q], const f32x4 (&v)[Q], uint32_t quad, uint32_t shift, uint32_t key, uint32_t (&mc)[Q], uint32_t (&vc)[Q]) {
     uint32_t top_m = 0u, top_v = 0u;
 #pragma unroll
     for (int e = 0; e < 4 * Q; ++e) {
@@ -291,13 +301,16 @@ __device__ __forceinline__ uint32_t encode(const f32x4 (&m)[Q], const f32x4 (&v)
     const uint32_t base = (xv - 31u) << 23;
 #pragma unroll
     for (int c = 0; c < Q; ++c) {
-        const uint32_t hash = mix32((quad + c) ^ key);
+        const uint32_t hash = mix32((quad + c) ^ key), next = SHIFTED ? mix32((quad + c + 1u) ^ key) : 0u;
         uint32_t w[4];
         vc[c] = 0u;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            w[j] = m_word(m[c][j], xm, bits_for_m(hash, j));
-            vc[c] |= v_code(v[c][j], base, bits_for_v(hash, j)) << (8 * j);
+            // (element j's place in its aligned quad is (shift + j) % 4: the rotation by 8 times that, the last two bits of the
+            // shift being all that it takes)
+            const uint32_t h = SHIFTED ? __builtin_rotateleft32(shift + j < 4u ? hash : next, 8u * (shift & 3u)) : hash;
+            w[j] = m_word(m[c][j], xm, bits_for_m(h, j));
+            vc[c] |= v_code(v[c][j], base, bits_for_v(h, j)) << (8 * j);
         }
         mc[c] = xm == 255u ? 0u : pack_top_bytes(w[0], w[1], w[2], w[3]);
         vc[c] = xv == 255u ? 0u : vc[c];
@@ -313,7 +326,7 @@ struct Buffers {
     const char *grad;
     char *m, *v;
     uint8_t *exponents;
-    uint32_t quad;          // the first element's index / 4, for the rounding bits
+    uint32_t quad, shift;   // the first element's index / 4 and the rest, for the rounding bits
     __device__ __forceinline__ Buffers(const AdamwTensor &t, long long element, long long unit) {
         constexpr int BYTES = DT == GS_DTYPE_F32 ? 4 : 2, STATE = STATE8 ? 1 : 4;
         source = (const char *)(MASTER ? t.master_or_mask : t.param) + element * (MASTER ? 4 : BYTES);
@@ -323,6 +336,7 @@ struct Buffers {
         v = (char *)t.exp_avg_sq + element * STATE;
         exponents = t.exponents + 2 * unit;
         quad = (uint32_t)(element >> 2);
+        shift = (uint32_t)element & 3u;
     }
 };
 
@@ -335,15 +349,17 @@ __device__ __forceinline__ void stream_store(void *p, T x) { __builtin_nontempor
 
 // One or two quads of consecutive elements a lane: what a lane reads before the step and writes after it.  (Two float quads
 // a lane are no gain: an access of the wave then covers half of each cache line, and every line is asked for twice.)
-template <int DT, bool MASTER, bool STATE8, bool STREAM = true>
+// LANES: of a row of any length from 4 elements on, 0 for units of QUADS.  Where a row's length is no multiple of four its last
+// lane takes the last four elements, some of which its neighbour has, too: both read them before either writes the same result.
+template <int DT, bool MASTER, bool STATE8, int LANES = 0, bool STREAM = true>
 struct Share {
     typedef Buffers<DT, MASTER, STATE8> B;
     typedef typename Four<DT>::type Value;
     typedef typename Four<MASTER ? GS_DTYPE_F32 : DT>::type Source;
     typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-    static constexpr bool PAIR = pairs(DT, MASTER, STATE8);
-    static constexpr int Q = PAIR ? 2 : 1, GROUP = 16 / Q;
+    static constexpr bool PAIR = LANES == 0 && pairs(DT, MASTER, STATE8);
+    static constexpr int Q = PAIR ? 2 : 1, GROUP = LANES > 0 ? LANES : 16 / Q;
     Source p[Q];
     Value g[Q];
     f32x4 m[Q], v[Q];
@@ -404,7 +420,7 @@ struct Share {
     }
     // The step; returns the exponent bytes of the block that GROUP lanes share
     template <bool LATE>
-    __device__ __forceinline__ uint32_t step(f32x4 (&out)[Q], uint32_t x, float decay_m, float decay_v, uint32_t first_quad, float scale, const AdamwScalars &k) {
+    __device__ __forceinline__ uint32_t step(f32x4 (&out)[Q], uint32_t x, float decay_m, float decay_v, const B &b, float scale, const AdamwScalars &k) {
 #pragma unroll
         for (int c = 0; c < Q; ++c) out[c] = __builtin_convertvector(p[c], f32x4);
         if constexpr (STATE8) {
@@ -420,7 +436,8 @@ struct Share {
                     v[c][j] = vj;
                 }
             }
-            return encode<GROUP>(m, v, first_quad + (e >> 2), k.key, mc, vc);
+            const uint32_t at = b.shift + e;
+            return encode<GROUP, (LANES > 0)>(m, v, b.quad + (LANES > 0 ? at : e) / 4u, at % 4u, k.key, mc, vc);
         } else {
 #pragma unroll
             for (int c = 0; c < Q; ++c) {
@@ -442,7 +459,8 @@ struct Share {
     }
 };
 
-// The element-wise form: GROUP lanes take a unit, elements GROUP apart.
+// The element-wise form, for what the others leave: the last unit of a flat tensor (GROUP 16), narrow rows behind the last whole
+// quads and 16-bit rows of 1 to 4 elements (GROUP 1).  GROUP lanes take a unit, elements GROUP apart.
 template <int GROUP, int DT, bool MASTER, bool STATE8>
 __device__ __forceinline__ void step_unit(const AdamwTensor &t, const AdamwScalars &k, float scale, long long unit, int unit_len) {
     const int sub = threadIdx.x % GROUP;
@@ -511,11 +529,12 @@ __device__ __forceinline__ void step_unit(const AdamwTensor &t, const AdamwScala
     }
 }
 
-// A workgroup's share in units is 16 (32 with pairs) times UNROLL; a lane asks for all its units' data before it uses any.
-// Lanes past a row's end and units past the tensor's read their neighbours' data again (the same largest value) and store nothing.
-template <int UNROLL, int DT, bool MASTER, bool STATE8>
+// A workgroup's share in units is a block's groups of lanes times UNROLL; a lane asks for all its units' data before it uses
+// any.  Lanes past a row's end and units past the tensor's read their neighbours' data again (the same largest value) and store
+// nothing.
+template <int UNROLL, int DT, bool MASTER, bool STATE8, int LANES>
 __device__ __forceinline__ void step_quads(const AdamwTensor &t, const AdamwScalars &k, float scale, unsigned chunk) {
-    typedef Share<DT, MASTER, STATE8> S;
+    typedef Share<DT, MASTER, STATE8, LANES> S;
     constexpr int GROUP = S::GROUP, PER_PASS = GS_BLOCK / GROUP, SHARE = PER_PASS * UNROLL;
     const uint32_t unit_len = t.row_len > 0 ? t.row_len : UNIT;
     const long long chunk_unit = (long long)chunk * SHARE, whole = t.numel / unit_len;         // units of full length
@@ -536,7 +555,7 @@ __device__ __forceinline__ void step_quads(const AdamwTensor &t, const AdamwScal
         for (int u = 0; u < UNROLL; ++u) {
             const uint32_t unit = threadIdx.x / GROUP + u * PER_PASS;
             f32x4 p[S::Q];
-            const uint32_t new_x = q[u].template step<false>(p, x[u], 1.f, 1.f, b.quad, scale, k);
+            const uint32_t new_x = q[u].template step<false>(p, x[u], 1.f, 1.f, b, scale, k);
             if (unit < units && S::inside(unit_len, sub)) {
                 q[u].store(b, p);
                 if (STATE8 && sub == 0) store_at(b.exponents + 2u * unit, (uint16_t)new_x);
@@ -544,16 +563,16 @@ __device__ __forceinline__ void step_quads(const AdamwTensor &t, const AdamwScal
         }
     }
     // the last unit of a flat tensor, where it is shorter
-    if (whole * unit_len < t.numel && whole >= chunk_unit && whole < chunk_unit + SHARE && threadIdx.x < GS_WAVE)
+    if (LANES == 0 && whole * unit_len < t.numel && whole >= chunk_unit && whole < chunk_unit + SHARE && threadIdx.x < GS_WAVE)
         step_unit<16, DT, MASTER, STATE8>(t, k, scale, whole + threadIdx.x / 16, (int)unit_len);
 }
 
-// Rows under a mask: a wave reads the mask and the stamps of its rows, packs the live ones and steps them four at a time, so
+// Rows under a mask: a wave reads the mask and the stamps of its rows, packs the live ones and steps them PER_PASS at a time, so
 // that no lane waits beside a row without a point and none of such a row's data is asked for.
-template <int UNROLL, bool STATE8>
+template <bool STATE8, int LANES>
 __device__ __forceinline__ void step_quads_masked(const AdamwTensor &t, const AdamwScalars &k, float scale, unsigned chunk) {
-    typedef Share<GS_DTYPE_F32, false, STATE8> S;
-    constexpr int GROUP = S::GROUP, PER_PASS = GS_WAVE / GROUP, WAVE_ROWS = PER_PASS * UNROLL;
+    typedef Share<GS_DTYPE_F32, false, STATE8, LANES> S;
+    constexpr int GROUP = S::GROUP, PER_PASS = GS_WAVE / GROUP, WAVE_ROWS = masked_rows(GROUP, STATE8), UNROLL = WAVE_ROWS / PER_PASS;
     const uint32_t row_len = t.row_len, lane = gs_lane(), sub = lane % GROUP;
     const long long row0 = ((long long)chunk * (GS_BLOCK / GS_WAVE) + __builtin_amdgcn_readfirstlane(threadIdx.x / GS_WAVE)) * WAVE_ROWS;
     const long long rows = t.numel / row_len;
@@ -589,7 +608,7 @@ __device__ __forceinline__ void step_quads_masked(const AdamwTensor &t, const Ad
         const uint32_t old_x = STATE8 ? (uint32_t)__shfl(x, from[u], GS_WAVE) : 0u;
         const float dm = any_late ? __shfl(decay_m, from[u], GS_WAVE) : 1.f, dv = any_late ? __shfl(decay_v, from[u], GS_WAVE) : 1.f;
         f32x4 p[S::Q];
-        const uint32_t new_x = q[u].template step<true>(p, old_x, dm, dv, b.quad, scale, k);
+        const uint32_t new_x = q[u].template step<true>(p, old_x, dm, dv, b, scale, k);
         if (PER_PASS * u + (int)(lane / GROUP) < n_live && S::inside(row_len, sub)) {
             q[u].store(b, p);
             if (STATE8 && sub == 0) store_at(b.exponents + 2 * from[u], (uint16_t)new_x);
@@ -598,106 +617,127 @@ __device__ __forceinline__ void step_quads_masked(const AdamwTensor &t, const Ad
 }
 
 // Float rows of L = 1..4 elements, as many rows a lane as make whole quads (rows of three: four rows, three quads): every access
-// is 16 bytes (4 for codes) although a row is not.  Of rows under a mask the lane writes back what it read.
+// is 16 bytes (4 for codes) although a row is not.  Of rows under a mask the lane writes back what it read.  With codes of one
+// quad only a lane has too little in flight: it takes rows at two places (40M floats, rows of 1 / 2 / 4: 157 / 143 / 136 us at
+// one, 145 / 134 / 127 at two, 152 / 140 / 132 at four; all live under a mask 268 / 237 / 235, 210 / 179 / 164, 217 / 181 / 155).
 __host__ __device__ constexpr int narrow_rows(int row_len) { return row_len == 4 ? 1 : (row_len == 2 ? 2 : 4); }
+__host__ __device__ constexpr int narrow_passes(int row_len, bool state8) { return state8 && row_len != 3 ? 2 : 1; }
 
-template <int L, bool STATE8>
+template <int L, bool STATE8, bool MASKED>
 __device__ __forceinline__ void step_narrow(const AdamwTensor &t, const AdamwScalars &k, float scale, unsigned chunk) {
-    constexpr int R = narrow_rows(L), Q = R * L / 4;
-    const long long rows = t.numel / L, row0 = R * ((long long)chunk * GS_BLOCK + threadIdx.x);
-    if (row0 >= rows) return;
-    if (row0 + R > rows) {
-        for (long long r = row0; r < rows; ++r) step_unit<1, GS_DTYPE_F32, false, STATE8>(t, k, scale, r, L);
-        return;
-    }
-    bool live[R];
-    float decay_m[R], decay_v[R];
+    constexpr int R = narrow_rows(L), Q = R * L / 4, PASSES = narrow_passes(L, STATE8), SHARE = R * PASSES * GS_BLOCK;
+    const long long rows = t.numel / L, first = (long long)chunk * SHARE;
+    const int left = (int)min((long long)SHARE, rows - first);
+    const Buffers<GS_DTYPE_F32, false, STATE8> b(t, first * L, first);
+    const int8_t *mask_of = (const int8_t *)t.master_or_mask + (MASKED ? first : 0);
+    int32_t *stamps = t.last_step + (MASKED ? first : 0);
+    int8_t mask[PASSES][R];
+    int last[PASSES][R];
+    bool go[PASSES];
+    Share<GS_DTYPE_F32, false, STATE8, 0, false> q[PASSES][Q];      // (cached: several accesses of the lane touch a line; 202 us, else 232)
+    uint16_t x[PASSES][R];
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        live[r] = true;
-        decay_m[r] = decay_v[r] = 1.f;
-    }
-    if (t.masked) {
-        int8_t mask[R];
-        int last[R];
-        __builtin_memcpy(mask, (const int8_t *)t.master_or_mask + row0, R);
-        __builtin_memcpy(last, t.last_step + row0, 4 * R);
-        bool any = false;
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            live[r] = mask[r] == 0;
-            any = any || live[r];
-            if (live[r]) {
-                row_decay(k, last[r], decay_m[r], decay_v[r]);
-                last[r] = k.step;
-            }
+    for (int u = 0; u < PASSES; ++u) {
+        const int row = R * (u * GS_BLOCK + (int)threadIdx.x);
+        go[u] = row + R <= left;
+        if (MASKED && go[u]) {
+            __builtin_memcpy(mask[u], mask_of + row, R);
+            __builtin_memcpy(last[u], stamps + row, 4 * R);
         }
-        if (!any) return;
-        __builtin_memcpy(t.last_step + row0, last, 4 * R);
     }
-    const Buffers<GS_DTYPE_F32, false, STATE8> b(t, row0 * L, row0);
-    Share<GS_DTYPE_F32, false, STATE8, false> q[Q];      // (cached: several accesses of the lane touch a line; 202 us, else 232)
-    uint16_t x[R];
 #pragma unroll
-    for (int c = 0; c < Q; ++c) {
-        q[c].e = 4u * c;
-        q[c].load(b);
+    for (int u = 0; u < PASSES; ++u) {
+        const int row = R * (u * GS_BLOCK + (int)threadIdx.x);
+        if (MASKED) {
+            bool any = false;
+#pragma unroll
+            for (int r = 0; r < R; ++r) any = any || mask[u][r] == 0;
+            go[u] = go[u] && any;
+        }
+        if (!go[u]) continue;
+#pragma unroll
+        for (int c = 0; c < Q; ++c) {
+            q[u][c].e = (uint32_t)(row * L + 4 * c);
+            q[u][c].load(b);
+        }
+        if (STATE8) __builtin_memcpy(x[u], b.exponents + 2 * row, 2 * R);
     }
-    if (STATE8) __builtin_memcpy(x, b.exponents, 2 * R);
-    f32x4 p[Q][1];
-    if constexpr (STATE8) {
+#pragma unroll
+    for (int u = 0; u < PASSES; ++u) {
+        if (!go[u]) continue;
+        const int row = R * (u * GS_BLOCK + (int)threadIdx.x);
+        f32x4 p[Q][1];
         uint32_t mc[Q] = {}, vc[Q] = {};
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const OldBlock o(x[r], decay_m[r], decay_v[r]);
-            float m[L], v[L];
-            uint32_t top_m = 0u, top_v = 0u;
-#pragma unroll
-            for (int i = 0; i < L; ++i) {
-                const int c = (r * L + i) / 4, j = (r * L + i) % 4;
-                const float out = update_coded<false, true>(q[c].p[0][j], scaled(q[c].g[0][j], scale), unit_at(q[c].mc[0], j), (q[c].vc[0] >> (8 * j)) & 255u, o, m[i], v[i], k);
-                p[c][0][j] = live[r] ? out : q[c].p[0][j];
-                top_m = max(top_m, to_bits(m[i]) & 0x7FFFFFFFu);
-                top_v = max(top_v, to_bits(v[i]) & 0x7FFFFFFFu);
+            const bool live = !MASKED || mask[u][r] == 0;
+            float decay_m = 1.f, decay_v = 1.f;
+            if (MASKED && live) {
+                row_decay(k, last[u][r], decay_m, decay_v);
+                last[u][r] = k.step;
             }
-            const uint32_t xm = block_exponent(top_m, CARRY_M, LOW_M), xv = block_exponent(top_v, CARRY_V, LOW_V);
+            if constexpr (STATE8) {
+                const OldBlock o(x[u][r], decay_m, decay_v);
+                float m[L], v[L];
+                uint32_t top_m = 0u, top_v = 0u;
 #pragma unroll
-            for (int i = 0; i < L; ++i) {
-                const int c = (r * L + i) / 4, j = (r * L + i) % 4;
-                const uint32_t hash = mix32((b.quad + c) ^ k.key);
-                const uint32_t a = xm == 255u ? 0u : m_word(m[i], xm, bits_for_m(hash, j)) >> 24;
-                const uint32_t d = xv == 255u ? 0u : v_code(v[i], (xv - 31u) << 23, bits_for_v(hash, j));
-                mc[c] |= live[r] ? a << (8 * j) : q[c].mc[0] & (255u << (8 * j));
-                vc[c] |= live[r] ? d << (8 * j) : q[c].vc[0] & (255u << (8 * j));
+                for (int i = 0; i < L; ++i) {
+                    const int c = (r * L + i) / 4, j = (r * L + i) % 4;
+                    const auto &s = q[u][c];
+                    const float out = update_coded<false, MASKED>(s.p[0][j], scaled(s.g[0][j], scale), unit_at(s.mc[0], j), (s.vc[0] >> (8 * j)) & 255u, o, m[i], v[i], k);
+                    p[c][0][j] = live ? out : s.p[0][j];
+                    top_m = max(top_m, to_bits(m[i]) & 0x7FFFFFFFu);
+                    top_v = max(top_v, to_bits(v[i]) & 0x7FFFFFFFu);
+                }
+                const uint32_t xm = block_exponent(top_m, CARRY_M, LOW_M), xv = block_exponent(top_v, CARRY_V, LOW_V);
+#pragma unroll
+                for (int i = 0; i < L; ++i) {
+                    const int c = (r * L + i) / 4, j = (r * L + i) % 4;
+                    const uint32_t hash = mix32((b.quad + q[u][c].e / 4u) ^ k.key);
+                    const uint32_t a = xm == 255u ? 0u : m_word(m[i], xm, bits_for_m(hash, j)) >> 24;
+                    const uint32_t d = xv == 255u ? 0u : v_code(v[i], (xv - 31u) << 23, bits_for_v(hash, j));
+                    mc[c] |= live ? a << (8 * j) : q[u][c].mc[0] & (255u << (8 * j));
+                    vc[c] |= live ? d << (8 * j) : q[u][c].vc[0] & (255u << (8 * j));
+                }
+                if (live) x[u][r] = (uint16_t)(xm | xv << 8);
+            } else {
+#pragma unroll
+                for (int i = 0; i < L; ++i) {
+                    const int c = (r * L + i) / 4, j = (r * L + i) % 4;
+                    auto &s = q[u][c];
+                    float m = s.m[0][j] * decay_m, v = s.v[0][j] * decay_v;
+                    const float out = update_one<false>(s.p[0][j], scaled(s.g[0][j], scale), m, v, k);
+                    p[c][0][j] = live ? out : s.p[0][j];
+                    s.m[0][j] = live ? m : s.m[0][j];
+                    s.v[0][j] = live ? v : s.v[0][j];
+                }
             }
-            if (live[r]) x[r] = (uint16_t)(xm | xv << 8);
         }
+        if (MASKED) __builtin_memcpy(stamps + row, last[u], 4 * R);
+        if (STATE8) __builtin_memcpy(b.exponents + 2 * row, x[u], 2 * R);
 #pragma unroll
         for (int c = 0; c < Q; ++c) {
-            q[c].mc[0] = mc[c];
-            q[c].vc[0] = vc[c];
-        }
-        __builtin_memcpy(b.exponents, x, 2 * R);
-    } else {
-#pragma unroll
-        for (int e = 0; e < R * L; ++e) {
-            const int r = e / L, c = e / 4, j = e % 4;
-            float m = q[c].m[0][j] * decay_m[r], v = q[c].v[0][j] * decay_v[r];
-            const float out = update_one<false>(q[c].p[0][j], scaled(q[c].g[0][j], scale), m, v, k);
-            p[c][0][j] = live[r] ? out : q[c].p[0][j];
-            q[c].m[0][j] = live[r] ? m : q[c].m[0][j];
-            q[c].v[0][j] = live[r] ? v : q[c].v[0][j];
+            if (STATE8) {
+                q[u][c].mc[0] = mc[c];
+                q[u][c].vc[0] = vc[c];
+            }
+            q[u][c].store(b, p[c]);
         }
     }
-#pragma unroll
-    for (int c = 0; c < Q; ++c) q[c].store(b, p[c]);
+    // rows behind the last whole quads
+    if (threadIdx.x == 0)
+        for (int r = left / R * R; r < left; ++r) step_unit<1, GS_DTYPE_F32, false, STATE8>(t, k, scale, first + r, L);
 }
 
 // Chunks that a form makes of a tensor (a workgroup each)
-__host__ __device__ inline long long form_chunks(int form, long long numel, int row_len, int per_quads, bool state8) {
+__host__ __device__ inline long long form_chunks(int form, long long numel, int row_len, int quads, bool pair, bool state8) {
     const long long units = row_len > 0 ? numel / row_len : (numel + UNIT - 1) / UNIT;
-    const int group = row_len == 0 || row_len > 16 ? 16 : (row_len > 4 ? 4 : 1);
-    const int per = form == QUADS ? GS_BLOCK / 16 * per_quads : form == QUADS_MASKED ? GS_BLOCK / GS_WAVE * masked_rows(state8) : form == NARROW ? narrow_rows(row_len) * GS_BLOCK : GS_BLOCK / group;
+    const int lanes = form == QUADS || form == QUADS_MASKED ? 16 : lanes_of(row_len);
+    const int per = form == QUADS                                 ? GS_BLOCK / lanes * passes(quads, pair) * (pair ? 2 : 1)
+                    : form == ROWS                                ? GS_BLOCK / lanes * passes(quads, pair)
+                    : form == QUADS_MASKED || form == ROWS_MASKED ? GS_BLOCK / GS_WAVE * masked_rows(lanes, state8)
+                    : form == NARROW                              ? narrow_rows(row_len) * narrow_passes(row_len, state8) * GS_BLOCK
+                                                                  : GS_BLOCK;
     return (units + per - 1) / per;
 }
 
@@ -711,23 +751,34 @@ __global__ __launch_bounds__(GS_BLOCK) void adamw_kernel(AdamwBatch b) {
     if (!b.device_scalars) k.key = t.key;
     const float scale = b.grad_scale ? *b.grad_scale : 1.f;
     const unsigned chunk = blockIdx.x - b.first_chunk[ti];
-    if constexpr (MASKED) {
-        if (t.form == QUADS_MASKED) return step_quads_masked<masked_rows(STATE8) / 4, STATE8>(t, k, scale, chunk);
-    } else {
-        if (t.form == QUADS) return step_quads<pairs(DT, MASTER, STATE8) ? (QUADS_A_LANE + 1) / 2 : QUADS_A_LANE, DT, MASTER, STATE8>(t, k, scale, chunk);
+    constexpr int PASSES = passes(QUADS_A_LANE, pairs(DT, MASTER, STATE8));
+    if constexpr (!MASKED) {
+        if (t.form == QUADS) return step_quads<PASSES, DT, MASTER, STATE8, 0>(t, k, scale, chunk);
     }
-    if constexpr (DT == GS_DTYPE_F32 && (MASKED || STATE8)) {
-        if (t.form == NARROW) {
-            if (t.row_len == 3) return step_narrow<3, STATE8>(t, k, scale, chunk);
-            if (t.row_len == 1) return step_narrow<1, STATE8>(t, k, scale, chunk);
-            if (t.row_len == 2) return step_narrow<2, STATE8>(t, k, scale, chunk);
-            return step_narrow<4, STATE8>(t, k, scale, chunk);
+    if constexpr (MASKED) {
+        if (t.form == QUADS_MASKED) return step_quads_masked<STATE8, 0>(t, k, scale, chunk);
+        if (t.form == ROWS_MASKED) {
+            if (t.row_len > 32) return step_quads_masked<STATE8, 16>(t, k, scale, chunk);
+            if (t.row_len > 16) return step_quads_masked<STATE8, 8>(t, k, scale, chunk);
+            if (t.row_len > 8) return step_quads_masked<STATE8, 4>(t, k, scale, chunk);
+            return step_quads_masked<STATE8, 2>(t, k, scale, chunk);
+        }
+    } else if constexpr (STATE8) {
+        if (t.form == ROWS) {
+            if (t.row_len > 32) return step_quads<PASSES, DT, MASTER, true, 16>(t, k, scale, chunk);
+            if (t.row_len > 16) return step_quads<PASSES, DT, MASTER, true, 8>(t, k, scale, chunk);
+            if (t.row_len > 8) return step_quads<PASSES, DT, MASTER, true, 4>(t, k, scale, chunk);
+            return step_quads<PASSES, DT, MASTER, true, 2>(t, k, scale, chunk);
         }
     }
-    const int row_len = t.row_len > 0 ? t.row_len : UNIT;
-    if (row_len > 16) step_unit<16, DT, MASTER, STATE8>(t, k, scale, (long long)chunk * (GS_BLOCK / 16) + threadIdx.x / 16, row_len);
-    else if (row_len > 4) step_unit<4, DT, MASTER, STATE8>(t, k, scale, (long long)chunk * (GS_BLOCK / 4) + threadIdx.x / 4, row_len);
-    else step_unit<1, DT, MASTER, STATE8>(t, k, scale, (long long)chunk * GS_BLOCK + threadIdx.x, row_len);
+    if constexpr (DT == GS_DTYPE_F32 && (MASKED || STATE8)) {
+        if (t.row_len == 3) return step_narrow<3, STATE8, MASKED>(t, k, scale, chunk);
+        if (t.row_len == 1) return step_narrow<1, STATE8, MASKED>(t, k, scale, chunk);
+        if (t.row_len == 2) return step_narrow<2, STATE8, MASKED>(t, k, scale, chunk);
+        return step_narrow<4, STATE8, MASKED>(t, k, scale, chunk);
+    } else if constexpr (STATE8) {
+        step_unit<1, DT, MASTER, true>(t, k, scale, (long long)chunk * GS_BLOCK + threadIdx.x, t.row_len);
+    }
 }
 
 // Scalars of tensors whose step count or learning rate lives on the device.  1 - beta^t is taken as -expm1(t log beta) in
@@ -770,7 +821,7 @@ struct MomentsTensor {
     const uint8_t *m, *v, *exponents;
     void *m_out, *v_out;
     long long numel;
-    int row_len, form;
+    int row_len;
 };
 struct MomentsBatch {
     int n_tensors;
@@ -804,9 +855,10 @@ __device__ __forceinline__ void read_four(uint32_t mc, uint32_t vc, uint32_t x, 
     stream_store((char *)v_out + i * (long long)(sizeof(Value) / 4), __builtin_convertvector(v, Value));
 }
 
-template <int UNROLL, int DT>
+// Units of 64 or rows from five elements on, GROUP lanes each, as in the step
+template <int UNROLL, int DT, int GROUP>
 __device__ __forceinline__ void read_quads(const MomentsTensor &t, unsigned chunk) {
-    constexpr int GROUP = 16, PER_PASS = GS_BLOCK / GROUP, SHARE = PER_PASS * UNROLL, BYTES = DT == GS_DTYPE_F32 ? 4 : 2;
+    constexpr int PER_PASS = GS_BLOCK / GROUP, SHARE = PER_PASS * UNROLL, BYTES = DT == GS_DTYPE_F32 ? 4 : 2;
     const uint32_t unit_len = t.row_len > 0 ? t.row_len : UNIT;
     const long long chunk_unit = (long long)chunk * SHARE, whole = t.numel / unit_len;
     const uint32_t units = (uint32_t)min((long long)SHARE, max(0LL, whole - chunk_unit)), sub = threadIdx.x % GROUP;
@@ -826,7 +878,7 @@ __device__ __forceinline__ void read_quads(const MomentsTensor &t, unsigned chun
         for (int u = 0; u < UNROLL; ++u)
             if (threadIdx.x / GROUP + u * PER_PASS < units && 4u * sub < unit_len) read_four<DT>(mc[u], vc[u], x[u], m_out, v_out, e[u]);
     }
-    if (whole * unit_len < t.numel && whole >= chunk_unit && whole < chunk_unit + SHARE && threadIdx.x < GROUP)
+    if (GROUP == 16 && whole * unit_len < t.numel && whole >= chunk_unit && whole < chunk_unit + SHARE && threadIdx.x < GROUP)
         read_unit<GROUP, DT>(t, whole, (int)unit_len);
 }
 
@@ -861,17 +913,17 @@ __global__ __launch_bounds__(GS_BLOCK) void read_moments_kernel(MomentsBatch b) 
     const int ti = find_tensor<MAX_TENSORS>(b.first_chunk, b.n_tensors, blockIdx.x);
     const MomentsTensor &t = b.t[ti];
     const unsigned chunk = blockIdx.x - b.first_chunk[ti];
-    if (t.form == QUADS) return read_quads<UNROLL, DT>(t, chunk);
-    if (t.form == NARROW) {
-        if (t.row_len == 3) return read_narrow<3, DT>(t, chunk);
-        if (t.row_len == 1) return read_narrow<1, DT>(t, chunk);
-        if (t.row_len == 2) return read_narrow<2, DT>(t, chunk);
-        return read_narrow<4, DT>(t, chunk);
+    const int lanes = lanes_of(t.row_len);
+    if (t.row_len == 0 || t.row_len > 4) {
+        if (lanes == 16) return read_quads<UNROLL, DT, 16>(t, chunk);
+        if (lanes == 8) return read_quads<UNROLL, DT, 8>(t, chunk);
+        if (lanes == 4) return read_quads<UNROLL, DT, 4>(t, chunk);
+        return read_quads<UNROLL, DT, 2>(t, chunk);
     }
-    const int row_len = t.row_len > 0 ? t.row_len : UNIT;
-    if (row_len > 16) read_unit<16, DT>(t, (long long)chunk * (GS_BLOCK / 16) + threadIdx.x / 16, row_len);
-    else if (row_len > 4) read_unit<4, DT>(t, (long long)chunk * (GS_BLOCK / 4) + threadIdx.x / 4, row_len);
-    else read_unit<1, DT>(t, (long long)chunk * GS_BLOCK + threadIdx.x, row_len);
+    if (t.row_len == 3) return read_narrow<3, DT>(t, chunk);
+    if (t.row_len == 1) return read_narrow<1, DT>(t, chunk);
+    if (t.row_len == 2) return read_narrow<2, DT>(t, chunk);
+    return read_narrow<4, DT>(t, chunk);
 }
 
 // ------------------------------------------------------------------ norm of gradients
@@ -961,46 +1013,49 @@ __device__ __forceinline__ double flat_squares(const void *grad, long long begin
     return s;
 }
 
-// Rows begin..end of a tensor with a row mask, element by element, GROUP lanes a row
-template <int GROUP, int DT>
+// Rows begin..end of a tensor with a row mask, of up to four elements: a row a lane
+template <int DT>
 __device__ __forceinline__ double row_squares(const NormMaskedTensor &t, long long begin, long long end) {
-    const int sub = threadIdx.x % GROUP, len = t.row_len;
     double s = 0.0;
-    for (long long row = begin + threadIdx.x / GROUP; row < end; row += GS_BLOCK / GROUP) {
+    for (long long row = begin + threadIdx.x; row < end; row += GS_BLOCK) {
         if (t.row_mask[row] != 0) continue;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (sub + j * GROUP < len) {
-                const double y = (double)load_one<DT>(t.grad, row * len + sub + j * GROUP);
-                s = fma(y, y, s);
-            }
+        for (int j = 0; j < t.row_len; ++j) {
+            const double y = (double)load_one<DT>(t.grad, row * t.row_len + j);
+            s = fma(y, y, s);
+        }
     }
     return s;
 }
 
-// The same for rows of 20, 24 .. 64 elements: a wave packs the live ones of 64 rows and reads them four at a
-// time, AHEAD of them in flight.
-template <int DT>
+// The same for longer rows, GROUP lanes each: a wave packs the live ones of 64 rows and has AHEAD quads a lane in flight.  The last
+// lane of a row whose length is no multiple of four leaves out what its neighbour has.
+template <int DT, int GROUP>
 __device__ __forceinline__ double packed_row_squares(const NormMaskedTensor &t, long long begin, long long end) {
-    constexpr int GROUP = 16, AHEAD = 4, BYTES = DT == GS_DTYPE_F32 ? 4 : 2;
-    const int len = t.row_len, lane = gs_lane(), sub = lane % GROUP;
+    constexpr int AHEAD = 4, PER_PASS = GS_WAVE / GROUP, BYTES = DT == GS_DTYPE_F32 ? 4 : 2;
+    const int len = t.row_len, lane = gs_lane(), sub = lane % GROUP, from = min(4 * sub, len - 4), skip = 4 * sub - from;
     double s = 0.0;
     for (long long row0 = begin + threadIdx.x / GS_WAVE * GS_WAVE; row0 < end; row0 += GS_BLOCK) {
         const bool live = row0 + lane < end && t.row_mask[row0 + lane < end ? row0 + lane : row0] == 0;
         const u64 lives = __ballot(live), below = (1ull << lane) - 1ull;
         const int n_live = __popcll(lives);
         const int order = __builtin_amdgcn_ds_permute(4 * (live ? __popcll(lives & below) : 63 - __popcll(~lives & below)), lane);
-        for (int at = 0; at < n_live; at += 4 * AHEAD) {
+        for (int at = 0; at < n_live; at += PER_PASS * AHEAD) {
             typename Four<DT>::type x[AHEAD];
 #pragma unroll
             for (int a = 0; a < AHEAD; ++a) {
-                const int i = at + 4 * a + lane / GROUP;
+                const int i = at + PER_PASS * a + lane / GROUP;
                 const long long row = row0 + __shfl(order, i < n_live ? i : 0, GS_WAVE);
                 x[a] = {};
-                if (i < n_live && 4 * sub < len) x[a] = load_at<typename Four<DT>::type>((const char *)t.grad + (row * len + 4 * sub) * BYTES);
+                if (i < n_live && skip < 4) x[a] = load_at<typename Four<DT>::type>((const char *)t.grad + (row * len + from) * BYTES);
             }
 #pragma unroll
-            for (int a = 0; a < AHEAD; ++a) s = add_squares<4>(s, x[a]);
+            for (int a = 0; a < AHEAD; ++a) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const double y = j >= skip ? (double)(float)x[a][j] : 0.0;
+                    s = fma(y, y, s);
+                }
+            }
         }
     }
     return s;
@@ -1033,15 +1088,17 @@ template <int DT>
 __device__ __forceinline__ double masked_squares(const NormMaskedTensor &t, unsigned part, unsigned chunk) {
     const long long rows = t.numel / t.row_len, per = norm_rows(chunk, t.row_len);
     const long long begin = part * per, end = min(rows, begin + per);
-    if (t.row_len > 16) return t.row_len % 4 == 0 ? packed_row_squares<DT>(t, begin, end) : row_squares<16, DT>(t, begin, end);
-    if (t.row_len > 4) return row_squares<4, DT>(t, begin, end);
+    if (t.row_len > 32) return packed_row_squares<DT, 16>(t, begin, end);
+    if (t.row_len > 16) return packed_row_squares<DT, 8>(t, begin, end);
+    if (t.row_len > 8) return packed_row_squares<DT, 4>(t, begin, end);
+    if (t.row_len > 4) return packed_row_squares<DT, 2>(t, begin, end);
     if constexpr (DT == GS_DTYPE_F32) {
         if (t.row_len == 3) return narrow_squares<3>(t, begin, end);
         if (t.row_len == 1) return narrow_squares<1>(t, begin, end);
         if (t.row_len == 2) return narrow_squares<2>(t, begin, end);
         return narrow_squares<4>(t, begin, end);
     }
-    return row_squares<1, DT>(t, begin, end);
+    return row_squares<DT>(t, begin, end);
 }
 
 // A workgroup's sum goes behind those of the launches before (`base` of them); spans[i] = {first, number} of tensor i's.
@@ -1142,6 +1199,17 @@ constexpr int UNROLL = 4, UNROLL_READ = 4;
 constexpr int OCCUPANCY_LDS = 40960;
 constexpr long long SMALL_CHUNKS = 2048;    // of 16 units
 
+int form_of(int dtype, int row, bool masked, bool pair) {
+    if (row >= 1 && row <= 4) return dtype == GS_DTYPE_F32 ? NARROW : ELEMENTS;
+    if (row == 0 || (row > 32 && row % (pair ? 8 : 4) == 0)) return masked ? QUADS_MASKED : QUADS;
+    return masked ? ROWS_MASKED : ROWS;
+}
+long long read_chunks(long long numel, int row, int unroll) {
+    const long long units = row > 0 ? numel / row : (numel + UNIT - 1) / UNIT;
+    const int per = row >= 1 && row <= 4 ? narrow_rows(row) * GS_BLOCK : GS_BLOCK / lanes_of(row) * unroll;
+    return (units + per - 1) / per;
+}
+
 template <int U, bool STATE8>
 void launch_step(int dtype, bool master, bool masked, const AdamwBatch &b, hipStream_t s) {
     const dim3 grid(b.first_chunk[b.n_tensors]), block(GS_BLOCK);
@@ -1204,7 +1272,9 @@ extern "C" int gs_adamw_step(int n_tensors, const uint64_t *host_param, const ui
         GS_REQUIRE(n >= 0 && n < (1LL << 46) && row >= 0 && row <= UNIT && (row == 0 || n % row == 0),
                    "gs_adamw_step: numel in [0, 2^46), too large else, rows of 1..64 elements");
         GS_REQUIRE(dt == GS_DTYPE_F32 || dt == GS_DTYPE_BF16 || dt == GS_DTYPE_F16, "gs_adamw_step: unknown dtype");
-        GS_REQUIRE(form_chunks(ELEMENTS, n, row, 1, false) < 0x7fffffffLL, "gs_adamw_step: tensor too large");
+        const bool masked = entry(host_row_mask, i) != 0;
+        const int rows = masked || state8 ? row : 0;
+        GS_REQUIRE(form_chunks(form_of(dt, rows, masked, false), n, rows, 1, false, state8) < 0x7fffffffLL, "gs_adamw_step: tensor too large");
         GS_REQUIRE(n == 0 || (host_param[i] && host_grad[i] && host_exp_avg[i] && host_exp_avg_sq[i] && (!state8 || host_exponents[i])),
                    "gs_adamw_step: null tensor");
         GS_REQUIRE(!entry(host_row_mask, i) || (row > 0 && dt == GS_DTYPE_F32 && host_last_step[i]), "gs_adamw_step: a row mask needs float rows and last steps");
@@ -1214,7 +1284,7 @@ extern "C" int gs_adamw_step(int n_tensors, const uint64_t *host_param, const ui
         GS_REQUIRE(aligned_to(host_param[i] | host_grad[i], element_bytes(dt)) && aligned_to(state8 ? 0 : host_exp_avg[i] | host_exp_avg_sq[i], 4) &&
                        aligned_to(entry(host_master, i) | (entry(host_row_mask, i) ? host_last_step[i] : 0), 4),
                    "gs_adamw_step: an address is no multiple of its type's size");
-        units_of_16 += form_chunks(QUADS, n, row, 1, false);
+        units_of_16 += form_chunks(QUADS, n, row, 1, false, false);
     }
     {
         Range *r = (Range *)malloc((size_t)n_tensors * 8 * sizeof(Range));
@@ -1256,14 +1326,12 @@ extern "C" int gs_adamw_step(int n_tensors, const uint64_t *host_param, const ui
             long long chunks = 0;
             int set = 0;
             if (!end) {
-                const u64 mask = entry(host_row_mask, i);
-                const int row = mask || state8 ? host_row_len[i] : 0;      // (moments in 32 bits without a mask: units of 64 whatever the shape)
+                const int row = masked || state8 ? host_row_len[i] : 0;      // (moments in 32 bits without a mask: units of 64 whatever the shape)
                 const bool pair = pairs(dtype, master, state8);
-                const bool quads = row == 0 || (row > 16 && row % (pair ? 8 : 4) == 0), narrow = dtype == GS_DTYPE_F32 && row >= 1 && row <= 4;
-                t.form = narrow ? NARROW : quads ? (mask ? QUADS_MASKED : QUADS) : ELEMENTS;
+                t.form = form_of(dtype, row, masked, pair);
                 t.row_len = (uint8_t)row;
-                t.masked = mask != 0;
-                chunks = form_chunks(t.form, host_numel[i], row, pair ? std::max(2, unroll) : unroll, state8);
+                t.masked = masked;
+                chunks = form_chunks(t.form, host_numel[i], row, unroll, pair, state8);
                 while (!on_device && set < q.n_sets &&
                        (q.step[set] != host_step[i] || memcmp(q.hyper[set], host_hyper + 5 * (size_t)i, 5 * sizeof(double)) != 0)) ++set;
             }
@@ -1327,11 +1395,11 @@ extern "C" int gs_read_moments(int n_tensors, const uint64_t *host_exp_avg, cons
         const int row = host_row_len[i];
         GS_REQUIRE(n >= 0 && n < (1LL << 46) && row >= 0 && row <= UNIT && (row == 0 || n % row == 0),
                    "gs_read_moments: numel in [0, 2^46), rows of 1..64 elements");
-        GS_REQUIRE(form_chunks(ELEMENTS, n, row, 1, false) < 0x7fffffffLL, "gs_read_moments: tensor too large");
+        GS_REQUIRE(read_chunks(n, row, 1) < 0x7fffffffLL, "gs_read_moments: tensor too large");
         GS_REQUIRE(n == 0 || (host_exp_avg[i] && host_exp_avg_sq[i] && host_exponents[i] && host_m_out[i] && host_v_out[i]),
                    "gs_read_moments: null tensor");
         GS_REQUIRE(aligned_to(host_m_out[i] | host_v_out[i], element_bytes(out_dtype)), "gs_read_moments: misaligned output");
-        units_of_16 += form_chunks(QUADS, n, row, 1, false);
+        units_of_16 += form_chunks(QUADS, n, row, 1, false, false);
     }
     {
         Range *r = (Range *)malloc((size_t)n_tensors * 5 * sizeof(Range));
@@ -1361,9 +1429,8 @@ extern "C" int gs_read_moments(int n_tensors, const uint64_t *host_exp_avg, cons
         if (!end) {
             const int row = host_row_len[i];
             t = {(const uint8_t *)host_exp_avg[i], (const uint8_t *)host_exp_avg_sq[i], (const uint8_t *)host_exponents[i],
-                 (void *)host_m_out[i], (void *)host_v_out[i], host_numel[i], row, 0};
-            t.form = row >= 1 && row <= 4 ? NARROW : row == 0 || (row > 16 && row % 4 == 0) ? QUADS : ELEMENTS;
-            chunks = form_chunks(t.form, host_numel[i], row, unroll, true);
+                 (void *)host_m_out[i], (void *)host_v_out[i], host_numel[i], row};
+            chunks = read_chunks(host_numel[i], row, unroll);
         }
         if (b.n_tensors > 0 && (end || b.n_tensors == MAX_TENSORS || (long long)b.first_chunk[b.n_tensors] + chunks >= 0x7fffffffLL)) {
             if (unroll == 1) launch_moments<1>(out_dtype, b, (hipStream_t)stream);

@@ -108,7 +108,7 @@ TYPES = [(torch.float32, False), (torch.bfloat16, False), (torch.bfloat16, True)
 @pytest.mark.parametrize("dtype,with_master", TYPES)
 @pytest.mark.parametrize("offset", [0, 1])
 def test_step_of_many_shapes_against_64_bits(bits, dtype, with_master, offset):
-    """All shapes in one call; at an offset of one element nothing is aligned and every tensor takes the element-wise form."""
+    """All shapes in one call; at an offset of one element nothing is aligned."""
     o = _optim()
     tensors = [_inputs(s, dtype, bits, 100 + i, offset) for i, s in enumerate(SHAPES)]
     masters = None
@@ -817,3 +817,44 @@ def test_steps_from_two_threads_equal_steps_from_one():
         t.join(60)
     for seed in (1, 2):
         assert all(torch.equal(a, b) for a, b in zip(alone[seed], together[seed])), seed
+
+
+@pytest.mark.parametrize("dtype,with_master", TYPES)
+@pytest.mark.parametrize("rows,offset", [(97, 1), (601, 0)])
+def test_rows_of_every_length_with_8_bits(dtype, with_master, rows, offset):
+    """Blocks of 1 to 64 elements, few of them (a quad a lane) and many; their moments read out."""
+    o = _optim()
+    tensors = [_inputs((rows + n % 3, n), dtype, 8, n, offset) for n in range(1, 65)]
+    masters = [_place(t[0].float() * (1 + 2e-3), offset) for t in tensors] if with_master else None
+    before = [((_np(masters[i]) if masters else _np(t[0])), *(_np(x) for x in t[1:])) for i, t in enumerate(tensors)]
+    for out_dtype in (torch.float32, torch.bfloat16):
+        for t, m, v in zip(tensors, *o.read_moments(*([t[k] for t in tensors] for k in (2, 3, 4)), dtype=out_dtype)):
+            true_m, true_v = plain.decode(_np(t[2]), _np(t[3]), _np(t[4]), tuple(t[0].shape))
+            normal = np.abs(true_m) >= 2.0 ** -126, true_v >= 2.0 ** -126
+            assert np.array_equal(_np(m)[normal[0]], true_m[normal[0]]) and np.array_equal(_np(v)[normal[1]], true_v[normal[1]])
+            assert (np.abs(_np(m)[~normal[0]]) <= 2.0 ** -125).all() and (_np(v)[~normal[1]] <= 2.0 ** -125).all()
+    o.adamw_step_(*[[t[k] for t in tensors] for k in range(4)], step=17, exponents=[t[4] for t in tensors], masters=masters, seed=5, **HYPER)
+    for i, t in enumerate(tensors):
+        _check_step(before[i], (t[0], t[2], t[3], t[4]), dtype, 17, 8, seed=5, tensor=i, master=masters[i] if masters else None)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("columns", [2, 5, 8, 12, 15, 20, 24, 31, 32, 33, 36, 45, 60, 63])
+def test_row_masks_of_more_lengths(bits, columns):
+    test_row_masks_leave_rows_alone_and_late_rows_decay(bits, columns, 0.4)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("offset", [0, 1])
+def test_norms_of_masked_rows_of_every_length(dtype, offset):
+    o = _optim()
+    gen = torch.Generator().manual_seed(offset)
+    grads = [_place((torch.randn(211 + n, n, generator=gen)).to(dtype), offset) for n in range(1, 65)]
+    masks = [(torch.rand(len(g), generator=gen) < 0.3).to(torch.int8).to(DEV) for g in grads]
+    true = np.array([np.sqrt((_np(g) ** 2)[_np(mask) == 0].sum()) for g, mask in zip(grads, masks)])
+    for g, mask in zip(grads, masks):
+        g[mask != 0] = float("nan")
+    norm, each = o.grad_norm(grads, masks, per_tensor=True)
+    _assert_near(_np(each), true, true * 2.0 ** -24 * 1.001, "each")
+    total = np.sqrt((true ** 2).sum())
+    assert abs(float(norm) - total) <= total * 2.0 ** -24 * 1.001
