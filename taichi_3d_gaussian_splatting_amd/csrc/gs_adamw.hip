@@ -51,8 +51,7 @@ enum Form : int {
     ROWS,           // other rows from five elements on: 2, 4, 8 or 16 lanes a row
     QUADS_MASKED,   // the rows of QUADS under a mask: a wave packs the live ones
     ROWS_MASKED,    // the rows of ROWS under a mask, the same way
-    NARROW,         // float rows of 1 to 4 elements: whole quads of rows a lane
-    ELEMENTS        // 16-bit rows of 1 to 4 elements: a row a lane, element by element
+    NARROW          // rows of 1 to 4 elements: whole quads of rows a lane
 };
 // Passes of a lane over its workgroup's units, of a quad each, or of a pair where QUADS has pairs (ROWS has none)
 constexpr int passes(int quads, bool pair) { return pair ? (quads + 1) / 2 : quads; }
@@ -459,8 +458,8 @@ struct Share {
     }
 };
 
-// The element-wise form, for what the others leave: the last unit of a flat tensor (GROUP 16), narrow rows behind the last whole
-// quads and 16-bit rows of 1 to 4 elements (GROUP 1).  GROUP lanes take a unit, elements GROUP apart.
+// The element-wise form, for what the others leave: the last unit of a flat tensor (GROUP 16) and narrow rows behind the last
+// whole quads (GROUP 1).  GROUP lanes take a unit, elements GROUP apart.
 template <int GROUP, int DT, bool MASTER, bool STATE8>
 __device__ __forceinline__ void step_unit(const AdamwTensor &t, const AdamwScalars &k, float scale, long long unit, int unit_len) {
     const int sub = threadIdx.x % GROUP;
@@ -616,25 +615,27 @@ __device__ __forceinline__ void step_quads_masked(const AdamwTensor &t, const Ad
     }
 }
 
-// Float rows of L = 1..4 elements, as many rows a lane as make whole quads (rows of three: four rows, three quads): every access
-// is 16 bytes (4 for codes) although a row is not.  Of rows under a mask the lane writes back what it read.  With codes of one
+// Rows of L = 1..4 elements, as many rows a lane as make whole quads (rows of three: four rows, three quads): every access
+// is four elements although a row is not.  Of rows under a mask the lane writes back what it read.  With codes of one
 // quad only a lane has too little in flight: it takes rows at two places (40M floats, rows of 1 / 2 / 4: 157 / 143 / 136 us at
 // one, 145 / 134 / 127 at two, 152 / 140 / 132 at four; all live under a mask 268 / 237 / 235, 210 / 179 / 164, 217 / 181 / 155).
+// 40M bfloat16 in rows of 1 / 2 / 3 / 4: 102 / 90 / 92 / 79 us, a row a lane and element by element 304 / 188 / 152 / 148.
 __host__ __device__ constexpr int narrow_rows(int row_len) { return row_len == 4 ? 1 : (row_len == 2 ? 2 : 4); }
 __host__ __device__ constexpr int narrow_passes(int row_len, bool state8) { return state8 && row_len != 3 ? 2 : 1; }
 
-template <int L, bool STATE8, bool MASKED>
+template <int L, int DT, bool MASTER, bool STATE8, bool MASKED>
 __device__ __forceinline__ void step_narrow(const AdamwTensor &t, const AdamwScalars &k, float scale, unsigned chunk) {
     constexpr int R = narrow_rows(L), Q = R * L / 4, PASSES = narrow_passes(L, STATE8), SHARE = R * PASSES * GS_BLOCK;
     const long long rows = t.numel / L, first = (long long)chunk * SHARE;
     const int left = (int)min((long long)SHARE, rows - first);
-    const Buffers<GS_DTYPE_F32, false, STATE8> b(t, first * L, first);
+    const Buffers<DT, MASTER, STATE8> b(t, first * L, first);
     const int8_t *mask_of = (const int8_t *)t.master_or_mask + (MASKED ? first : 0);
     int32_t *stamps = t.last_step + (MASKED ? first : 0);
     int8_t mask[PASSES][R];
     int last[PASSES][R];
     bool go[PASSES];
-    Share<GS_DTYPE_F32, false, STATE8, 0, false> q[PASSES][Q];      // (cached: several accesses of the lane touch a line; 202 us, else 232)
+    // (single quads; cached: several accesses of the lane touch a line; 202 us, else 232)
+    Share<DT, MASTER, STATE8, 2, false> q[PASSES][Q];
     uint16_t x[PASSES][R];
 #pragma unroll
     for (int u = 0; u < PASSES; ++u) {
@@ -684,8 +685,9 @@ __device__ __forceinline__ void step_narrow(const AdamwTensor &t, const AdamwSca
                 for (int i = 0; i < L; ++i) {
                     const int c = (r * L + i) / 4, j = (r * L + i) % 4;
                     const auto &s = q[u][c];
-                    const float out = update_coded<false, MASKED>(s.p[0][j], scaled(s.g[0][j], scale), unit_at(s.mc[0], j), (s.vc[0] >> (8 * j)) & 255u, o, m[i], v[i], k);
-                    p[c][0][j] = live ? out : s.p[0][j];
+                    const float old = (float)s.p[0][j];
+                    const float out = update_coded<MASTER, MASKED>(old, scaled((float)s.g[0][j], scale), unit_at(s.mc[0], j), (s.vc[0] >> (8 * j)) & 255u, o, m[i], v[i], k);
+                    p[c][0][j] = live ? out : old;
                     top_m = max(top_m, to_bits(m[i]) & 0x7FFFFFFFu);
                     top_v = max(top_v, to_bits(v[i]) & 0x7FFFFFFFu);
                 }
@@ -726,7 +728,7 @@ __device__ __forceinline__ void step_narrow(const AdamwTensor &t, const AdamwSca
     }
     // rows behind the last whole quads
     if (threadIdx.x == 0)
-        for (int r = left / R * R; r < left; ++r) step_unit<1, GS_DTYPE_F32, false, STATE8>(t, k, scale, first + r, L);
+        for (int r = left / R * R; r < left; ++r) step_unit<1, DT, MASTER, STATE8>(t, k, scale, first + r, L);
 }
 
 // Chunks that a form makes of a tensor (a workgroup each)
@@ -736,15 +738,16 @@ __host__ __device__ inline long long form_chunks(int form, long long numel, int 
     const int per = form == QUADS                                 ? GS_BLOCK / lanes * passes(quads, pair) * (pair ? 2 : 1)
                     : form == ROWS                                ? GS_BLOCK / lanes * passes(quads, pair)
                     : form == QUADS_MASKED || form == ROWS_MASKED ? GS_BLOCK / GS_WAVE * masked_rows(lanes, state8)
-                    : form == NARROW                              ? narrow_rows(row_len) * narrow_passes(row_len, state8) * GS_BLOCK
-                                                                  : GS_BLOCK;
+                                                                  : narrow_rows(row_len) * narrow_passes(row_len, state8) * GS_BLOCK;
     return (units + per - 1) / per;
 }
 
 // All tensors of one parameter type and one form of moments, whatever their shapes: the branches on `form` are uniform in a
-// workgroup.  Masked tensors have a kernel of their own, whose registers would cost the others occupancy.
+// workgroup.  Masked tensors have a kernel of their own, whose registers would cost the others occupancy.  Where pairs of quads
+// are bound by arithmetic, narrow rows of three would take 83 registers: at least six waves to a SIMD (40M bfloat16, rows of
+// 3 / 4 / 7 / 16 / 56: 92 / 79 / 103 / 83 / 71 us; five waves 81 / 84 / 110 / 91 / 74, seven 142 / 75 / 97 / 80 / 70).
 template <int QUADS_A_LANE, int DT, bool MASTER, bool STATE8, bool MASKED>
-__global__ __launch_bounds__(GS_BLOCK) void adamw_kernel(AdamwBatch b) {
+__global__ __launch_bounds__(GS_BLOCK, pairs(DT, MASTER, STATE8) ? 6 : 1) void adamw_kernel(AdamwBatch b) {
     const int ti = find_tensor<MAX_TENSORS>(b.first_chunk, b.n_tensors, blockIdx.x);
     const AdamwTensor &t = b.t[ti];
     AdamwScalars k = b.device_scalars ? b.device_scalars[ti] : b.scalars[t.set];
@@ -771,13 +774,11 @@ __global__ __launch_bounds__(GS_BLOCK) void adamw_kernel(AdamwBatch b) {
             return step_quads<PASSES, DT, MASTER, true, 2>(t, k, scale, chunk);
         }
     }
-    if constexpr (DT == GS_DTYPE_F32 && (MASKED || STATE8)) {
-        if (t.row_len == 3) return step_narrow<3, STATE8, MASKED>(t, k, scale, chunk);
-        if (t.row_len == 1) return step_narrow<1, STATE8, MASKED>(t, k, scale, chunk);
-        if (t.row_len == 2) return step_narrow<2, STATE8, MASKED>(t, k, scale, chunk);
-        return step_narrow<4, STATE8, MASKED>(t, k, scale, chunk);
-    } else if constexpr (STATE8) {
-        step_unit<1, DT, MASTER, true>(t, k, scale, (long long)chunk * GS_BLOCK + threadIdx.x, t.row_len);
+    if constexpr (MASKED || STATE8) {
+        if (t.row_len == 3) return step_narrow<3, DT, MASTER, STATE8, MASKED>(t, k, scale, chunk);
+        if (t.row_len == 1) return step_narrow<1, DT, MASTER, STATE8, MASKED>(t, k, scale, chunk);
+        if (t.row_len == 2) return step_narrow<2, DT, MASTER, STATE8, MASKED>(t, k, scale, chunk);
+        return step_narrow<4, DT, MASTER, STATE8, MASKED>(t, k, scale, chunk);
     }
 }
 
@@ -1199,8 +1200,8 @@ constexpr int UNROLL = 4, UNROLL_READ = 4;
 constexpr int OCCUPANCY_LDS = 40960;
 constexpr long long SMALL_CHUNKS = 2048;    // of 16 units
 
-int form_of(int dtype, int row, bool masked, bool pair) {
-    if (row >= 1 && row <= 4) return dtype == GS_DTYPE_F32 ? NARROW : ELEMENTS;
+int form_of(int row, bool masked, bool pair) {
+    if (row >= 1 && row <= 4) return NARROW;
     if (row == 0 || (row > 32 && row % (pair ? 8 : 4) == 0)) return masked ? QUADS_MASKED : QUADS;
     return masked ? ROWS_MASKED : ROWS;
 }
@@ -1274,7 +1275,7 @@ extern "C" int gs_adamw_step(int n_tensors, const uint64_t *host_param, const ui
         GS_REQUIRE(dt == GS_DTYPE_F32 || dt == GS_DTYPE_BF16 || dt == GS_DTYPE_F16, "gs_adamw_step: unknown dtype");
         const bool masked = entry(host_row_mask, i) != 0;
         const int rows = masked || state8 ? row : 0;
-        GS_REQUIRE(form_chunks(form_of(dt, rows, masked, false), n, rows, 1, false, state8) < 0x7fffffffLL, "gs_adamw_step: tensor too large");
+        GS_REQUIRE(form_chunks(form_of(rows, masked, false), n, rows, 1, false, state8) < 0x7fffffffLL, "gs_adamw_step: tensor too large");
         GS_REQUIRE(n == 0 || (host_param[i] && host_grad[i] && host_exp_avg[i] && host_exp_avg_sq[i] && (!state8 || host_exponents[i])),
                    "gs_adamw_step: null tensor");
         GS_REQUIRE(!entry(host_row_mask, i) || (row > 0 && dt == GS_DTYPE_F32 && host_last_step[i]), "gs_adamw_step: a row mask needs float rows and last steps");
@@ -1328,7 +1329,7 @@ extern "C" int gs_adamw_step(int n_tensors, const uint64_t *host_param, const ui
             if (!end) {
                 const int row = masked || state8 ? host_row_len[i] : 0;      // (moments in 32 bits without a mask: units of 64 whatever the shape)
                 const bool pair = pairs(dtype, master, state8);
-                t.form = form_of(dtype, row, masked, pair);
+                t.form = form_of(row, masked, pair);
                 t.row_len = (uint8_t)row;
                 t.masked = masked;
                 chunks = form_chunks(t.form, host_numel[i], row, unroll, pair, state8);
