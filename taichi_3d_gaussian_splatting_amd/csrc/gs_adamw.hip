@@ -14,6 +14,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -137,12 +138,6 @@ template <int DT> struct Wide;
 template <> struct Wide<GS_DTYPE_F32> { typedef f32x4 type; };
 template <> struct Wide<GS_DTYPE_BF16> { typedef bf16x8 type; };
 template <> struct Wide<GS_DTYPE_F16> { typedef f16x8 type; };
-
-template <int DT>
-__device__ __forceinline__ void store_four(void *p, long long i, f32x4 x) {
-    typedef typename Four<DT>::type V;
-    store_at((char *)p + i * (long long)(sizeof(V) / 4), __builtin_convertvector(x, V));
-}
 
 // ------------------------------------------------------------------ 8-bit moments
 __device__ __forceinline__ float from_bits(uint32_t u) { return __builtin_bit_cast(float, u); }
@@ -845,69 +840,101 @@ __device__ __forceinline__ void read_unit(const MomentsTensor &t, long long unit
     }
 }
 
-template <int DT>
-__device__ __forceinline__ void read_four(uint32_t mc, uint32_t vc, uint32_t x, void *m_out, void *v_out, long long i) {
-    f32x4 v;
+// (whole cache lines, not read again soon: 240 -> 227 us for a step of 1M points and this, the codes from the caches)
+template <int DT, int Q, typename Codes>
+__device__ __forceinline__ void read_codes(Codes mc, Codes vc, uint32_t x, char *m_out, char *v_out) {
+    typedef float Floats __attribute__((ext_vector_type(4 * Q)));
+    typedef typename std::conditional<DT == GS_DTYPE_F32, float, __bf16>::type Element;
+    typedef Element Value __attribute__((ext_vector_type(4 * Q)));
+    Floats m, v;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = v_value((vc >> (8 * j)) & 255u, x);
-    // (whole cache lines, not read again soon: 240 -> 227 us for a step of 1M points and this, the codes from the caches)
-    typedef typename Four<DT>::type Value;
-    stream_store((char *)m_out + i * (long long)(sizeof(Value) / 4), __builtin_convertvector(units_of(mc) * m_scale(x), Value));
-    stream_store((char *)v_out + i * (long long)(sizeof(Value) / 4), __builtin_convertvector(v, Value));
+    for (int c = 0; c < Q; ++c) {
+        const f32x4 units = units_of(mc[c]) * m_scale(x);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            m[4 * c + j] = units[j];
+            v[4 * c + j] = v_value((vc[c] >> (8 * j)) & 255u, x);
+        }
+    }
+    stream_store(m_out, __builtin_convertvector(m, Value));
+    stream_store(v_out, __builtin_convertvector(v, Value));
 }
 
-// Units of 64 or rows from five elements on, GROUP lanes each, as in the step
-template <int UNROLL, int DT, int GROUP>
+// Units of 64 or rows from five elements on, GROUP lanes each, as in the step; PAIR: two quads a lane
+template <int UNROLL, int DT, int GROUP, bool PAIR>
 __device__ __forceinline__ void read_quads(const MomentsTensor &t, unsigned chunk) {
-    constexpr int PER_PASS = GS_BLOCK / GROUP, SHARE = PER_PASS * UNROLL, BYTES = DT == GS_DTYPE_F32 ? 4 : 2;
+    constexpr int PER_PASS = GS_BLOCK / GROUP, SHARE = PER_PASS * UNROLL, BYTES = DT == GS_DTYPE_F32 ? 4 : 2, Q = PAIR ? 2 : 1;
+    typedef uint32_t Codes __attribute__((ext_vector_type(Q)));
     const uint32_t unit_len = t.row_len > 0 ? t.row_len : UNIT;
     const long long chunk_unit = (long long)chunk * SHARE, whole = t.numel / unit_len;
-    const uint32_t units = (uint32_t)min((long long)SHARE, max(0LL, whole - chunk_unit)), sub = threadIdx.x % GROUP;
+    const uint32_t units = (uint32_t)min((long long)SHARE, max(0LL, whole - chunk_unit)), first = 4u * Q * (threadIdx.x % GROUP);
     if (units > 0) {
         const uint8_t *m = t.m + chunk_unit * unit_len, *v = t.v + chunk_unit * unit_len, *exponents = t.exponents + 2 * chunk_unit;
         char *m_out = (char *)t.m_out + chunk_unit * unit_len * BYTES, *v_out = (char *)t.v_out + chunk_unit * unit_len * BYTES;
-        uint32_t mc[UNROLL], vc[UNROLL], x[UNROLL], e[UNROLL];
+        Codes mc[UNROLL], vc[UNROLL];
+        uint32_t x[UNROLL], e[UNROLL];
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
             const uint32_t unit = min(threadIdx.x / GROUP + u * PER_PASS, units - 1u);
-            e[u] = unit * unit_len + min(4u * sub, unit_len - 4u);
-            mc[u] = load_at<uint32_t>(m + e[u]);
-            vc[u] = load_at<uint32_t>(v + e[u]);
+            e[u] = unit * unit_len + min(first, unit_len - 4u * Q);
+            mc[u] = load_at<Codes>(m + e[u]);
+            vc[u] = load_at<Codes>(v + e[u]);
             x[u] = load_at<uint16_t>(exponents + 2u * unit);
         }
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u)
-            if (threadIdx.x / GROUP + u * PER_PASS < units && 4u * sub < unit_len) read_four<DT>(mc[u], vc[u], x[u], m_out, v_out, e[u]);
+            if (threadIdx.x / GROUP + u * PER_PASS < units && first < unit_len) read_codes<DT, Q>(mc[u], vc[u], x[u], m_out + e[u] * BYTES, v_out + e[u] * BYTES);
     }
-    if (GROUP == 16 && whole * unit_len < t.numel && whole >= chunk_unit && whole < chunk_unit + SHARE && threadIdx.x < GROUP)
+    if (GROUP * Q == 16 && whole * unit_len < t.numel && whole >= chunk_unit && whole < chunk_unit + SHARE && threadIdx.x < GROUP)
         read_unit<GROUP, DT>(t, whole, (int)unit_len);
 }
 
-template <int L, int DT>
+// Rows of L = 1..4 elements: nothing is shared by a row but its exponents, so a lane reads quads wherever rows begin (rows of
+// three, 56M elements to bfloat16 / float: 55 / 88 us; with whole rows a lane, 48 bytes from lane to lane, 109 / 242)
+template <int UNROLL, int L, int DT>
 __device__ __forceinline__ void read_narrow(const MomentsTensor &t, unsigned chunk) {
-    constexpr int R = narrow_rows(L), Q = R * L / 4;
-    const long long rows = t.numel / L, row0 = R * ((long long)chunk * GS_BLOCK + threadIdx.x);
-    if (row0 >= rows) return;
-    if (row0 + R > rows) {
-        for (long long r = row0; r < rows; ++r) read_unit<1, DT>(t, r, L);
-        return;
-    }
-    uint16_t x[R];
-    __builtin_memcpy(x, t.exponents + 2 * row0, 2 * R);
+    constexpr uint32_t SHARE = 4 * GS_BLOCK * UNROLL, BYTES = DT == GS_DTYPE_F32 ? 4 : 2;
+    constexpr int R = L == 1 ? 4 : (L == 4 ? 1 : 2);        // rows that a quad meets
+    typedef typename Four<DT>::type Value;
+    const long long first = (long long)chunk * SHARE, row0 = first / L;
+    const uint32_t left = (uint32_t)min((long long)SHARE, t.numel - first), ahead = (uint32_t)(first - row0 * L);
+    const uint8_t *m = t.m + first, *v = t.v + first, *exponents = t.exponents + 2 * row0;
+    char *m_out = (char *)t.m_out + first * BYTES, *v_out = (char *)t.v_out + first * BYTES;
+    uint32_t mc[UNROLL], vc[UNROLL];
+    uint16_t x[UNROLL][R];
 #pragma unroll
-    for (int c = 0; c < Q; ++c) {
-        const uint32_t mc = load_at<uint32_t>(t.m + row0 * L + 4 * c), vc = load_at<uint32_t>(t.v + row0 * L + 4 * c);
-        f32x4 m = units_of(mc), v;
+    for (int u = 0; u < UNROLL; ++u) {
+        const uint32_t e = 4u * (u * GS_BLOCK + threadIdx.x);
+        if (e + 4u > left) continue;
+        mc[u] = load_at<uint32_t>(m + e);
+        vc[u] = load_at<uint32_t>(v + e);
+        __builtin_memcpy(x[u], exponents + 2u * ((ahead + e) / L), 2 * R);
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+        const uint32_t e = 4u * (u * GS_BLOCK + threadIdx.x), phase = L == 3 ? (ahead + e) % L : 0u;      // (place in the first row)
+        if (e + 4u > left) continue;
+        const f32x4 units = units_of(mc[u]);
+        f32x4 mo, vo;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const uint32_t xr = x[(4 * c + j) / L];
-            m[j] *= m_scale(xr);
-            v[j] = v_value((vc >> (8 * j)) & 255u, xr);
+            const uint32_t xr = L == 3 ? x[u][phase + j < 3u ? 0 : R - 1] : x[u][j / L];
+            mo[j] = units[j] * m_scale(xr);
+            vo[j] = v_value((vc[u] >> (8 * j)) & 255u, xr);
         }
-        store_four<DT>(t.m_out, row0 * L + 4 * c, m);
-        store_four<DT>(t.v_out, row0 * L + 4 * c, v);
+        stream_store(m_out + e * BYTES, __builtin_convertvector(mo, Value));
+        stream_store(v_out + e * BYTES, __builtin_convertvector(vo, Value));
+    }
+    if (const uint32_t e = left / 4u * 4u + threadIdx.x; e < left && threadIdx.x < 4) {     // behind the last whole quad
+        const uint32_t row = (ahead + e) / L, xr = load_at<uint16_t>(exponents + 2u * row);
+        store_one<DT>(m_out, e, unit_of(m[e]) * m_scale(xr));
+        store_one<DT>(v_out, e, v_value(v[e], xr));
     }
 }
+
+// Two quads a lane to 16-bit values, so that they are 16 bytes: units of 64 and rows of 40, 48, 56 and 64 (56M elements in rows
+// of 56: 50 us, 6.7 TB/s, a quad a lane 53)
+__host__ __device__ constexpr bool read_pairs(int row_len) { return row_len == 0 || (row_len > 32 && row_len % 8 == 0); }
 
 template <int UNROLL, int DT>
 __global__ __launch_bounds__(GS_BLOCK) void read_moments_kernel(MomentsBatch b) {
@@ -916,15 +943,17 @@ __global__ __launch_bounds__(GS_BLOCK) void read_moments_kernel(MomentsBatch b) 
     const unsigned chunk = blockIdx.x - b.first_chunk[ti];
     const int lanes = lanes_of(t.row_len);
     if (t.row_len == 0 || t.row_len > 4) {
-        if (lanes == 16) return read_quads<UNROLL, DT, 16>(t, chunk);
-        if (lanes == 8) return read_quads<UNROLL, DT, 8>(t, chunk);
-        if (lanes == 4) return read_quads<UNROLL, DT, 4>(t, chunk);
-        return read_quads<UNROLL, DT, 2>(t, chunk);
+        if constexpr (DT != GS_DTYPE_F32)
+            if (read_pairs(t.row_len)) return read_quads<passes(UNROLL, true), DT, 8, true>(t, chunk);
+        if (lanes == 16) return read_quads<UNROLL, DT, 16, false>(t, chunk);
+        if (lanes == 8) return read_quads<UNROLL, DT, 8, false>(t, chunk);
+        if (lanes == 4) return read_quads<UNROLL, DT, 4, false>(t, chunk);
+        return read_quads<UNROLL, DT, 2, false>(t, chunk);
     }
-    if (t.row_len == 3) return read_narrow<3, DT>(t, chunk);
-    if (t.row_len == 1) return read_narrow<1, DT>(t, chunk);
-    if (t.row_len == 2) return read_narrow<2, DT>(t, chunk);
-    return read_narrow<4, DT>(t, chunk);
+    if (t.row_len == 3) return read_narrow<UNROLL, 3, DT>(t, chunk);
+    if (t.row_len == 1) return read_narrow<UNROLL, 1, DT>(t, chunk);
+    if (t.row_len == 2) return read_narrow<UNROLL, 2, DT>(t, chunk);
+    return read_narrow<UNROLL, 4, DT>(t, chunk);
 }
 
 // ------------------------------------------------------------------ norm of gradients
@@ -1205,9 +1234,10 @@ int form_of(int row, bool masked, bool pair) {
     if (row == 0 || (row > 32 && row % (pair ? 8 : 4) == 0)) return masked ? QUADS_MASKED : QUADS;
     return masked ? ROWS_MASKED : ROWS;
 }
-long long read_chunks(long long numel, int row, int unroll) {
+long long read_chunks(long long numel, int row, int dtype, int unroll) {
     const long long units = row > 0 ? numel / row : (numel + UNIT - 1) / UNIT;
-    const int per = row >= 1 && row <= 4 ? narrow_rows(row) * GS_BLOCK : GS_BLOCK / lanes_of(row) * unroll;
+    if (row >= 1 && row <= 4) return (numel + 4 * GS_BLOCK * unroll - 1) / (4 * GS_BLOCK * unroll);
+    const int per = dtype != GS_DTYPE_F32 && read_pairs(row) ? GS_BLOCK / 8 * passes(unroll, true) : GS_BLOCK / lanes_of(row) * unroll;
     return (units + per - 1) / per;
 }
 
@@ -1396,7 +1426,7 @@ extern "C" int gs_read_moments(int n_tensors, const uint64_t *host_exp_avg, cons
         const int row = host_row_len[i];
         GS_REQUIRE(n >= 0 && n < (1LL << 46) && row >= 0 && row <= UNIT && (row == 0 || n % row == 0),
                    "gs_read_moments: numel in [0, 2^46), rows of 1..64 elements");
-        GS_REQUIRE(read_chunks(n, row, 1) < 0x7fffffffLL, "gs_read_moments: tensor too large");
+        GS_REQUIRE(read_chunks(n, row, out_dtype, 1) < 0x7fffffffLL, "gs_read_moments: tensor too large");
         GS_REQUIRE(n == 0 || (host_exp_avg[i] && host_exp_avg_sq[i] && host_exponents[i] && host_m_out[i] && host_v_out[i]),
                    "gs_read_moments: null tensor");
         GS_REQUIRE(aligned_to(host_m_out[i] | host_v_out[i], element_bytes(out_dtype)), "gs_read_moments: misaligned output");
@@ -1431,7 +1461,7 @@ extern "C" int gs_read_moments(int n_tensors, const uint64_t *host_exp_avg, cons
             const int row = host_row_len[i];
             t = {(const uint8_t *)host_exp_avg[i], (const uint8_t *)host_exp_avg_sq[i], (const uint8_t *)host_exponents[i],
                  (void *)host_m_out[i], (void *)host_v_out[i], host_numel[i], row};
-            chunks = read_chunks(host_numel[i], row, unroll);
+            chunks = read_chunks(host_numel[i], row, out_dtype, unroll);
         }
         if (b.n_tensors > 0 && (end || b.n_tensors == MAX_TENSORS || (long long)b.first_chunk[b.n_tensors] + chunks >= 0x7fffffffLL)) {
             if (unroll == 1) launch_moments<1>(out_dtype, b, (hipStream_t)stream);
