@@ -388,6 +388,10 @@ class AdamW(torch.optim.Optimizer):
             if not self.capturable:
                 for state, count in zip(states, steps):
                     state["step"] = count
+            if masked:                  # (without a mask no row is late any more)
+                for p, state in zip(params, states):
+                    if id(p) not in self._row_mask:
+                        state.pop("last_step", None)
         return loss
 
     def _work(self) -> dict:
@@ -404,9 +408,11 @@ class AdamW(torch.optim.Optimizer):
                 params, grads, ids = ([column[i] for i in kept] for column in (params, grads, ids))
             states = [self.state[p] for p in params]
             masks = [self._row_mask.get(id(p)) for p in params] if self._row_mask else [None] * len(params)
-            for p, state, mask in zip(params, states, masks):
+            for i, (p, state, mask) in enumerate(zip(params, states, masks)):
                 if not state or (mask is not None and "last_step" not in state):
                     self._complete(p, state, mask, group)
+                elif mask is None and "last_step" in state:
+                    masks[i] = self._no_row_masked(p)
             kinds = [("exponents" in s, p.get_device()) for p, s in zip(params, states)]
             for kind in sorted(set(kinds)):
                 columns = params, grads, states, masks, ids
@@ -420,7 +426,7 @@ class AdamW(torch.optim.Optimizer):
 
     def _complete(self, p: torch.Tensor, state: dict, mask: Optional[torch.Tensor], group: dict) -> None:
         """The state of a parameter that has none, or none for its row mask yet."""
-        if not p.is_cuda:
+        if not state and not p.is_cuda:
             raise RuntimeError("optim.AdamW needs parameters on the HIP device: there is no CPU path")
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("run one step of AdamW before capturing one: its state is made there")
@@ -429,6 +435,13 @@ class AdamW(torch.optim.Optimizer):
         if mask is not None:
             # moments from a state_dict without row masks are current as of the previous step
             state["last_step"] = torch.full((p.shape[0],), int(state["step"]), dtype=torch.int32, device=p.device)
+
+    def _no_row_masked(self, p: torch.Tensor) -> torch.Tensor:
+        """For a parameter whose state comes from steps under a row mask and that has no mask now: one that lets every row take
+        this step, late ones with their decay.  The stamps end with it: the steps after it would not keep them."""
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("run one step of AdamW before capturing one: rows that an earlier mask held back take it there")
+        return torch.zeros(p.shape[0], dtype=torch.int8, device=p.device)
 
     def _clip(self, parts) -> torch.Tensor:
         """The clipping coefficient of all gradients (and ``last_grad_norm``)."""
@@ -503,6 +516,8 @@ class AdamW(torch.optim.Optimizer):
             if name not in held or (name == "master" and (not self.master_weights or p.dtype == torch.float32)):
                 continue
             value = held[name]
+            if name == "last_step" and (_row_length(p.shape) == 0 or p.dtype != torch.float32):
+                raise ValueError("state_dict: last_step belongs to a float32 parameter of rows")
             if tuple(value.shape) != tuple(shape):
                 raise ValueError(f"state_dict: {name} has shape {tuple(value.shape)}, not {tuple(shape)}")
             if (value.dtype == torch.uint8) != (types[name] == torch.uint8):

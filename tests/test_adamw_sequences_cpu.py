@@ -1,0 +1,71 @@
+"""Sequences of calls of optim.AdamW that need no device: states that are loaded, masks that come and go, hooks.  The step itself
+is replaced by the plain one in 64 bits (adamw_plain.py); what it is handed is what is tested."""
+import numpy as np
+import pytest
+import torch
+
+from taichi_3d_gaussian_splatting_amd import optim
+from tests import adamw_plain as plain
+
+HYPER = dict(lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2)
+
+
+def _plain_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, betas, eps, weight_decay, exponents=None, masters=None, row_masks=None,
+                last_steps=None, grad_scale=None, seed=0, tensor_ids=None):
+    """adamw_step_ for float32 host tensors with moments in 32 bits."""
+    for i, p in enumerate(params):
+        mask = None if row_masks is None else row_masks[i]
+        missed = None if mask is None else step[i] - 1 - last_steps[i].numpy()
+        state = [t.detach().double().numpy() for t in (p, grads[i], exp_avgs[i], exp_avg_sqs[i])]
+        new = plain.update(*state, step=step[i], lr=lr[i], betas=betas, eps=eps, weight_decay=weight_decay[i], missed=missed)
+        for t, value in zip((p, exp_avgs[i], exp_avg_sqs[i]), new):
+            value = torch.from_numpy(value).float()
+            t.copy_(value if mask is None else torch.where(mask[:, None] == 0, value, t))
+        if mask is not None:
+            last_steps[i].copy_(torch.where(mask == 0, torch.full_like(last_steps[i], step[i]), last_steps[i]))
+
+
+@pytest.fixture
+def host_steps(monkeypatch):
+    """AdamW on host tensors: the plain step in the kernels' place."""
+    monkeypatch.setattr(optim, "adamw_step_", _plain_step)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+
+
+def _masked_state(shape, step, stamps, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    return {"state": {0: dict(step=step, exp_avg=torch.randn(shape, generator=gen), exp_avg_sq=torch.rand(shape, generator=gen),
+                              last_step=torch.as_tensor(stamps, dtype=torch.int32))},
+            "param_groups": [dict(params=[0], state_bits=32, **HYPER)]}
+
+
+def test_stamps_of_rows_do_not_outlive_steps_without_a_mask(host_steps):
+    """A state saved under a row mask goes on without one, and under one again: late rows are decayed by the first step that
+    reaches them, and the steps without the mask owe no decay."""
+    shape, stamps = (4, 3), [100, 97, 100, 60]
+    p = torch.nn.Parameter(torch.ones(shape))
+    opt = optim.AdamW([p], **HYPER)
+    saved = _masked_state(shape, 100, stamps)
+    opt.load_state_dict(saved)
+    want = [np.ones(shape), *(saved["state"][0][k].double().numpy() for k in ("exp_avg", "exp_avg_sq"))]
+    missed = 100 - np.array(stamps)
+    gen = torch.Generator().manual_seed(1)
+    for t in range(101, 113):
+        if t == 106:
+            opt.set_row_mask(p, torch.zeros(4, dtype=torch.int8))
+        p.grad = torch.randn(shape, generator=gen)
+        opt.step()
+        want = plain.update(want[0], p.grad.double().numpy(), want[1], want[2], step=t, missed=missed, **HYPER)
+        missed = None
+        state = opt.state[p]
+        # the host's step rounds each value to float32 once a step: t steps of half a spacing
+        for got, value in zip((p.detach(), state["exp_avg"], state["exp_avg_sq"]), want):
+            assert np.allclose(got.numpy(), value, rtol=20 * 2.0 ** -24, atol=20 * 2.0 ** -24), t
+    assert (opt.state[p]["last_step"] == 112).all()
+
+
+def test_stamps_are_not_taken_for_parameters_that_cannot_have_them():
+    for p in (torch.zeros(4, 3, dtype=torch.bfloat16), torch.zeros(4, 65)):
+        opt = optim.AdamW([torch.nn.Parameter(p)], master_weights=False, **HYPER)
+        with pytest.raises(ValueError, match="last_step"):
+            opt.load_state_dict(_masked_state(tuple(p.shape), 5, [5, 5, 3, 5]))
