@@ -479,27 +479,35 @@ class AdamW(torch.optim.Optimizer):
             self._row_mask = {id(params[i]): mask for i, mask in masks.items()}
 
     def load_state_dict(self, state_dict) -> None:
-        """As in torch, but the state keeps its own types (torch would cast codes, counts and float32 moments of 16-bit
-        parameters to the parameter's type).  Whether moments have 8 or 32 bits is what was saved; amsgrad and maximize are not
-        known here.  A state_dict that does not fit is refused and changes nothing."""
-        saved_groups = state_dict["param_groups"]
-        for group in saved_groups:
-            if group.get("amsgrad") or group.get("maximize"):
-                raise ValueError("state_dict: AdamW here has neither amsgrad nor maximize")
-        saved = [i for group in saved_groups for i in group["params"]]
+        """As in torch, hooks among it, but the state keeps its own types (torch would cast codes, counts and float32 moments of
+        16-bit parameters to the parameter's type).  Whether moments have 8 or 32 bits is what was saved; amsgrad and maximize are
+        not known here.  A state_dict that does not fit is refused and changes nothing."""
         params = [p for group in self.param_groups for p in group["params"]]
-        held = [state_dict["state"].get(i) for i in saved]
-        states = [self._loaded(p, h) if h else None for p, h in zip(params, held)]
-        super().load_state_dict({"state": {}, "param_groups": saved_groups})       # (refuses other groups)
-        self.state.clear()
-        for p, state in zip(params, states):
-            if state is not None:
-                self.state[p] = state
-        for group in self.param_groups:
-            group.setdefault("state_bits", self.defaults["state_bits"])
-            for p in group["params"]:
-                if p in self.state:
-                    group["state_bits"] = 8 if "exponents" in self.state[p] else 32
+        states = []
+
+        def take(_, given):         # (behind the other hooks: what they return is what is loaded)
+            saved_groups = given["param_groups"]
+            for group in saved_groups:
+                if group.get("amsgrad") or group.get("maximize"):
+                    raise ValueError("state_dict: AdamW here has neither amsgrad nor maximize")
+            held = [given["state"].get(i) for group in saved_groups for i in group["params"]]
+            states.extend(self._loaded(p, h) if h else None for p, h in zip(params, held))
+            return {**given, "state": {}}
+
+        def put(_):                 # (in front of the other hooks: they find the state)
+            self.state.clear()
+            self.state.update((p, state) for p, state in zip(params, states) if state is not None)
+            for group in self.param_groups:
+                group.setdefault("state_bits", self.defaults["state_bits"])
+                for p in group["params"]:
+                    if p in self.state:
+                        group["state_bits"] = 8 if "exponents" in self.state[p] else 32
+        handles = [self.register_load_state_dict_pre_hook(take), self.register_load_state_dict_post_hook(put, prepend=True)]
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for handle in handles:
+                handle.remove()
 
     def _loaded(self, p: torch.Tensor, held: dict) -> dict:
         """A saved state as this optimiser's, on the parameter's device."""

@@ -69,3 +69,56 @@ def test_stamps_are_not_taken_for_parameters_that_cannot_have_them():
         opt = optim.AdamW([torch.nn.Parameter(p)], master_weights=False, **HYPER)
         with pytest.raises(ValueError, match="last_step"):
             opt.load_state_dict(_masked_state(tuple(p.shape), 5, [5, 5, 3, 5]))
+
+
+def _plain_state(shape=(4, 3), step=7, seed=0):
+    saved = _masked_state(shape, step, [step] * shape[0], seed)
+    del saved["state"][0]["last_step"]
+    return saved
+
+
+def test_hooks_of_load_state_dict_see_and_change_what_is_loaded():
+    """As in torch: a hook before the load may return another state_dict, one behind it finds the loaded state and groups."""
+    seen = []
+    for kind in (torch.optim.AdamW, optim.AdamW):
+        opt = kind([torch.nn.Parameter(torch.zeros(4, 3))], **HYPER)
+        saved = _plain_state()
+        kept = {k: v.clone() if isinstance(v, torch.Tensor) else v for k, v in saved["state"][0].items()}
+
+        def before(optimizer, state_dict):
+            state = dict(state_dict["state"][0], step=77, exp_avg=state_dict["state"][0]["exp_avg"] + 1)
+            return {"state": {0: state}, "param_groups": [dict(state_dict["param_groups"][0], lr=0.5)]}
+
+        def after(optimizer):
+            (state,) = optimizer.state.values()
+            seen.append((int(state["step"]), optimizer.param_groups[0]["lr"], state["exp_avg"].clone(), "state_bits" in optimizer.param_groups[0]))
+        handles = [opt.register_load_state_dict_pre_hook(before), opt.register_load_state_dict_post_hook(after)]
+        opt.load_state_dict(saved)
+        for name, value in kept.items():
+            assert torch.equal(saved["state"][0][name], value) if isinstance(value, torch.Tensor) else saved["state"][0][name] == value
+        for handle in handles:
+            handle.remove()
+        opt.load_state_dict(saved)
+        (state,) = opt.state.values()
+        assert int(state["step"]) == 7
+        assert not opt._optimizer_load_state_dict_pre_hooks and not opt._optimizer_load_state_dict_post_hooks
+    assert [s[:2] for s in seen] == [(77, 0.5)] * 2 and torch.equal(seen[0][2], seen[1][2]) and seen[1][3]
+
+
+def test_a_refused_state_dict_changes_nothing_and_leaves_no_hook():
+    opt = optim.AdamW([torch.nn.Parameter(torch.zeros(4, 3))], **HYPER)
+    opt.load_state_dict(_plain_state())
+    (before,) = (dict(s) for s in opt.state.values())
+    wrong_shape, two_groups = _plain_state(step=9), _plain_state(step=9)
+    wrong_shape["state"][0]["exp_avg"] = torch.zeros(5, 3)
+    two_groups["param_groups"] *= 2
+    other_size = _plain_state(step=9)
+    other_size["param_groups"] = [dict(other_size["param_groups"][0], params=[0, 1])]
+    amsgrad = _plain_state(step=9)
+    amsgrad["param_groups"][0]["amsgrad"] = True
+    for bad in (wrong_shape, two_groups, other_size, amsgrad):
+        with pytest.raises(ValueError):
+            opt.load_state_dict(bad)
+        (state,) = opt.state.values()
+        assert state.keys() == before.keys() and all(state[k] is before[k] for k in before)
+        assert not opt._optimizer_load_state_dict_pre_hooks
