@@ -480,8 +480,9 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict) -> None:
         """As in torch, hooks among it, but the state keeps its own types (torch would cast codes, counts and float32 moments of
-        16-bit parameters to the parameter's type).  Whether moments have 8 or 32 bits is what was saved; amsgrad and maximize are
-        not known here.  A state_dict that does not fit is refused and changes nothing."""
+        16-bit parameters to the parameter's type).  Whether moments have 8 or 32 bits is what was saved; options that a saved
+        group does not name stay the group's own; amsgrad and maximize are not known here.  A state_dict that does not fit is
+        refused and changes nothing."""
         params = [p for group in self.param_groups for p in group["params"]]
         states = []
 
@@ -492,13 +493,14 @@ class AdamW(torch.optim.Optimizer):
                     raise ValueError("state_dict: AdamW here has neither amsgrad nor maximize")
             held = [given["state"].get(i) for group in saved_groups for i in group["params"]]
             states.extend(self._loaded(p, h) if h else None for p, h in zip(params, held))
-            return {**given, "state": {}}
+            kept = [{name: group[name] for name in self.defaults if name in group} for group in self.param_groups]
+            kept += [{}] * (len(saved_groups) - len(kept))
+            return {**given, "state": {}, "param_groups": [{**own, **group} for own, group in zip(kept, saved_groups)]}
 
         def put(_):                 # (in front of the other hooks: they find the state)
             self.state.clear()
             self.state.update((p, state) for p, state in zip(params, states) if state is not None)
             for group in self.param_groups:
-                group.setdefault("state_bits", self.defaults["state_bits"])
                 for p in group["params"]:
                     if p in self.state:
                         group["state_bits"] = 8 if "exponents" in self.state[p] else 32

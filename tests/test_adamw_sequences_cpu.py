@@ -122,3 +122,23 @@ def test_a_refused_state_dict_changes_nothing_and_leaves_no_hook():
         (state,) = opt.state.values()
         assert state.keys() == before.keys() and all(state[k] is before[k] for k in before)
         assert not opt._optimizer_load_state_dict_pre_hooks
+
+
+def test_options_that_a_saved_group_does_not_name_stay_the_groups_own(host_steps):
+    """A state_dict of optim.Adam has no weight decay: the step takes the group's."""
+    p = torch.nn.Parameter(torch.ones(4, 3))
+    adam = optim.Adam([p], lr=2e-3)
+    saved = {"state": _plain_state()["state"], "param_groups": adam.state_dict()["param_groups"]}
+    opt = optim.AdamW([dict(params=[p], weight_decay=0.3)], lr=1e-3)
+    opt.load_state_dict(saved)
+    assert "weight_decay" not in saved["param_groups"][0]
+    assert opt.param_groups[0]["lr"] == 2e-3 and opt.param_groups[0]["weight_decay"] == 0.3 and opt.param_groups[0]["state_bits"] == 32
+    p.grad = torch.zeros(4, 3)
+    m, v = (saved["state"][0][k].double().numpy() for k in ("exp_avg", "exp_avg_sq"))
+    want = plain.update(np.ones((4, 3)), np.zeros((4, 3)), m, v, step=8, **{**HYPER, "lr": 2e-3, "weight_decay": 0.3})[0]
+    opt.step()
+    assert np.allclose(p.detach().numpy(), want, rtol=4 * 2.0 ** -24, atol=0)
+    # groups without a state keep the form that they were made with
+    opt = optim.AdamW([dict(params=[p], state_bits=8)], lr=1e-3)
+    opt.load_state_dict({"state": {}, "param_groups": torch.optim.AdamW([p]).state_dict()["param_groups"]})
+    assert opt.param_groups[0]["state_bits"] == 8
