@@ -199,6 +199,9 @@ def host():
             raise RuntimeError(f"_gs_host is missing or does not load ({e}): build it with `make -C {os.path.join(_HERE, 'csrc')}` "
                                "(or __graft_entry__.build()).  There is no fallback path.") from e
         lib = load()
+        built_for = getattr(_gs_host, "ABI_VERSION", None)
+        if built_for != ABI_VERSION:
+            raise RuntimeError(f"_gs_host was built for ABI {built_for}, not {ABI_VERSION}: build it again")
         _gs_host.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
                         for name in ("gs_adamw_step", "gs_grad_norm", "gs_read_moments")))
         _host = _gs_host

@@ -369,5 +369,7 @@ PyMODINIT_FUNC PyInit__gs_host(void) {
         {"CODE", CODE}, {"EXPONENTS", EXPONENTS}, {"MASK", MASK}, {"PARAM_MASK", PARAM_MASK}, {"STAMP", STAMP}, {"VALUE", VALUE}};
     for (const auto &k : kinds)
         if (PyModule_AddIntConstant(m, k.name, k.value) < 0) return nullptr;
+    // (of the header that the calls above were compiled from: the package compares it with the library's before it binds)
+    if (PyModule_AddIntConstant(m, "ABI_VERSION", GS_ABI_VERSION) < 0) return nullptr;
     return m;
 }
