@@ -611,10 +611,14 @@ __device__ __forceinline__ void step_quads_masked(const AdamwTensor &t, const Ad
 }
 
 // Rows of L = 1..4 elements, as many rows a lane as make whole quads (rows of three: four rows, three quads): every access
-// is four elements although a row is not.  Of rows under a mask the lane writes back what it read.  With codes of one
-// quad only a lane has too little in flight: it takes rows at two places (40M floats, rows of 1 / 2 / 4: 157 / 143 / 136 us at
-// one, 145 / 134 / 127 at two, 152 / 140 / 132 at four; all live under a mask 268 / 237 / 235, 210 / 179 / 164, 217 / 181 / 155).
+// is four elements although a row is not.  With codes of one quad only a lane has too little in flight: it takes rows at two places
+// (40M floats, rows of 1 / 2 / 4: 157 / 143 / 136 us at one, 145 / 134 / 127 at two, 152 / 140 / 132 at four; all live under a mask
+// 268 / 237 / 235, 210 / 179 / 164, 217 / 181 / 155).
 // 40M bfloat16 in rows of 1 / 2 / 3 / 4: 102 / 90 / 92 / 79 us, a row a lane and element by element 304 / 188 / 152 / 148.
+// Masked rows are not written, someone else may do so meanwhile: where some of a lane's rows are masked it stores the others row by
+// row.  40M floats under a mask, rows of 1 / 2 / 3, 32 bits, all live 262 / 233 / 243 us, half of them at random 342 / 261 / 290
+// (266 / 237 / 248 with whole quads, masked rows as they were read), 30 % 326 / 267 / 276; 8 bits 212 / 181 / 162,
+// 279 / 199 / 197, 262 / 197 / 182; row by row throughout, all live: 342 / 246 / 292 and 269 / 189 / 197.
 __host__ __device__ constexpr int narrow_rows(int row_len) { return row_len == 4 ? 1 : (row_len == 2 ? 2 : 4); }
 __host__ __device__ constexpr int narrow_passes(int row_len, bool state8) { return state8 && row_len != 3 ? 2 : 1; }
 
@@ -708,6 +712,43 @@ __device__ __forceinline__ void step_narrow(const AdamwTensor &t, const AdamwSca
                     s.m[0][j] = live ? m : s.m[0][j];
                     s.v[0][j] = live ? v : s.v[0][j];
                 }
+            }
+        }
+        if (MASKED && R > 1) {
+            bool all = true;
+#pragma unroll
+            for (int r = 0; r < R; ++r) all = all && mask[u][r] == 0;
+            if (!all) {
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    if (mask[u][r] != 0) continue;
+                    const uint32_t e = (uint32_t)((row + r) * L);
+                    float out[3][L];
+                    uint8_t codes[2][L];
+#pragma unroll
+                    for (int i = 0; i < L; ++i) {
+                        const int c = (r * L + i) / 4, j = (r * L + i) % 4;
+                        out[0][i] = p[c][0][j];
+                        if constexpr (STATE8) {
+                            codes[0][i] = (uint8_t)(mc[c] >> (8 * j));
+                            codes[1][i] = (uint8_t)(vc[c] >> (8 * j));
+                        } else {
+                            out[1][i] = q[u][c].m[0][j];
+                            out[2][i] = q[u][c].v[0][j];
+                        }
+                    }
+                    __builtin_memcpy(b.param + 4 * e, out[0], 4 * L);
+                    if constexpr (STATE8) {
+                        __builtin_memcpy(b.m + e, codes[0], L);
+                        __builtin_memcpy(b.v + e, codes[1], L);
+                        store_at(b.exponents + 2 * (row + r), x[u][r]);
+                    } else {
+                        __builtin_memcpy(b.m + 4 * e, out[1], 4 * L);
+                        __builtin_memcpy(b.v + 4 * e, out[2], 4 * L);
+                    }
+                    stamps[row + r] = k.step;
+                }
+                continue;
             }
         }
         if (MASKED) __builtin_memcpy(stamps + row, last[u], 4 * R);

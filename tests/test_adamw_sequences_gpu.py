@@ -67,3 +67,37 @@ def test_a_mask_that_goes_and_comes_back_owes_no_decay(bits, capturable):
         for name in ("step", "exp_avg", "exp_avg_sq", "exponents", "last_step"):
             x, y = a.state[q].get(name), b.state[r].get(name)
             assert torch.equal(x, y) if isinstance(x, torch.Tensor) else x == y, name
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("columns", [1, 2, 3, 4, 5, 17, 56])
+def test_masked_rows_may_be_written_while_the_others_are_stepped(bits, columns):
+    """A writer of masked rows on one stream (new points that are laid out, say) and steps of the live rows on another: neither loses
+    what it wrote.  Compared with the same work one after the other, bit for bit."""
+    o = _optim()
+    n, rounds = 1_200_000 // columns, 30
+    gen = torch.Generator(device=DEV).manual_seed(columns)
+    p, g = (torch.randn(n, columns, device=DEV, generator=gen) for _ in range(2))
+    mask = (torch.rand(n, device=DEV, generator=gen) < 0.5).to(torch.int8)
+    dead = mask.nonzero()[:, 0]
+
+    def run(together):
+        m, v, x = o.new_moments(p, bits)
+        q, stamps = p.clone(), torch.zeros(n, dtype=torch.int32, device=DEV)
+        written = [t for t in (q, m, v, stamps, x) if t is not None]
+        streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+        torch.cuda.synchronize()
+        for t in range(1, rounds + 1):
+            with torch.cuda.stream(streams[0]):
+                o.adamw_step_([q], [g], [m], [v], step=t, exponents=None if x is None else [x], row_masks=[mask], last_steps=[stamps])
+            if not together:
+                torch.cuda.synchronize()
+            with torch.cuda.stream(streams[1]):
+                for w in written:
+                    w[dead] = w[dead] + 1
+            if not together:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        return written
+    for got, want in zip(run(True), run(False)):
+        assert torch.equal(got, want)
