@@ -1269,6 +1269,8 @@ u64 entry(const uint64_t *column, int i) { return column ? column[i] : 0; }
 constexpr int UNROLL = 4, UNROLL_READ = 4;
 constexpr int OCCUPANCY_LDS = 40960;
 constexpr long long SMALL_CHUNKS = 2048;    // of 16 units
+// Workgroups of the largest launch: gridDim.x * blockDim.x has to stay below 2^32
+constexpr long long MAX_CHUNKS = (1LL << 32) / GS_BLOCK - 1;
 
 int form_of(int row, bool masked, bool pair) {
     if (row >= 1 && row <= 4) return NARROW;
@@ -1344,9 +1346,6 @@ extern "C" int gs_adamw_step(int n_tensors, const uint64_t *host_param, const ui
         GS_REQUIRE(n >= 0 && n < (1LL << 46) && row >= 0 && row <= UNIT && (row == 0 || n % row == 0),
                    "gs_adamw_step: numel in [0, 2^46), too large else, rows of 1..64 elements");
         GS_REQUIRE(dt == GS_DTYPE_F32 || dt == GS_DTYPE_BF16 || dt == GS_DTYPE_F16, "gs_adamw_step: unknown dtype");
-        const bool masked = entry(host_row_mask, i) != 0;
-        const int rows = masked || state8 ? row : 0;
-        GS_REQUIRE(form_chunks(form_of(rows, masked, false), n, rows, 1, false, state8) < 0x7fffffffLL, "gs_adamw_step: tensor too large");
         GS_REQUIRE(n == 0 || (host_param[i] && host_grad[i] && host_exp_avg[i] && host_exp_avg_sq[i] && (!state8 || host_exponents[i])),
                    "gs_adamw_step: null tensor");
         GS_REQUIRE(!entry(host_row_mask, i) || (row > 0 && dt == GS_DTYPE_F32 && host_last_step[i]), "gs_adamw_step: a row mask needs float rows and last steps");
@@ -1357,6 +1356,12 @@ extern "C" int gs_adamw_step(int n_tensors, const uint64_t *host_param, const ui
                        aligned_to(entry(host_master, i) | (entry(host_row_mask, i) ? host_last_step[i] : 0), 4),
                    "gs_adamw_step: an address is no multiple of its type's size");
         units_of_16 += form_chunks(QUADS, n, row, 1, false, false);
+    }
+    const int unroll = !state8 || units_of_16 <= SMALL_CHUNKS ? 1 : UNROLL;
+    for (int i = 0; i < n_tensors; ++i) {
+        const bool masked = entry(host_row_mask, i) != 0, pair = pairs(host_dtype[i], entry(host_master, i) != 0, state8);
+        const int row = masked || state8 ? host_row_len[i] : 0;      // (moments in 32 bits without a mask: units of 64 whatever the shape)
+        GS_REQUIRE(form_chunks(form_of(row, masked, pair), host_numel[i], row, unroll, pair, state8) <= MAX_CHUNKS, "gs_adamw_step: tensor too large");
     }
     {
         Range *r = (Range *)malloc((size_t)n_tensors * 8 * sizeof(Range));
@@ -1382,7 +1387,6 @@ extern "C" int gs_adamw_step(int n_tensors, const uint64_t *host_param, const ui
     }
     hipStream_t s = (hipStream_t)stream;
     AdamwScalars *device_scalars = (AdamwScalars *)workspace;
-    const int unroll = !state8 || units_of_16 <= SMALL_CHUNKS ? 1 : UNROLL;
     StepBatch q;
     q.b.grad_scale = grad_scale;
     // one type after the other: float, float under a mask, 16 bits with and without a master copy
@@ -1398,7 +1402,7 @@ extern "C" int gs_adamw_step(int n_tensors, const uint64_t *host_param, const ui
             long long chunks = 0;
             int set = 0;
             if (!end) {
-                const int row = masked || state8 ? host_row_len[i] : 0;      // (moments in 32 bits without a mask: units of 64 whatever the shape)
+                const int row = masked || state8 ? host_row_len[i] : 0;
                 const bool pair = pairs(dtype, master, state8);
                 t.form = form_of(row, masked, pair);
                 t.row_len = (uint8_t)row;
@@ -1408,7 +1412,7 @@ extern "C" int gs_adamw_step(int n_tensors, const uint64_t *host_param, const ui
                        (q.step[set] != host_step[i] || memcmp(q.hyper[set], host_hyper + 5 * (size_t)i, 5 * sizeof(double)) != 0)) ++set;
             }
             if (q.b.n_tensors > 0 && (end || q.b.n_tensors == MAX_TENSORS || set == MAX_SETS ||
-                                      (long long)q.b.first_chunk[q.b.n_tensors] + chunks >= 0x7fffffffLL)) {
+                                      (long long)q.b.first_chunk[q.b.n_tensors] + chunks > MAX_CHUNKS)) {
                 q.b.device_scalars = on_device ? device_scalars : nullptr;
                 if (on_device) {
                     q.prep.n = q.b.n_tensors;
@@ -1467,12 +1471,14 @@ extern "C" int gs_read_moments(int n_tensors, const uint64_t *host_exp_avg, cons
         const int row = host_row_len[i];
         GS_REQUIRE(n >= 0 && n < (1LL << 46) && row >= 0 && row <= UNIT && (row == 0 || n % row == 0),
                    "gs_read_moments: numel in [0, 2^46), rows of 1..64 elements");
-        GS_REQUIRE(read_chunks(n, row, out_dtype, 1) < 0x7fffffffLL, "gs_read_moments: tensor too large");
         GS_REQUIRE(n == 0 || (host_exp_avg[i] && host_exp_avg_sq[i] && host_exponents[i] && host_m_out[i] && host_v_out[i]),
                    "gs_read_moments: null tensor");
         GS_REQUIRE(aligned_to(host_m_out[i] | host_v_out[i], element_bytes(out_dtype)), "gs_read_moments: misaligned output");
         units_of_16 += form_chunks(QUADS, n, row, 1, false, false);
     }
+    const int unroll = units_of_16 <= SMALL_CHUNKS ? 1 : UNROLL_READ;
+    for (int i = 0; i < n_tensors; ++i)
+        GS_REQUIRE(read_chunks(host_numel[i], host_row_len[i], out_dtype, unroll) <= MAX_CHUNKS, "gs_read_moments: tensor too large");
     {
         Range *r = (Range *)malloc((size_t)n_tensors * 5 * sizeof(Range));
         GS_REQUIRE(r != nullptr, "gs_read_moments: out of host memory");
@@ -1489,7 +1495,6 @@ extern "C" int gs_read_moments(int n_tensors, const uint64_t *host_exp_avg, cons
         free(r);
         GS_REQUIRE(!meet, "gs_read_moments: an output overlaps another buffer");
     }
-    const int unroll = units_of_16 <= SMALL_CHUNKS ? 1 : UNROLL_READ;
     MomentsBatch b;
     b.n_tensors = 0;
     b.first_chunk[0] = 0;
@@ -1504,7 +1509,7 @@ extern "C" int gs_read_moments(int n_tensors, const uint64_t *host_exp_avg, cons
                  (void *)host_m_out[i], (void *)host_v_out[i], host_numel[i], row};
             chunks = read_chunks(host_numel[i], row, out_dtype, unroll);
         }
-        if (b.n_tensors > 0 && (end || b.n_tensors == MAX_TENSORS || (long long)b.first_chunk[b.n_tensors] + chunks >= 0x7fffffffLL)) {
+        if (b.n_tensors > 0 && (end || b.n_tensors == MAX_TENSORS || (long long)b.first_chunk[b.n_tensors] + chunks > MAX_CHUNKS)) {
             if (unroll == 1) launch_moments<1>(out_dtype, b, (hipStream_t)stream);
             else launch_moments<UNROLL_READ>(out_dtype, b, (hipStream_t)stream);
             if (const int status = launch_status("gs_read_moments")) return status;

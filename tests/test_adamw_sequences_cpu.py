@@ -1,11 +1,14 @@
 """Sequences of calls of optim.AdamW that need no device: states that are loaded, masks that come and go, hooks.  The step itself
 is replaced by the plain one in 64 bits (adamw_plain.py); what it is handed is what is tested."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
 
-from taichi_3d_gaussian_splatting_amd import optim
+from taichi_3d_gaussian_splatting_amd import _lib, optim
 from tests import adamw_plain as plain
+from tests.test_adamw_cpu import _step
 
 HYPER = dict(lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2)
 
@@ -142,3 +145,31 @@ def test_options_that_a_saved_group_does_not_name_stay_the_groups_own(host_steps
     opt = optim.AdamW([dict(params=[p], state_bits=8)], lr=1e-3)
     opt.load_state_dict({"state": {}, "param_groups": torch.optim.AdamW([p]).state_dict()["param_groups"]})
     assert opt.param_groups[0]["state_bits"] == 8
+
+
+# Elements of the largest launch: gridDim.x * blockDim.x has to stay below 2^32, so 2^24 - 1 workgroups of 256 lanes, times what
+# a workgroup takes of each form
+WORKGROUPS = (1 << 24) - 1
+LARGEST = [(dict(), 1024), (dict(dtype=1), 1024), (dict(dtype=2, master=1 << 47), 1024), (dict(x=1 << 46), 4096), (dict(x=1 << 46, dtype=1), 4096),
+           (dict(x=1 << 46, dtype=1, row=56), 64 * 56), (dict(x=1 << 46, row=17), 128 * 17), (dict(x=1 << 46, row=2), 1024 * 2),
+           (dict(mask=1 << 46, last=1 << 47, row=56), 64 * 56), (dict(mask=1 << 46, last=1 << 47, row=1), 1024)]
+
+
+@pytest.mark.parametrize("change,share", LARGEST)
+def test_a_step_that_no_launch_holds_is_refused(change, share):
+    """At the limit the size is taken (what is said then is that these made-up buffers overlap), one row or element over it not."""
+    row = change.get("row", 1)
+    status, message = _step(numel=WORKGROUPS * share // row * row + row, **change)
+    assert status == -1 and "too large" in message, message
+    status, message = _step(numel=WORKGROUPS * share // row * row, **change)
+    assert status == -1 and "overlap" in message, message
+
+
+@pytest.mark.parametrize("dtype,row,share", [(0, 0, 4096), (1, 0, 4096), (1, 56, 64 * 56), (0, 56, 64 * 56), (0, 17, 128 * 17), (0, 3, 4096)])
+def test_a_reading_of_moments_that_no_launch_holds_is_refused(dtype, row, share):
+    lib = _lib.load()
+    for rows_more, says in ((1, "too large"), (0, "overlaps")):
+        n = WORKGROUPS * share // max(row, 1) * max(row, 1) + rows_more * max(row, 1)
+        columns = [(ctypes.c_uint64 * 1)(0x10000 * (i + 1)) for i in range(5)]
+        status = lib.gs_read_moments(1, *columns, (ctypes.c_int64 * 1)(n), (ctypes.c_int32 * 1)(row), dtype, None)
+        assert status == -1 and says in lib.gs_last_error().decode(), lib.gs_last_error()
