@@ -667,7 +667,9 @@ int gs_adam_step_rows(float *param, const float *grad, float *exp_avg, float *ex
  * else (row_len 0) 64 consecutive elements, the last block shorter.  What the bytes stand for:
  *   first moment:  c = 128 s + a:  (-1)^s * (a < 8 ? a 2^-9 : 2^((a >> 3) - 7) (1 + (a & 7) / 8)) * 2^(X_m - 135)
  *   second moment: c = 0: 0, else 2^(c >> 3) (1 + (c & 7) / 8) * 2^(X_v - 158)
- * X = 255: every element of the block is NaN.  X_m below 9 counts as 9, X_v below 32 as 32. */
+ * X = 255: every element of the block is NaN; a step writes it where a moment of the block is infinite or NaN.  Finite moments
+ * over 1.75 2^127 (the second: 1.875 2^127), the largest that X = 254 holds, are written as that.  X_m below 9 counts as 9, X_v
+ * below 32 as 32. */
 #define GS_DTYPE_F32 0
 #define GS_DTYPE_BF16 1
 #define GS_DTYPE_F16 2

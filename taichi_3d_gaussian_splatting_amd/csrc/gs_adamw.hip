@@ -171,25 +171,31 @@ __device__ __forceinline__ f32x4 units_of(uint32_t codes) {
 }
 
 // Exponent byte of a block from the bits of its largest magnitude (positive floats order like their bits, NaN above all):
-// `carry` moves values whose mantissa is over the largest code's to the next power, so that rounding up stays in range;
-// what has no finite value, or none below the largest power's end, makes 255.
+// `carry` moves values whose mantissa is over the largest code's to the next power, so that rounding up stays in range.  A finite
+// value makes 254 at most, what is infinite or NaN makes 255.
+constexpr uint32_t INF_BITS = 0x7F800000u;
 __device__ __forceinline__ uint32_t block_exponent(uint32_t largest, uint32_t carry, uint32_t low) {
-    return min(max((largest + carry) >> 23, low), 255u);
+    return max(min(largest + carry, max(largest, INF_BITS - 1u)) >> 23, low);
 }
 constexpr uint32_t CARRY_M = 0x1FFFFFu, CARRY_V = 0x0FFFFFu, LOW_M = 9u, LOW_V = 32u;
 
 // Code of a first moment, in the top byte of a word.  |m| 2^(15 - X) is a float whose bits, cut after the third mantissa
 // bit, are the code: float's own gradual underflow falls where the code's begins.  The 20 bits below meet 20 random ones:
-// the carry into the code has the chance that keeps the mean.
+// the carry into the code has the chance that keeps the mean.  Under X = 254 the largest code stands for 1.75 2^127, and finite
+// values beyond become that.  (A minimum an element: a branch for the rare blocks that need it parts the quads of a lane, and 1M
+// points took 230 us with it, 226 without.)
+constexpr uint32_t TOP_M = INF_BITS - 1u - CARRY_M;
 __device__ __forceinline__ uint32_t m_word(float m, uint32_t xm, uint32_t bits) {
-    const uint32_t u = (to_bits(ldexpf(fabsf(m), 15 - (int)xm)) + bits) << 4;
+    const uint32_t u = (to_bits(ldexpf(fminf(fabsf(m), from_bits(TOP_M)), 15 - (int)xm)) + bits) << 4;
     return (u & 0x7FFFFFFFu) | (to_bits(m) & 0x80000000u);
 }
 // Code of a second moment: v's bits less the block's base, rounded the same way; a value over zero stays over zero (it is a
-// divisor's square).  The difference is negative below the smallest code, and does not pass 2^28 above.
+// divisor's square), and 255 is the last.  The difference is negative below the smallest code, and does not pass 2^28 + 2^20 above.
 __device__ __forceinline__ uint32_t v_code(float v, uint32_t base, uint32_t bits) {
-    const int c = (int)(to_bits(v) - base + bits) >> 20;
-    return (uint32_t)max(c, (int)min(to_bits(v), 1u));
+    const int c = (int)(to_bits(v) - base + bits) >> 20, low = (int)min(to_bits(v), 1u);
+    int code;       // between low and 255, in one instruction
+    asm("v_med3_i32 %0, %1, %2, %3" : "=v"(code) : "v"(c), "v"(low), "s"(255));
+    return (uint32_t)code;
 }
 __device__ __forceinline__ uint32_t pack_top_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     return __builtin_amdgcn_perm(b, a, 0x0c0c0703u) | __builtin_amdgcn_perm(d, c, 0x07030c0cu);
@@ -614,7 +620,7 @@ __device__ __forceinline__ void step_quads_masked(const AdamwTensor &t, const Ad
 // is four elements although a row is not.  With codes of one quad only a lane has too little in flight: it takes rows at two places
 // (40M floats, rows of 1 / 2 / 4: 157 / 143 / 136 us at one, 145 / 134 / 127 at two, 152 / 140 / 132 at four; all live under a mask
 // 268 / 237 / 235, 210 / 179 / 164, 217 / 181 / 155).
-// 40M bfloat16 in rows of 1 / 2 / 3 / 4: 102 / 90 / 92 / 79 us, a row a lane and element by element 304 / 188 / 152 / 148.
+// 40M bfloat16 in rows of 1 / 2 / 3 / 4: 115 / 95 / 93 / 71 us, a row a lane and element by element 304 / 188 / 152 / 148.
 // Masked rows are not written, someone else may do so meanwhile: where some of a lane's rows are masked it stores the others row by
 // row.  40M floats under a mask, rows of 1 / 2 / 3, 32 bits, all live 262 / 233 / 243 us, half of them at random 342 / 261 / 290
 // (266 / 237 / 248 with whole quads, masked rows as they were read), 30 % 326 / 267 / 276; 8 bits 212 / 181 / 162,
@@ -780,10 +786,12 @@ __host__ __device__ inline long long form_chunks(int form, long long numel, int 
 
 // All tensors of one parameter type and one form of moments, whatever their shapes: the branches on `form` are uniform in a
 // workgroup.  Masked tensors have a kernel of their own, whose registers would cost the others occupancy.  Where pairs of quads
-// are bound by arithmetic, narrow rows of three would take 83 registers: at least six waves to a SIMD (40M bfloat16, rows of
-// 3 / 4 / 7 / 16 / 56: 92 / 79 / 103 / 83 / 71 us; five waves 81 / 84 / 110 / 91 / 74, seven 142 / 75 / 97 / 80 / 70).
+// are bound by arithmetic, narrow rows of three would take 83 registers: at least six waves to a SIMD, for which they spill 12 bytes a
+// lane (40M bfloat16, rows of 3 / 4 / 7 / 16 / 56: 92 / 79 / 103 / 83 / 71 us; five waves 81 / 84 / 110 / 91 / 74, seven
+// 142 / 75 / 97 / 80 / 70).  The other 8-bit forms: five; left alone the float one takes 97 registers and has four (1M points 226 us,
+// four waves 224; 40M floats in rows of 5 / 17: 130 / 146, four waves 135 / 153).
 template <int QUADS_A_LANE, int DT, bool MASTER, bool STATE8, bool MASKED>
-__global__ __launch_bounds__(GS_BLOCK, pairs(DT, MASTER, STATE8) ? 6 : 1) void adamw_kernel(AdamwBatch b) {
+__global__ __launch_bounds__(GS_BLOCK, pairs(DT, MASTER, STATE8) ? 6 : (STATE8 && !MASKED ? 5 : 1)) void adamw_kernel(AdamwBatch b) {
     const int ti = find_tensor<MAX_TENSORS>(b.first_chunk, b.n_tensors, blockIdx.x);
     const AdamwTensor &t = b.t[ti];
     AdamwScalars k = b.device_scalars ? b.device_scalars[ti] : b.scalars[t.set];

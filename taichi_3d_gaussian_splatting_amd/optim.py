@@ -211,7 +211,7 @@ def adamw_step_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], e
       with them.  8-bit moments are rounded at random so that their mean is kept (a code is 1/16 to 1/8 of its value, far more
       than a step moves the second moment): the bits are a hash of ``seed``, the tensor's id (``tensor_ids``, else its place in
       the list), its step and the element, so equal calls give equal results.  A block in which a moment is infinite or NaN
-      becomes NaN as a whole.
+      becomes NaN as a whole; finite ones at the end of float32's range (over 2.97e38) are held as the largest code.
     * ``masters``: float32 copies (or None) of 16-bit parameters; the step runs on the copy and the parameter receives its
       rounded value.  Without a copy the parameter itself is rounded to nearest, and steps below half its spacing are lost.
     * ``step``: this step's number (from 1), or a device tensor (int64, one element) that holds it when the kernels run;

@@ -101,3 +101,47 @@ def test_masked_rows_may_be_written_while_the_others_are_stepped(bits, columns):
         return written
     for got, want in zip(run(True), run(False)):
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype,masked", [(torch.float32, False), (torch.float32, True), (torch.bfloat16, False)])
+def test_finite_moments_at_the_end_of_float_stay_finite_in_8_bits(dtype, masked):
+    """Blocks whose largest moment is finite but over the largest code's value under the last exponent: that value is held, as
+    the format's tables say; infinite and NaN ones make 255.  With betas of zero the moments are the gradient and its square, which
+    gradients of few bits make exact."""
+    from tests import adamw_plain as plain
+    o = _optim()
+    shapes = [(40, 56), (40, 17), (40, 5), (41, 1), (41, 2), (41, 3), (41, 4), (40, 64)] + ([] if masked else [(1000,), (30, 65)])
+    gen = torch.Generator().manual_seed(3)
+    edge_v = [2.0 ** 63.5, 1.9 * 2.0 ** 63, 1.4 * 2.0 ** 63, 1.36 * 2.0 ** 63]      # squares about 2^127 (1 .. 2), the top code 1.875
+    edge_m = [1.99 * 2.0 ** 127, 1.76 * 2.0 ** 127, 1.75 * 2.0 ** 127, -1.9 * 2.0 ** 127]
+    over_v = [1.98 * 2.0 ** 63, 1.95 * 2.0 ** 63, 1.93 * 2.0 ** 63]                 # squares of 1.86 .. 1.97 times 2^127
+    for edge in (over_v, edge_v[2:], edge_m, [float("inf")], [float("nan")], [edge_v[0], edge_v[3]]):
+        grads = []
+        for s in shapes:
+            g = torch.randn(s, generator=gen)
+            at = torch.rand(s, generator=gen) < 0.05
+            g = g * abs(edge[0] if np.isfinite(edge[0]) else 1.0) * 0.3
+            g[at] = torch.tensor(edge)[torch.randint(len(edge), (int(at.sum()),), generator=gen)]
+            # (seven bits of mantissa: exact in bfloat16, squares exact in float32)
+            grads.append(g.to(torch.bfloat16).to(dtype).to(DEV))
+        params = [torch.zeros(s, dtype=dtype, device=DEV) for s in shapes]
+        ms, vs, xs = zip(*[o.new_moments(p, 8) for p in params])
+        more = {}
+        if masked:
+            masks = [torch.zeros(s[0], dtype=torch.int8, device=DEV) for s in shapes]
+            for mask in masks:
+                mask[1::5] = 1
+            more = dict(row_masks=masks, last_steps=[torch.zeros(s[0], dtype=torch.int32, device=DEV) for s in shapes])
+        o.adamw_step_(params, grads, ms, vs, step=1, exponents=xs, betas=(0.0, 0.0), lr=0.0, weight_decay=0.0, seed=6, **more)
+        for i, s in enumerate(shapes):
+            g = grads[i].double().cpu().numpy()
+            with np.errstate(over="ignore", invalid="ignore"):
+                mc, vc, x, _ = plain.encode(g, g * g, plain.noise(g.size, 6, i, 1), s)
+            if masked:
+                rows = (more["row_masks"][i] != 0).cpu().numpy()
+                mc[rows], vc[rows], x[rows] = 0, 0, 0
+            assert np.array_equal(xs[i].cpu().numpy(), x), (edge, s)
+            assert np.array_equal(ms[i].cpu().numpy() % 128, mc % 128) and np.array_equal(vs[i].cpu().numpy(), vc), (edge, s)
+            m, v = o.read_moments([ms[i]], [vs[i]], [xs[i]])
+            assert np.array_equal(torch.isfinite(m[0]).cpu().numpy(), (x[:, 0] != 255)[plain.blocks_of(s)[0]].reshape(s))
+            assert np.array_equal(torch.isfinite(v[0]).cpu().numpy(), (x[:, 1] != 255)[plain.blocks_of(s)[0]].reshape(s))
