@@ -453,15 +453,16 @@ class AdamW(torch.optim.Optimizer):
         return norms[1]
 
     def moments(self, param: torch.Tensor, dtype: torch.dtype = torch.float32) -> Tuple[torch.Tensor, torch.Tensor]:
-        """Copies of a parameter's first and second moment, whatever they are held in (of rows that miss steps under a row mask:
-        as of the last step that reached them)."""
+        """Copies of a parameter's first and second moment in any type, whatever they are held in (of rows that miss steps under a
+        row mask: as of the last step that reached them)."""
         state = self.state.get(param)
         if not state:
             raise KeyError("the parameter has no state yet")
         if "exponents" not in state:
             return state["exp_avg"].to(dtype, copy=True), state["exp_avg_sq"].to(dtype, copy=True)
-        m, v = read_moments([state["exp_avg"]], [state["exp_avg_sq"]], [state["exponents"]], dtype=dtype)
-        return m[0], v[0]
+        held = [state["exp_avg"]], [state["exp_avg_sq"]], [state["exponents"]]
+        (m,), (v,) = read_moments(*held, dtype=dtype if dtype == torch.bfloat16 else torch.float32)
+        return m.to(dtype), v.to(dtype)
 
     _OPTIONS = ("master_weights", "max_grad_norm", "norm_group", "capturable", "seed", "last_grad_norm")
 

@@ -145,3 +145,16 @@ def test_finite_moments_at_the_end_of_float_stay_finite_in_8_bits(dtype, masked)
             m, v = o.read_moments([ms[i]], [vs[i]], [xs[i]])
             assert np.array_equal(torch.isfinite(m[0]).cpu().numpy(), (x[:, 0] != 255)[plain.blocks_of(s)[0]].reshape(s))
             assert np.array_equal(torch.isfinite(v[0]).cpu().numpy(), (x[:, 1] != 255)[plain.blocks_of(s)[0]].reshape(s))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16, torch.float64])
+def test_moments_are_read_in_any_type_whatever_they_are_held_in(bits, dtype):
+    o = _optim()
+    p = torch.nn.Parameter(torch.zeros(100, 56, device=DEV))
+    opt = o.AdamW([p], state_bits=bits)
+    p.grad = torch.randn(100, 56, device=DEV)
+    opt.step()
+    want = [x.to(dtype) for x in opt.moments(p)]
+    for got, value in zip(opt.moments(p, dtype), want):
+        assert got.dtype == dtype and torch.equal(got, value)
