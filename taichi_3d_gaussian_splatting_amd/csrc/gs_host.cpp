@@ -275,6 +275,14 @@ PyObject *tuple_of(PyObject *o, Py_ssize_t n) {
     return o;
 }
 
+// A graph that has kept one of these tensors for its backward pass must notice that it changed, as after any operation in place.
+void count_as_changed(PyObject *tensors) {
+    for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(tensors); ++i) {
+        PyObject *t = PySequence_Fast_GET_ITEM(tensors, i);
+        if (THPVariable_Check(t) && !THPVariable_Unpack(t).is_inference()) THPVariable_Unpack(t).unsafeGetTensorImpl()->bump_version();
+    }
+}
+
 // step(collected, scalars, ids or None, grad scale address, seed, workspace address, stream): status of gs_adamw_step.
 // `collected`: params, grads, exp_avgs, exp_avg_sqs, exponents, masters, row masks, last steps.
 PyObject *step(PyObject *args) {
@@ -303,12 +311,7 @@ PyObject *step(PyObject *args) {
                                   column<U>(c, 6), column<U>(c, 7), column<int64_t>(collected, 1), column<int32_t>(collected, 2), column<int32_t>(collected, 3),
                                   id.data(), column<double>(numbers, 0), column<int64_t>(numbers, 1), column<U>(numbers, 2), column<U>(numbers, 3),
                                   (const float *)scale, seed, (void *)workspace, (void *)stream);
-    // A graph that has kept a parameter for its backward pass must notice that it changed, as after any operation in place.
-    PyObject *params = PyList_GET_ITEM(PyTuple_GET_ITEM(collected, 5), 0);
-    for (Py_ssize_t i = 0; status == 0 && i < PySequence_Fast_GET_SIZE(params); ++i) {
-        PyObject *p = PySequence_Fast_GET_ITEM(params, i);
-        if (THPVariable_Check(p) && !THPVariable_Unpack(p).is_inference()) THPVariable_Unpack(p).unsafeGetTensorImpl()->bump_version();
-    }
+    if (status == 0) count_as_changed(PyList_GET_ITEM(PyTuple_GET_ITEM(collected, 5), 0));
     return PyLong_FromLong(status);
 }
 
@@ -331,11 +334,14 @@ PyObject *read(PyObject *args) {
     int dtype;
     unsigned long long stream;
     if (!PyArg_ParseTuple(args, "OiK", &collected, &dtype, &stream)) return nullptr;
-    PyObject *c = tuple_of(PyTuple_GET_ITEM(tuple_of(collected, 4), 0), 5);
+    PyObject *c = tuple_of(PyTuple_GET_ITEM(tuple_of(collected, 6), 0), 5);
     if (!read_moments) throw Refused{PyExc_RuntimeError, "the library is not bound"};
     typedef uint64_t U;
-    return PyLong_FromLong(read_moments((int)(PyBytes_GET_SIZE(PyTuple_GET_ITEM(collected, 1)) / 8), column<U>(c, 0), column<U>(c, 1), column<U>(c, 2),
-                                        column<U>(c, 3), column<U>(c, 4), column<int64_t>(collected, 1), column<int32_t>(collected, 2), dtype, (void *)stream));
+    const int status = read_moments((int)(PyBytes_GET_SIZE(PyTuple_GET_ITEM(collected, 1)) / 8), column<U>(c, 0), column<U>(c, 1), column<U>(c, 2),
+                                    column<U>(c, 3), column<U>(c, 4), column<int64_t>(collected, 1), column<int32_t>(collected, 2), dtype, (void *)stream);
+    PyObject *kept = PyTuple_GET_ITEM(collected, 5);        // (the five lists, in their order)
+    for (Py_ssize_t k = 3; status == 0 && k < 5; ++k) count_as_changed(PyList_GET_ITEM(kept, k));
+    return PyLong_FromLong(status);
 }
 
 template <PyObject *(*F)(PyObject *)>

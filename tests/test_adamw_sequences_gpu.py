@@ -158,3 +158,17 @@ def test_moments_are_read_in_any_type_whatever_they_are_held_in(bits, dtype):
     want = [x.to(dtype) for x in opt.moments(p)]
     for got, value in zip(opt.moments(p, dtype), want):
         assert got.dtype == dtype and torch.equal(got, value)
+
+
+def test_a_graph_that_kept_what_moments_are_read_into_notices():
+    o = _optim()
+    m, v, x = o.new_moments(torch.zeros(640, device=DEV), 8)
+    out = [torch.randn(640, device=DEV) for _ in range(2)]
+    w = torch.ones(640, device=DEV, requires_grad=True)
+    y = [(w * t).sum() for t in out]
+    before = [t._version for t in out + [m, v, x]]
+    o.read_moments([m], [v], [x], out=([out[0]], [out[1]]))
+    assert [t._version for t in out] == [b + 1 for b in before[:2]] and [t._version for t in (m, v, x)] == before[2:]
+    for t in y:
+        with pytest.raises(RuntimeError, match="inplace operation"):
+            t.backward()
