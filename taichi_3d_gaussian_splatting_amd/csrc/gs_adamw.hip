@@ -1372,7 +1372,7 @@ extern "C" int gs_adamw_step(int n_tensors, const uint64_t *host_param, const ui
         GS_REQUIRE(form_chunks(form_of(row, masked, pair), host_numel[i], row, unroll, pair, state8) <= MAX_CHUNKS, "gs_adamw_step: tensor too large");
     }
     {
-        Range *r = (Range *)malloc((size_t)n_tensors * 8 * sizeof(Range));
+        Range *r = (Range *)malloc(((size_t)n_tensors * 10 + 1) * sizeof(Range));
         GS_REQUIRE(r != nullptr, "gs_adamw_step: out of host memory");
         size_t k = 0;
         for (int i = 0; i < n_tensors; ++i) {
@@ -1388,7 +1388,10 @@ extern "C" int gs_adamw_step(int n_tensors, const uint64_t *host_param, const ui
                 r[k++] = {host_last_step[i], host_last_step[i] + 4 * blocks, 1};
                 r[k++] = {host_row_mask[i], host_row_mask[i] + blocks, 0};
             }
+            if (entry(host_step_device, i)) r[k++] = {host_step_device[i], host_step_device[i] + 8, 0};
+            if (entry(host_lr_device, i)) r[k++] = {host_lr_device[i], host_lr_device[i] + 4, 0};
         }
+        if (grad_scale) r[k++] = {(u64)(uintptr_t)grad_scale, (u64)(uintptr_t)grad_scale + 4, 0};
         const bool meet = ranges_meet(r, k);
         free(r);
         GS_REQUIRE(!meet, "gs_adamw_step: buffers overlap");

@@ -173,3 +173,22 @@ def test_a_reading_of_moments_that_no_launch_holds_is_refused(dtype, row, share)
         columns = [(ctypes.c_uint64 * 1)(0x10000 * (i + 1)) for i in range(5)]
         status = lib.gs_read_moments(1, *columns, (ctypes.c_int64 * 1)(n), (ctypes.c_int32 * 1)(row), dtype, None)
         assert status == -1 and says in lib.gs_last_error().decode(), lib.gs_last_error()
+
+
+@pytest.mark.parametrize("change", [dict(step_dev=0x10010, ws=0x90000), dict(lr_dev=0x30000, ws=0x90000), dict(step_dev=0x40000 - 4, ws=0x90000),
+                                    dict(lr_dev=0x50000, x=0x50000, ws=0x90000)])
+def test_device_scalars_inside_written_buffers_are_refused(change):
+    """The kernels read them while they write there."""
+    status, message = _step(**change)
+    assert status == -1 and "overlap" in message, message
+
+
+def test_a_gradient_scale_inside_a_written_buffer_is_refused():
+    u64 = ctypes.c_uint64
+    lib = _lib.load()
+    columns = [(u64 * 1)(x) for x in (0x10000, 0x20000, 0x30000, 0x40000)]
+    for scale in (0x10000, 0x30000 + 4 * 63, 0x40010):
+        status = lib.gs_adamw_step(1, *columns, None, None, None, None, (ctypes.c_int64 * 1)(64), (ctypes.c_int32 * 1)(0), (ctypes.c_int32 * 1)(0),
+                                   (ctypes.c_int32 * 1)(0), (ctypes.c_double * 5)(1e-3, 0.9, 0.999, 1e-8, 0.0), (ctypes.c_int64 * 1)(1), None, None,
+                                   scale, 0, None, None)
+        assert status == -1 and "overlap" in lib.gs_last_error().decode(), (hex(scale), lib.gs_last_error())
