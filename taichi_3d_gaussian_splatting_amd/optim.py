@@ -149,6 +149,14 @@ def _stream(device_index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(device_index)
 
 
+def _capturing(device_index: int) -> bool:
+    """Whether the device's current stream is being captured into a graph (a host tensor's, -1, never is)."""
+    if device_index < 0:
+        return False
+    with _on(device_index):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _norm_of(host, collected, grads, masks, max_norm: float, each: bool, group=None) -> torch.Tensor:
     """[norm, clip, each ...] of collected gradients, on their device's current stream."""
     index = collected[4]
@@ -253,7 +261,7 @@ def adamw_step_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], e
     if grad_scale is not None and (grad_scale.get_device() != index or grad_scale.dtype is not torch.float32 or grad_scale.numel() != 1):
         raise ValueError("grad_scale: one float32 on the parameters' device")
     numbers = host.scalars(n, step, lr, weight_decay, beta1, beta2, eps, index)
-    if numbers[4] and torch.cuda.is_current_stream_capturing():
+    if numbers[4] and _capturing(index):
         raise RuntimeError("a captured step needs its step count in a device tensor: a number would be the same at every replay")
 
     norms, clip = None, 0
@@ -428,7 +436,7 @@ class AdamW(torch.optim.Optimizer):
         """The state of a parameter that has none, or none for its row mask yet."""
         if not state and not p.is_cuda:
             raise RuntimeError("optim.AdamW needs parameters on the HIP device: there is no CPU path")
-        if torch.cuda.is_current_stream_capturing():
+        if _capturing(p.get_device()):
             raise RuntimeError("run one step of AdamW before capturing one: its state is made there")
         if not state:
             state.update(self._new_state(p, group))
@@ -439,7 +447,7 @@ class AdamW(torch.optim.Optimizer):
     def _no_row_masked(self, p: torch.Tensor) -> torch.Tensor:
         """For a parameter whose state comes from steps under a row mask and that has no mask now: one that lets every row take
         this step, late ones with their decay.  The stamps end with it: the steps after it would not keep them."""
-        if torch.cuda.is_current_stream_capturing():
+        if _capturing(p.get_device()):
             raise RuntimeError("run one step of AdamW before capturing one: rows that an earlier mask held back take it there")
         return torch.zeros(p.shape[0], dtype=torch.int8, device=p.device)
 

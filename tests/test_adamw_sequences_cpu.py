@@ -192,3 +192,26 @@ def test_a_gradient_scale_inside_a_written_buffer_is_refused():
                                    (ctypes.c_int32 * 1)(0), (ctypes.c_double * 5)(1e-3, 0.9, 0.999, 1e-8, 0.0), (ctypes.c_int64 * 1)(1), None, None,
                                    scale, 0, None, None)
         assert status == -1 and "overlap" in lib.gs_last_error().decode(), (hex(scale), lib.gs_last_error())
+
+
+def test_whether_a_graph_is_captured_is_asked_on_the_parameters_device(monkeypatch):
+    """A step with a number for its count, of tensors on another device than the current one, whose stream is being captured."""
+    import contextlib
+    entered = []
+
+    @contextlib.contextmanager
+    def on(index):
+        entered.append(index)
+        yield
+        entered.pop()
+
+    class Host:
+        PARAM = GRAD = FLOAT = CODE = EXPONENTS = MASTER = PARAM_MASK = STAMP = 0
+        collect = staticmethod(lambda *lists: ((None,) * 8, b"", b"", b"", 1, []))
+        scalars = staticmethod(lambda *numbers: (b"", b"", None, None, True))
+    monkeypatch.setattr(optim, "_on", on)
+    monkeypatch.setattr(optim._lib, "host", Host)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: entered == [1])
+    one = [torch.zeros(8)]
+    with pytest.raises(RuntimeError, match="same at every replay"):
+        optim.adamw_step_(one, one, one, one, step=1)
