@@ -364,10 +364,12 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         work = self._work()
         if not work:
-            if self.max_grad_norm is not None and self.norm_group is not None:     # (the other ranks wait for this one's share)
-                share = torch.zeros(1, dtype=torch.float64, device=self.param_groups[0]["params"][0].device)
-                _sum_over_ranks(share, self.norm_group)
-                self.last_grad_norm = share.sqrt().float()[0]
+            if self.max_grad_norm is not None:
+                device = next(p.device for group in self.param_groups for p in group["params"])
+                share = torch.zeros((), dtype=torch.float64, device=device)
+                if self.norm_group is not None:     # (the other ranks wait for this one's share)
+                    _sum_over_ranks(share, self.norm_group)
+                self.last_grad_norm = share.sqrt().float()
             return loss
         clip = None
         if self.max_grad_norm is not None:

@@ -215,3 +215,14 @@ def test_whether_a_graph_is_captured_is_asked_on_the_parameters_device(monkeypat
     one = [torch.zeros(8)]
     with pytest.raises(RuntimeError, match="same at every replay"):
         optim.adamw_step_(one, one, one, one, step=1)
+
+
+def test_no_norm_stays_from_a_step_before_where_no_parameter_has_a_gradient():
+    p = torch.nn.Parameter(torch.zeros(4))
+    opt = optim.AdamW([p], max_grad_norm=1.0)
+    opt.last_grad_norm = torch.tensor(3.0)
+    opt.step()
+    assert float(opt.last_grad_norm) == 0.0 and opt.last_grad_norm.dtype == torch.float32 and opt.last_grad_norm.shape == ()
+    opt = optim.AdamW([p])
+    opt.step()
+    assert opt.last_grad_norm is None
