@@ -366,10 +366,10 @@ class AdamW(torch.optim.Optimizer):
         if not work:
             if self.max_grad_norm is not None:
                 device = next(p.device for group in self.param_groups for p in group["params"])
-                share = torch.zeros((), dtype=torch.float64, device=device)
+                share = torch.zeros(1, dtype=torch.float64, device=device)
                 if self.norm_group is not None:     # (the other ranks wait for this one's share)
                     _sum_over_ranks(share, self.norm_group)
-                self.last_grad_norm = share.sqrt().float()
+                self.last_grad_norm = share.sqrt().float()[0]
             return loss
         clip = None
         if self.max_grad_norm is not None:
