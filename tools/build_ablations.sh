@@ -7,17 +7,17 @@
 set -e
 ROOT=$(cd "$(dirname "$0")/.." && pwd)
 SRC=$ROOT/taichi_3d_gaussian_splatting_amd/csrc
+OUT=${GS_VARIANTS_DIR:-$ROOT/variants}
 TMP=$(mktemp -d)
-mkdir -p $TMP/pkg $ROOT/variants
-cp -r $SRC $TMP/pkg/csrc && cp -r $ROOT/include $TMP/include
+mkdir -p $TMP/pkg $OUT
+cp -rp $SRC $TMP/pkg/csrc && cp -rp $ROOT/include $TMP/include     # (with their times: what is built there stays built here)
 patch -s $TMP/pkg/csrc/gs_frontend.hip $ROOT/tools/ubench/frontend_ablation.patch
-make -s -C $SRC > /dev/null
 cd $TMP/pkg/csrc
 for spec in "k1:-DGS_ABLATE_KEYS=1" "k2:-DGS_ABLATE_KEYS=2" "k3:-DGS_ABLATE_KEYS=3" "p1:-DGS_ABLATE_PRE=1" "p2:-DGS_ABLATE_PRE=2" "p3:-DGS_ABLATE_PRE=3"; do
     tag=${spec%%:*}; flags=${spec#*:}
-    /opt/rocm/bin/hipcc -O3 -std=c++17 --offload-arch=gfx950 -fPIC -munsafe-fp-atomics -Wno-unused-function $flags -c gs_frontend.hip -o $TMP/fe_$tag.o
-    /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC $SRC/gs_api.o $SRC/gs_frame.o $TMP/fe_$tag.o $SRC/gs_sort.o $SRC/gs_blend.o \
-        $SRC/gs_shard.o $SRC/gs_point_backward.o $SRC/gs_controller.o $SRC/gs_loss.o $SRC/gs_optim.o -o $ROOT/variants/libgsplat_hip_abl_$tag.so
+    rm -f gs_frontend.o
+    make -s -j8 EXTRA="$flags" ../libgsplat_hip.so
+    cp ../libgsplat_hip.so $OUT/libgsplat_hip_abl_$tag.so
     echo "built $tag ($flags)"
 done
 rm -rf $TMP

@@ -6,11 +6,9 @@ import os, re, subprocess, sys, tempfile
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 name, extra = sys.argv[1], sys.argv[2:]
 src = os.path.join(ROOT, "taichi_3d_gaussian_splatting_amd", "csrc", name + ".hip")
-per_file = ["-fno-slp-vectorize"] if name in ("gs_frontend", "gs_point_backward") else []
+flags = subprocess.check_output(["make", "-s", "-C", os.path.dirname(src), "flags-" + name], text=True).split()
 with tempfile.TemporaryDirectory() as tmp:
-    subprocess.run(["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "--offload-arch=gfx950", "-fPIC", "-munsafe-fp-atomics",
-                    "-Wno-unused-function", "-I" + os.path.join(ROOT, "include"), *per_file, *extra, "-c", src, "--save-temps",
-                    "-o", "x.o"], cwd=tmp, check=True, stderr=subprocess.DEVNULL)
+    subprocess.run([os.environ.get("HIPCC", "/opt/rocm/bin/hipcc"), *flags, *extra, "-c", src, "--save-temps", "-o", "x.o"], cwd=tmp, check=True, stderr=subprocess.DEVNULL)
     asm = open(os.path.join(tmp, f"{name}-hip-amdgcn-amd-amdhsa-gfx950.s")).read()
     keep = os.environ.get("KEEP_ASM")
     if keep:
