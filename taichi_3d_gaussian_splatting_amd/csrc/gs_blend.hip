@@ -6,7 +6,7 @@
 // gs_entry_in_tile) with an ORDER-PRESERVING compaction (wave ballots + mbcnt) and stages up to 128 packed records
 // (16-B gathers) in LDS per blend round -- the sequence a tile blends is exactly the reference's per-tile list.
 //  forward : front-to-back blend (RAS:318-485, weight UTL:275-284); 2 waves per tile, two pixels per lane
-//            on packed fp32 math; whole-tile early exit with a workgroup vote (the reference could not
+//            in pairs of floats; whole-tile early exit with a workgroup vote (the reference could not
 //            express it, RAS:387-394).  With a binned layout it also writes out the entries each tile keeps
 //            (walked_list): the backward pass then walks plain per-tile lists and never filters a bin list again.
 //  backward: back-to-front traversal (RAS:531-705, gradients UTL:331-348) starting at the tile's last
@@ -168,8 +168,8 @@ __device__ __forceinline__ TileCoord owned_tile_at(int b, int nb, int tw, int ro
 
 // ------------------------------------------------------------------------------- the Gaussian weight
 // Workgroup = one tile = 2 wave64s; every lane owns TWO horizontally adjacent pixels and does its fp32 arithmetic on float2
-// values, which the compiler maps to the packed CDNA instructions (v_pk_add_f32 / v_pk_mul_f32 / v_pk_fma_f32: two pixels
-// per VALU issue).
+// values: two plain instructions each (the library is built without packed fp32 instructions, csrc/Makefile; one of them takes
+// as long as two plain ones).
 typedef float v2f __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ v2f fma2(v2f a, v2f b, v2f c) { return __builtin_elementwise_fma(a, b, c); }
 __device__ __forceinline__ v2f splat(float x) { return (v2f){x, x}; }
@@ -185,17 +185,17 @@ constexpr float GS_LOG2E = 1.4426950408889634f;
 //   skips the pair for certain (float 14: gs_common.h, "the 1/255 decision in the exponent's domain"); s_hi = -2 e_lo, the same
 //   bound on the backward pass' quadratic form s = -2 e.  Forward: the second half of Q and the colour row are read on the
 //   hit path only.
-//   (C, which the packed arithmetic only ever uses as a per-lane scalar, sits in the one position -- the upper half of the
-//   second register pair -- from which the compiler will not broadcast without a v_mov)
+//   (C sits in the upper half of the second register pair, from which packed arithmetic could not have broadcast it; plain
+//   instructions read it anywhere)
 // THE EXPONENT IS THE REFERENCE'S TO THE LAST BIT (gs_common.h, "threshold decisions"): each pass evaluates the quadratic
 // form in the operation order of its counterpart, contraction off (this file) --
 //   forward  UTL:281-283   e = -0.5 * (dx*dx*A + dy*dy*C) - dx*dy*B        (the final fma rounds once, as the reference's
 //                                                                           subtraction does: -0.5 * t is exact)
 //   backward UTL:336-339   m = conic @ d,  e = -0.5 * (dx*m0 + dy*m1)      (m is also what the gradients need, UTL:343-346)
-// -- and alpha = 2^(e * log2 e) * amp: four packed instructions more per pixel pair than the pre-scaled log2-domain form of
+// -- and alpha = 2^(e * log2 e) * amp: four operations more per pixel than the pre-scaled log2-domain form of
 // rounds 1-4 (two in the backward pass, which gets m for free), for an alpha within u (2 |e| + 9) of the reference's
 // whatever the conic, instead of 9 u times the cancellation inside the quadratic form.
-// Round 6: the exponent is compared with e_lo FIRST, and the exponential (two v_exp_f32 and two packed products per pixel
+// Round 6: the exponent is compared with e_lo FIRST, and the exponential (two v_exp_f32 and four products per pixel
 // pair: 14 of the 35 ns a visit without a hit cost the SIMD) is evaluated on the hit path only -- a quarter of the (wave,
 // entry) visits never get there.
 __device__ __forceinline__ v2f gs_weight_from_exponent(v2f e, float amp) {
@@ -1050,7 +1050,7 @@ __global__ __launch_bounds__(BLEND_THREADS, GS_BWD_MIN_WAVES) void blend_backwar
                     qa = src[0]; qb = src[1]; qc = src[2]; qd = src[3];
                     __builtin_amdgcn_wave_barrier();   // (this entry's stores stay below these reads)
                 }
-                v2f pq[11];   // the eleven packed (two-pixel) partials of this entry
+                v2f pq[11];   // the eleven partials (two pixels each) of this entry
                 {
                     // alpha = 0 for a pixel that is not hit makes its whole update an exact no-op
                     // (1/(1-0) = 1, a*T = 0); only dL/dalpha needs an explicit mask.
@@ -1086,8 +1086,8 @@ __global__ __launch_bounds__(BLEND_THREADS, GS_BWD_MIN_WAVES) void blend_backwar
                     pq[0] = v0; pq[1] = v1; pq[2] = c00; pq[3] = c01; pq[4] = c11; pq[5] = gr; pq[6] = gg; pq[7] = gb;
                     pq[8] = w; pq[9] = nv; pq[10] = h;
                 }
-                // in-lane sums over the lane's two pixels (inline asm: the vectoriser would otherwise shuffle the operands
-                // into v_pk_add_f32 pairs with more moves than it saves adds)
+                // in-lane sums over the lane's two pixels (inline asm: where packed additions are allowed, the vectoriser
+                // shuffles the operands into pairs with more moves than it saves adds)
                 // (value 9 -- the two square roots -- is added by the compiler: a transcendental result needs a wait state before
                 // another VALU instruction reads it, and the hazard recogniser does not look inside an asm statement: scheduled
                 // straight behind v_sqrt_f32 the asm form read a stale register once in ~30 hit entries, REDUCE 4's schedule)
@@ -1500,8 +1500,8 @@ __global__ __launch_bounds__(GS_WAVE, GS_BWD_WIDE_MIN_WAVES) void blend_backward
                         w_.dc1 += hit1 ? 1u : 0u; w_.dh1 += hit1 ? hv : 0u;
                     }
                     const v2f pq[GS_TR_ROWS] = {v0, v1, c00, c01, c11, gr, gg, gb, wv, nv, hm};
-                    // (inline asm: left to itself the vectoriser shuffles the operands into v_pk_add_f32 pairs -- fifteen moves for
-                    // five packed adds; the leading s_nop covers the transcendental results of value 9, which the hazard
+                    // (inline asm: where packed additions are allowed, the vectoriser shuffles the operands into pairs -- fifteen moves
+                    // for five additions; the leading s_nop covers the transcendental results of value 9, which the hazard
                     // recogniser cannot see an asm statement read)
 #pragma unroll
                     for (int n = 0; n < GS_TR_ROWS; ++n) {
@@ -1580,8 +1580,7 @@ __global__ __launch_bounds__(GS_WAVE, GS_BWD_WIDE_MIN_WAVES) void blend_backward
 // two of its CU's four SIMDs and the launch lasts as long as the longest list (10k Gaussians at 256 x 256: 256 tiles, 96 +
 // 146 us in the two kernels above).  These arms give a tile FOUR waves -- one pixel per lane, so a list entry costs a wave
 // about half the issue slots of the two-pixel form -- for per-tile lists taken as they are (bin_shift 0, no filter: what
-// small frames use).  Per pixel they execute the same IEEE operations in the same order as the two-pixel kernels (packed
-// instructions are per-component), so image, depth, counts, state and hit decisions are bit-identical; the backward's slot
+// small frames use).  Per pixel they execute the same IEEE operations in the same order as the two-pixel kernels, so image, depth, counts, state and hit decisions are bit-identical; the backward's slot
 // sums add the same per-pixel terms in another order (four waves of 64 pixels instead of two of 128).
 constexpr int SMALL_THREADS = 256;
 #ifndef GS_SMALL_GRID_TILES

@@ -110,7 +110,7 @@ __device__ __forceinline__ float gs_exp_cr(float xf) {
 //     delta_i a_i / (1 - a_i) + 4 u (two roundings per side once the inputs differ), delta_i = u (2 ln(1 / a_i) + 9):
 //       a ln(1/a) / (1 - a) <= min(1, 6 a) on [1/255, 0.99] (and for a clamped factor)      -> 2 u * 6 a_i
 //       a / (1 - a) <= a H_k,  H_k = 1 / (1 - min(amp_k, 0.99)) -- per GAUSSIAN: alpha <= amp    -> 9 u * H_k a_i
-//     accumulated PER PIXEL with one packed FMA per hit-path execution: thr += W_k a_i, W_k = gs_stop_weight(amp_k) (stored
+//     accumulated PER PIXEL with one FMA per hit-path execution: thr += W_k a_i, W_k = gs_stop_weight(amp_k) (stored
 //     in the record), thr = upper edge of the pixel's bracket around 1e-4; the rounding term (4 u per blended Gaussian) is
 //     added per batch from the list positions walked (gates the rare path) and replaced by the pixel's own count inside it.
 //     thr = STOP (1 + 1.1 beta) >= STOP e^beta holds for beta <= 0.19; here beta <= 4/3 u (12 + 9 * 101) sum(a_i) < 1.2e-3
