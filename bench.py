@@ -54,6 +54,7 @@ import hashlib
 import json
 import math
 import os
+import re
 import sys
 import time
 
@@ -66,7 +67,7 @@ if ROOT not in sys.path:
 HBM_PEAK_GBS = 8000.0  # /opt/skills/guides/MI355X_MICROARCH.md: HBM3E 8.0 TB/s spec
 # VALU issue ceiling: 256 CUs x 4 SIMD-32, one wave64 fp32 instruction per 2 cycles per SIMD at 2.4 GHz
 VALU_PEAK_WAVE_INSTR_PER_S = 256 * 4 * 2.4e9 / 2.0
-PROFILE_TAG = "r06"
+PROFILE_TAG = "frame"
 # Warm-up floor (ms of continuous load before the timed region; profiles/r05_clock_ramp.txt): the W warm-up steps are
 # followed by untimed steps until the GPU has been under this load that long.  0 = exactly W steps.
 WARMUP_FLOOR_MS = float(os.environ.get("GS_BENCH_WARMUP_FLOOR_MS", "40"))
@@ -93,14 +94,21 @@ def algorithmic_bytes(n, m, k, p, key_bytes=8, k_tile=None):
     }
 
 
-def kernel_source_hash() -> str:
-    """sha256 over the HIP sources (the profile summaries record the hash they were taken with)."""
+# Files of csrc without a kernel that runs in a frame: optimisers and the loss.
+OUTSIDE_THE_FRAME = ("gs_adamw.hip", "gs_optim.hip", "gs_loss.hip")
+
+
+def kernel_source_hash(csrc: str = os.path.join(ROOT, "taichi_3d_gaussian_splatting_amd", "csrc")) -> str:
+    """sha256 over the HIP sources of the frame's kernels and the flags that they are compiled with (the profile summaries
+    record the hash they were taken with; other operators of the library do not make them stale)."""
     h = hashlib.sha256()
-    csrc = os.path.join(ROOT, "taichi_3d_gaussian_splatting_amd", "csrc")
     for name in sorted(os.listdir(csrc)):
-        if name.endswith((".hip", ".h")):
+        if name.endswith((".hip", ".h")) and name not in OUTSIDE_THE_FRAME:
             with open(os.path.join(csrc, name), "rb") as fh:
                 h.update(name.encode() + b"\0" + fh.read())
+    with open(os.path.join(csrc, "Makefile")) as fh:
+        for flags in re.findall(r"^(?:ARCH|FLAGS\w*)\s*[:?]?=(?:.*\\\n)*.*$", fh.read(), re.M):
+            h.update(" ".join(flags.replace("\\\n", " ").split()).encode() + b"\0")
     return h.hexdigest()[:16]
 
 

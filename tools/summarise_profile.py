@@ -68,7 +68,7 @@ json.dump(bench, open(os.path.join(dst, f"{name}_bench_lines.json"), "w"), inden
 hashes = {b.get("roofline", {}).get("kernel_source_hash") for b in bench.values()}
 if len(hashes) == 1 and None not in hashes:
     with open(os.path.join(dst, f"{name}_source_hash.txt"), "w") as fh:
-        fh.write(hashes.pop() + "  # sha256[:16] of csrc/*.hip,*.h at profile time (bench.py kernel_source_hash)\n")
+        fh.write(hashes.pop() + "  # sha256[:16] of the frame's sources and flags at profile time (bench.py kernel_source_hash)\n")
 pd.set_option("display.width", 200)
 print(stats.head(14).to_string())
 print(t.round(2).head(14).to_string())
