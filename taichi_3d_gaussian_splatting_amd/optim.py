@@ -25,8 +25,8 @@ class Adam(torch.optim.Optimizer):
         if lr < 0 or eps < 0 or not (0 <= betas[0] < 1 and 0 <= betas[1] < 1):
             raise ValueError("invalid Adam hyper-parameters")
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps))
-        self._scale_regulariser = {}   # id(param) -> (weight, point_invalid_mask)
-        self._row_mask = {}            # id(param) -> point_invalid_mask: rows of invalid points are skipped
+        self._scale_regulariser = {}   # param -> (weight, point_invalid_mask)
+        self._row_mask = {}            # param -> point_invalid_mask: rows of invalid points are skipped
 
     def set_row_mask(self, param: torch.Tensor, point_invalid_mask: torch.Tensor) -> None:
         """``param`` is a fixed-capacity [N,3] or [N,56] tensor with one row per point and ``point_invalid_mask`` (int8 [N],
@@ -40,7 +40,7 @@ class Adam(torch.optim.Optimizer):
             raise ValueError("set_row_mask: [N,3] or [N,56] parameter and an [N] mask")
         if point_invalid_mask.dtype != torch.int8:
             raise TypeError("point_invalid_mask must be int8")
-        self._row_mask[id(param)] = point_invalid_mask
+        self._row_mask[param] = point_invalid_mask
 
     def set_scale_regulariser(self, features: torch.Tensor, weight: float, point_invalid_mask: torch.Tensor,
                               local_share=None) -> None:
@@ -56,9 +56,9 @@ class Adam(torch.optim.Optimizer):
         if features.dim() != 2 or features.shape[1] != 56:
             raise ValueError("the scale regulariser applies to the [N,56] feature matrix")
         if weight:
-            self._scale_regulariser[id(features)] = (float(weight), point_invalid_mask, local_share)
+            self._scale_regulariser[features] = (float(weight), point_invalid_mask, local_share)
         else:
-            self._scale_regulariser.pop(id(features), None)
+            self._scale_regulariser.pop(features, None)
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -80,8 +80,8 @@ class Adam(torch.optim.Optimizer):
                     state["exp_avg"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
                     state["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
                 state["step"] = int(state["step"]) + 1
-                reg = self._scale_regulariser.get(id(p))
-                mask = self._row_mask.get(id(p))
+                reg = self._scale_regulariser.get(p)
+                mask = self._row_mask.get(p)
                 if mask is not None:
                     if reg is not None and reg[1] is not mask:
                         raise RuntimeError("set_row_mask and set_scale_regulariser were given different masks")
@@ -335,7 +335,7 @@ class AdamW(torch.optim.Optimizer):
         self.master_weights, self.max_grad_norm, self.norm_group = bool(master_weights), max_grad_norm, norm_group
         self.capturable, self.seed = bool(capturable), int(seed)
         self.last_grad_norm: Optional[torch.Tensor] = None
-        self._row_mask = {}            # id(param) -> point_invalid_mask
+        self._row_mask = {}            # param -> point_invalid_mask
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits))
 
     def set_row_mask(self, param: torch.Tensor, point_invalid_mask: torch.Tensor) -> None:
@@ -345,7 +345,7 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"set_row_mask: [N, 1..{MOMENT_BLOCK}] parameter and an [N] mask")
         if point_invalid_mask.dtype != torch.int8 or param.dtype != torch.float32:
             raise TypeError("set_row_mask: float32 parameter and int8 mask")
-        self._row_mask[id(param)] = point_invalid_mask
+        self._row_mask[param] = point_invalid_mask
 
     def _new_state(self, p: torch.Tensor, group: dict) -> dict:
         m, v, exponents = new_moments(p, group["state_bits"])
@@ -400,7 +400,7 @@ class AdamW(torch.optim.Optimizer):
                     state["step"] = count
             if masked:                  # (without a mask no row is late any more)
                 for p, state in zip(params, states):
-                    if id(p) not in self._row_mask:
+                    if p not in self._row_mask:
                         state.pop("last_step", None)
         return loss
 
@@ -417,7 +417,7 @@ class AdamW(torch.optim.Optimizer):
                 kept = [i for i, g in enumerate(grads) if g is not None]
                 params, grads, ids = ([column[i] for i in kept] for column in (params, grads, ids))
             states = [self.state[p] for p in params]
-            masks = [self._row_mask.get(id(p)) for p in params] if self._row_mask else [None] * len(params)
+            masks = [self._row_mask.get(p) for p in params] if self._row_mask else [None] * len(params)
             for i, (p, state, mask) in enumerate(zip(params, states, masks)):
                 if not state or (mask is not None and "last_step" not in state):
                     self._complete(p, state, mask, group)
@@ -477,7 +477,7 @@ class AdamW(torch.optim.Optimizer):
     _OPTIONS = ("master_weights", "max_grad_norm", "norm_group", "capturable", "seed", "last_grad_norm")
 
     def __getstate__(self) -> dict:
-        places = {id(p): i for i, p in enumerate(p for group in self.param_groups for p in group["params"])}
+        places = {p: i for i, p in enumerate(p for group in self.param_groups for p in group["params"])}
         return {**super().__getstate__(), **{name: getattr(self, name) for name in self._OPTIONS},
                 "row_masks": {places[i]: mask for i, mask in self._row_mask.items() if i in places}}
 
@@ -487,7 +487,7 @@ class AdamW(torch.optim.Optimizer):
         super().__setstate__(state)
         if masks is not None:       # (a copy or an unpickled optimiser; load_state_dict brings none)
             params = [p for group in self.param_groups for p in group["params"]]
-            self._row_mask = {id(params[i]): mask for i, mask in masks.items()}
+            self._row_mask = {params[i]: mask for i, mask in masks.items()}
 
     def load_state_dict(self, state_dict) -> None:
         """As in torch, hooks among it, but the state keeps its own types (torch would cast codes, counts and float32 moments of

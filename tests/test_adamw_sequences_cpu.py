@@ -226,3 +226,23 @@ def test_no_norm_stays_from_a_step_before_where_no_parameter_has_a_gradient():
     opt = optim.AdamW([p])
     opt.step()
     assert opt.last_grad_norm is None
+
+
+@pytest.mark.parametrize("kind", [optim.AdamW, optim.Adam])
+def test_a_mask_does_not_pass_on_to_a_parameter_that_takes_anothers_place(kind):
+    """Parameters are replaced where points are added and removed; a new object may have the address of the one that went."""
+    mask = torch.ones(4, dtype=torch.int8)
+    for _ in range(100):
+        opt = kind([torch.nn.Parameter(torch.zeros(4, 3))])
+        opt.set_row_mask(opt.param_groups[0]["params"][0], mask)
+        opt.param_groups[0]["params"][0] = None
+        q = torch.nn.Parameter(torch.zeros(4, 3))
+        opt.param_groups[0]["params"][0] = q
+        assert not any(key is q or key == id(q) for key in opt._row_mask)
+    # copies keep the masks of the parameters that are there
+    if kind is optim.AdamW:
+        import copy
+        opt.set_row_mask(q, mask)
+        twin = copy.deepcopy(opt)
+        (r,) = twin.param_groups[0]["params"]
+        assert [(key is r, bool(m.all())) for key, m in twin._row_mask.items()] == [(True, True)]
