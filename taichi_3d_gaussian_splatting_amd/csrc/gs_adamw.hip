@@ -56,9 +56,9 @@ enum Form : int {
 };
 // Passes of a lane over its workgroup's units, of a quad each, or of a pair where QUADS has pairs (ROWS has none)
 constexpr int passes(int quads, bool pair) { return pair ? (quads + 1) / 2 : quads; }
-// Lanes for a row of ROWS.  40M floats with 8-bit moments in rows of 5 / 8 / 17 / 24 / 45: 128 / 107 / 139 / 110 / 127 us (element by
+// Lanes for a row of ROWS.  40M floats with 8-bit moments in rows of 5 / 8 / 17 / 24 / 45: 128 / 107 / 144 / 112 / 128 us (element by
 // element 404 / 278 / 461 / 178 / 235; 16 lanes for all would idle most of them), rows of 56 as QUADS 113; all live under a mask
-// 205 / 134 / 159 / 121 / 139 (646 / 426 / 715 / 176 / 325), rows of 56 118.
+// 202 / 133 / 162 / 123 / 138 (646 / 426 / 715 / 176 / 325), rows of 56 118.
 __host__ __device__ constexpr int lanes_of(int row_len) { return row_len == 0 || row_len > 32 ? 16 : (row_len > 16 ? 8 : (row_len > 8 ? 4 : 2)); }
 
 struct AdamwTensor {
@@ -1006,9 +1006,9 @@ __global__ __launch_bounds__(GS_BLOCK) void read_moments_kernel(MomentsBatch b) 
 }
 
 // ------------------------------------------------------------------ norm of gradients
-// First pass: each workgroup adds the squares of one chunk in double precision (a float's square is exact there, so the
-// result does not depend on the order to within 1e-16) and leaves a partial sum; the second adds the partial sums in a
-// fixed order.
+// First pass: each workgroup adds the squares of one chunk in double precision (a float's square is exact there) and
+// leaves a partial sum; the second adds the partial sums.  The order is fixed, so equal inputs give equal bits; the sum of n squares is
+// off by n 2^-53 of itself at worst.
 struct NormTensor {
     const void *grad;
     u64 numel_type;             // numel * 4 + type

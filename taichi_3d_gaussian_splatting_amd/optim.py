@@ -145,7 +145,7 @@ def _on(device_index: int):
 
 
 def _stream(device_index: int) -> int:
-    """Handle of the current stream (``_lib.current_stream`` without the stream object: a step is 13 us in all)."""
+    """Handle of the current stream (``_lib.current_stream`` without the stream object: a small step is 7 us in all)."""
     return torch._C._cuda_getCurrentRawStream(device_index)
 
 
