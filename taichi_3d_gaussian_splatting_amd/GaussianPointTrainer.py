@@ -42,7 +42,7 @@ from .GaussianPointCloudRasterisation import GaussianPointCloudRasterisation
 from .GaussianPointCloudScene import GaussianPointCloudScene
 from .ImagePoseDataset import ImagePoseDataset
 from .LossFunction import LossFunction, ssim
-from .optim import Adam, AdamW
+from .optim import Adam, AdamW, _sum_over_ranks
 from .yaml_config import YAMLConfig
 
 _log = logging.getLogger(__name__)
@@ -391,7 +391,7 @@ class GaussianPointCloudTrainer:
         if cached is None or cached[0] != version:
             counts = (self.scene.point_invalid_mask == 0).sum().to(torch.float64).reshape(1)
             total = counts.clone()
-            torch.distributed.all_reduce(total)
+            _sum_over_ranks(total)
             cached = (version, float(counts.item()) / max(float(total.item()), 1.0))
             self._live_share_cache = cached
         return cached[1]
@@ -484,7 +484,7 @@ class GaussianPointCloudTrainer:
                                                                     self.scene.point_cloud_features)
                 if self.owner_sharded:   # mean over ALL live Gaussians: the blocks' means weighted by their share
                     reg_value = reg_value * self._local_live_share()
-                    torch.distributed.all_reduce(reg_value)
+                    _sum_over_ranks(reg_value)
                 loss = loss + reg_value
             raw_pred = image_pred.detach()
             image_pred = None   # the clamped CHW copy is only materialised on logging iterations (below)

@@ -175,7 +175,7 @@ def _norm_of(host, collected, grads, masks, max_norm: float, each: bool, group=N
     return out
 
 
-def _sum_over_ranks(value: torch.Tensor, group) -> None:
+def _sum_over_ranks(value: torch.Tensor, group=None) -> None:
     import torch.distributed as dist
     if dist.get_backend(group) == "nccl":
         dist.all_reduce(value, group=group)

@@ -113,3 +113,20 @@ def _owner(rank, world, port):
 
 def test_gradient_over_owners_is_that_of_all_live_points():
     mp.spawn(_owner, args=(2, _free_port()), nprocs=2, join=True)
+
+
+@pytest.mark.parametrize("backend", ["gloo", "nccl"])
+def test_live_share_hands_device_memory_to_back_ends_that_take_it(monkeypatch, backend):
+    """(a sum over two ranks that hold the same: doubled)"""
+    features, mask, _ = _scene()
+    trainer = _trainer(features, mask, owner_sharded=True)
+    handed = []
+
+    def all_reduce(value, *args, **kwargs):
+        handed.append(value.device.type)
+        value *= 2
+    monkeypatch.setattr(dist, "get_backend", lambda group=None: backend)
+    monkeypatch.setattr(dist, "all_reduce", all_reduce)
+    assert trainer._local_live_share() == 0.5
+    assert handed == ["cpu" if backend == "gloo" else "cuda"]
+    assert trainer._local_live_share() == 0.5 and len(handed) == 1      # (kept while the live set stays)
