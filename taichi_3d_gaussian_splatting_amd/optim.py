@@ -261,20 +261,19 @@ def adamw_step_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], e
     if grad_scale is not None and (grad_scale.get_device() != index or grad_scale.dtype is not torch.float32 or grad_scale.numel() != 1):
         raise ValueError("grad_scale: one float32 on the parameters' device")
     numbers = host.scalars(n, step, lr, weight_decay, beta1, beta2, eps, index)
-    if numbers[4] and _capturing(index):
-        raise RuntimeError("a captured step needs its step count in a device tensor: a number would be the same at every replay")
-
     norms, clip = None, 0
-    if max_grad_norm is not None:
-        norms = _norm_of(host, collected, columns[1], columns[6], float(max_grad_norm), False, norm_group)
-        clip = norms.data_ptr() + 4
-    elif grad_scale is not None:
-        clip = grad_scale.data_ptr()
-    workspace, workspace_at = None, 0
-    if numbers[2] is not None or numbers[3] is not None:
-        workspace = torch.empty(int(_lib.load().gs_adamw_workspace_bytes(n)), dtype=torch.uint8, device=torch.device("cuda", index))
-        workspace_at = workspace.data_ptr()
     with _on(index):
+        if numbers[4] and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a captured step needs its step count in a device tensor: a number would be the same at every replay")
+        if max_grad_norm is not None:
+            norms = _norm_of(host, collected, columns[1], columns[6], float(max_grad_norm), False, norm_group)
+            clip = norms.data_ptr() + 4
+        elif grad_scale is not None:
+            clip = grad_scale.data_ptr()
+        workspace, workspace_at = None, 0
+        if numbers[2] is not None or numbers[3] is not None:
+            workspace = torch.empty(int(_lib.load().gs_adamw_workspace_bytes(n)), dtype=torch.uint8, device=torch.device("cuda", index))
+            workspace_at = workspace.data_ptr()
         check(host.step(collected, numbers, tensor_ids, clip, seed & 0xFFFFFFFF, workspace_at, _stream(index)), "gs_adamw_step")
     return None if norms is None else norms[0]
 
@@ -418,11 +417,13 @@ class AdamW(torch.optim.Optimizer):
                 params, grads, ids = ([column[i] for i in kept] for column in (params, grads, ids))
             states = [self.state[p] for p in params]
             masks = [self._row_mask.get(p) for p in params] if self._row_mask else [None] * len(params)
-            for i, (p, state, mask) in enumerate(zip(params, states, masks)):
-                if not state or (mask is not None and "last_step" not in state):
-                    self._complete(p, state, mask, group)
-                elif mask is None and "last_step" in state:
-                    masks[i] = self._no_row_masked(p)
+            for i, state in enumerate(states):
+                if state and (masks[i] is None) != ("last_step" in state):
+                    continue
+                if state and masks[i] is None:
+                    masks[i] = self._no_row_masked(params[i])
+                else:
+                    self._complete(params[i], state, masks[i], group)
             kinds = [("exponents" in s, p.get_device()) for p, s in zip(params, states)]
             for kind in sorted(set(kinds)):
                 columns = params, grads, states, masks, ids
